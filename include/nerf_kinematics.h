@@ -80,7 +80,7 @@ typedef struct nk_step_state {
     int32_t  view;                /* index into the camera table / image stack             */
     float    adam_step_size;      /* (float)(lr / (1 - beta1^step))                        */
     float    adam_bc2_sqrt;       /* (float)sqrt(1 - beta2^step)                           */
-    int32_t  reserved;
+    float    adamw_decay;         /* nk_adamw_step: (float)(lr * weight_decay), 0 = none   */
 } nk_step_state;
 
 /* Formats of the tensors a training forward saves for backward (nk_render_opts.act_format).
@@ -209,6 +209,48 @@ int nk_mse_loss(const float* rgb_coarse, const float* rgb_fine, const float* tar
 int nk_adam_step(float* params, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t n,
                  int64_t step, double lr, double beta1, double beta2, double eps, float grad_scale,
                  void* stream);
+
+/* Element types of the operators below that take more than fp32. */
+enum { NK_F32 = 0, NK_BF16 = 1, NK_F16 = 2 };
+
+/* AdamW (torch.optim.AdamW's update, decoupled weight decay) over many tensors in one launch per 56 of
+ * them.  No counterpart in the reference, whose optimiser is Adam on fp32 parameters.
+ *   param       n elements of opts->param_dtype, updated in place
+ *   master      NULL, or n fp32 values: then these are what the step updates, and param receives a copy
+ *               rounded to its type (low-precision parameters without a master lose updates smaller
+ *               than half their last place)
+ *   exp_avg, exp_avg_sq   state_bits 32: n fp32 values each.  state_bits 8: n bytes each, OCP e4m3 and OCP
+ *               e5m2 codes, worth code * scale_m[i / 256] and code * scale_v[i / 256]; the scales are powers
+ *               of two, ceil(n / 256) fp32 values each (all zero = zero moments).  Codes are rounded
+ *               stochastically with bits of RNG stream 5 (`seed`, index of the element in its tensor).
+ *               A block of 256 that meets an infinity or a NaN decodes to NaN from then on.
+ * Buffers may have any alignment their element type allows (16-byte aligned ones are faster); they must not
+ * overlap.  Tensors with n = 0 are skipped.                                                          */
+typedef struct nk_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* master;
+    float* scale_m;
+    float* scale_v;
+    int64_t n;
+} nk_adamw_tensor;
+typedef struct nk_adamw_opts {
+    int32_t param_dtype;          /* NK_F32 | NK_BF16 | NK_F16                                 */
+    int32_t grad_dtype;           /* NK_F32, or the same as param_dtype                       */
+    int32_t state_bits;           /* 32 | 8                                                   */
+    uint32_t seed;                /* of the stochastic rounding (state_bits 8)                */
+    int64_t step;                 /* this step's number, from 1                               */
+    double  lr, beta1, beta2, eps, weight_decay;
+    float   grad_scale;           /* the gradient is multiplied by this first                 */
+    int32_t reserved;
+    const nk_step_state* state;   /* device pointer or NULL; when set, step, lr, weight_decay and seed are
+                                     ignored and adam_step_size, adam_bc2_sqrt, adamw_decay and render_seed
+                                     of *state are read when the kernel runs (graph replay)    */
+} nk_adamw_opts;
+int nk_adamw_step(const nk_adamw_tensor* tensors /*host*/, int32_t count, const nk_adamw_opts* opts /*host*/,
+                  void* stream);
 
 /* *state_dev = *state_host, stream-ordered: the struct travels as a kernel argument (copied at the
  * call), so the host copy may be overwritten as soon as the call returns.                      */

@@ -29,7 +29,7 @@ void nk_set_error(const char* fmt, ...);
 
 // ---- counter-based RNG: 32 bits for element idx of a stream under a seed --------------------
 enum { NK_STREAM_STRATIFIED = 0, NK_STREAM_PDF = 1, NK_STREAM_NOISE_COARSE = 2,
-       NK_STREAM_NOISE_FINE = 3, NK_STREAM_PIXELS = 4 };
+       NK_STREAM_NOISE_FINE = 3, NK_STREAM_PIXELS = 4, NK_STREAM_OPTIMISER = 5 };
 
 NK_HD uint32_t nk_lowbias32(uint32_t x) {
     x ^= x >> 16; x *= 0x7FEB352Du; x ^= x >> 15; x *= 0x846CA68Bu; x ^= x >> 16;

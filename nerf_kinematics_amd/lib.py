@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # NK_LIB (development only): another build of the library, e.g. to compare two builds bit by bit
 LIB_PATH = os.environ.get("NK_LIB") or os.path.join(_HERE, "libnerfkin.so")
@@ -23,7 +25,7 @@ PAIR_GEMM_MAX_POINTS = 1 << 20
 # nk_render_opts.act_format: formats of the tensors saved for backward (experiments beyond bf16)
 ACT_FORMATS = {"bf16": 0, "fp8": 1, "fp8bf8": 2}
 
-STREAM_STRATIFIED, STREAM_PDF, STREAM_NOISE_COARSE, STREAM_NOISE_FINE, STREAM_PIXELS = 0, 1, 2, 3, 4
+STREAM_STRATIFIED, STREAM_PDF, STREAM_NOISE_COARSE, STREAM_NOISE_FINE, STREAM_PIXELS, STREAM_OPTIMISER = 0, 1, 2, 3, 4, 5
 
 
 ABI_VERSION = 103          # nk_version() of the library these ctypes declarations describe
@@ -37,7 +39,7 @@ class NkArch(C.Structure):
 class NkStepState(C.Structure):
     """Per-iteration scalars of a training step, read by the kernels from device memory (graph replay)."""
     _fields_ = [("render_seed", C.c_uint32), ("pixel_seed", C.c_uint32), ("pixel_counter", C.c_uint64),
-                ("view", C.c_int32), ("adam_step_size", C.c_float), ("adam_bc2_sqrt", C.c_float), ("reserved", C.c_int32)]
+                ("view", C.c_int32), ("adam_step_size", C.c_float), ("adam_bc2_sqrt", C.c_float), ("adamw_decay", C.c_float)]
 
 
 class NkRenderOpts(C.Structure):
@@ -58,6 +60,19 @@ class NkRenderOut(C.Structure):
                                           "rgb_coarse", "disp_coarse", "acc_coarse", "depth_coarse")]
 
 
+class NkAdamwTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "master", "scale_m", "scale_v")] + [("n", C.c_int64)]
+
+
+class NkAdamwOpts(C.Structure):
+    _fields_ = [("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("state_bits", C.c_int32), ("seed", C.c_uint32),
+                ("step", C.c_int64), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("grad_scale", C.c_float), ("reserved", C.c_int32), ("state", C.c_void_p)]
+
+
+# element types of the operators that take more than fp32 (NK_F32, NK_BF16, NK_F16)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 # name -> (restype, argtypes); every symbol include/nerf_kinematics.h declares
 _P, _I64, _I32, _F = C.c_void_p, C.c_int64, C.c_int32, C.c_float
 _PA, _PO, _PC, _PR = C.POINTER(NkArch), C.POINTER(NkRenderOpts), C.POINTER(NkCamera), C.POINTER(NkRenderOut)
@@ -72,6 +87,7 @@ SIGNATURES = {
     "nk_sample_training_rays_dev": (C.c_int, [_P, _I32, _P, _I64, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
     "nk_set_step_state": (C.c_int, [C.POINTER(NkStepState), _P, _P]),
     "nk_adam_step_dev": (C.c_int, [_P, _P, _P, _P, _I64, _P, C.c_double, C.c_double, C.c_double, _F, _P]),
+    "nk_adamw_step": (C.c_int, [C.POINTER(NkAdamwTensor), _I32, C.POINTER(NkAdamwOpts), _P]),
     "nk_stratified_z": (C.c_int, [_P, _I64, _PO, _P, _P]),
     "nk_act_bytes": (_I64, [_PA, _I64, _I32]),
     "nk_mlp_forward": (C.c_int, [_PA, _P, _P, _P, _I64, _I32, _P, _P, _P]),

@@ -1,0 +1,188 @@
+"""AdamW over many tensors in one launch (``nk_adamw_step``), with 32-bit or 8-bit moments.
+
+Stands beside :func:`~nerf_kinematics_amd.render.adam_step` (Adam on flat fp32 buffers, the optimiser of
+the reference's checkpoints).  ``adamw_step`` updates lists of tensors once; :class:`AdamW` keeps the
+moments of a list of parameters and the launch table a program reuses.  Everything runs on the current
+torch stream of the tensors' GPU; bad shapes, types or overlaps raise ``ValueError`` before any launch.
+
+8-bit moments: blocks of 256 consecutive elements of a tensor share a power-of-two fp32 scale; an element
+is ``code * scale`` with an OCP e4m3 code (first moment) or e5m2 code (second moment).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import lib as _lib
+
+BLOCK = 256                       # elements that share a scale in an 8-bit moment
+MOMENT_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
+_TENSOR_WORDS = C.sizeof(_lib.NkAdamwTensor) // 8
+
+
+def _check_list(name: str, tensors: Sequence[torch.Tensor], like: Sequence[torch.Tensor], dtype: torch.dtype, device) -> None:
+    if len(tensors) != len(like):
+        raise ValueError(f"{name}: {len(tensors)} tensors for {len(like)} parameters")
+    for i, (t, p) in enumerate(zip(tensors, like)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+            raise ValueError(f"{name}[{i}]: expected a {dtype} tensor on {device}")
+        if t.numel() != p.numel():
+            raise ValueError(f"{name}[{i}]: {t.numel()} elements, the parameter has {p.numel()}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}[{i}]: must be contiguous")
+
+
+def _check_disjoint(tensors: List[torch.Tensor]) -> None:
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise ValueError("parameters, masters and moments must not overlap in memory (the same tensor twice?)")
+
+
+def adamw_state(params: Sequence[torch.Tensor], state_bits: int = 32):
+    """Zero moments for ``params``: ``(exp_avgs, exp_avg_sqs, scales)``; ``scales`` is None for 32-bit moments
+    and a list of ``(scale_m, scale_v)`` pairs, one value per block of 256 elements, for 8-bit ones."""
+    if state_bits not in MOMENT_DTYPES:
+        raise ValueError(f"state_bits={state_bits}: 32 or 8")
+    dm, dv = MOMENT_DTYPES[state_bits]
+    m = [torch.zeros(p.numel(), dtype=dm, device=p.device) for p in params]
+    v = [torch.zeros(p.numel(), dtype=dv, device=p.device) for p in params]
+    if state_bits == 32:
+        return m, v, None
+    mk = lambda p: torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
+    return m, v, [(mk(p), mk(p)) for p in params]
+
+
+def decode_moment(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """fp32 values of an 8-bit moment (a host-side helper for checkpoints)."""
+    n = codes.numel()
+    return codes.reshape(-1).float() * scale.repeat_interleave(BLOCK)[:n]
+
+
+def encode_moment(values: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of fp32 values, rounded to nearest (a host-side helper for checkpoints); values
+    that ``decode_moment`` gave come back as the same values."""
+    top = {torch.float8_e4m3fn: 8, torch.float8_e5m2: 15}[dtype]
+    n = values.numel()
+    b = torch.nn.functional.pad(values.reshape(-1).float(), (0, -n % BLOCK)).view(-1, BLOCK)
+    frac, e = torch.frexp(b.abs().amax(1, keepdim=True))
+    e = torch.where(frac == 0, torch.full_like(e, -100), e - (frac == 0.5).to(e.dtype) - top).clamp_min(-100)
+    scaled = torch.ldexp(b, -e)
+    codes = scaled.to(dtype)
+    if dtype == torch.float8_e5m2:       # a second moment stays positive
+        least = torch.full_like(scaled, 2.0 ** -16).to(dtype)
+        codes = torch.where((scaled > 0) & (codes.float() == 0), least.view(torch.uint8), codes.view(torch.uint8)).view(dtype)
+    return codes.reshape(-1)[:n].clone(), torch.ldexp(torch.ones_like(b[:, 0]), e[:, 0])
+
+
+class AdamW:
+    """torch.optim.AdamW's update for a list of parameters, updated in place by one launch per 56 tensors.
+
+    ``params``: contiguous GPU tensors of one dtype (fp32, bf16 or fp16) on one device.  ``masters``: fp32
+    copies that the step updates instead, the parameters then receive them rounded; low-precision
+    parameters without masters lose updates below half their last place.  ``state_bits``: 32 or 8.
+    ``state``: moments to continue from, as ``adamw_state`` lays them out (their dtype decides the format)."""
+
+    def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, masters: Optional[Sequence[torch.Tensor]] = None,
+                 state=None, seed: int = 0):
+        self._L = _lib.load()
+        self._sources = list(params)
+        params = [p.detach() for p in params]
+        if not params:
+            raise ValueError("AdamW: no parameters")
+        dt, dev = params[0].dtype, params[0].device
+        if dt not in _lib.DTYPES:
+            raise ValueError(f"AdamW: parameters of dtype {dt} (float32, bfloat16 or float16)")
+        if dev.type != "cuda":
+            raise ValueError("AdamW: expected GPU tensors (there is no CPU implementation)")
+        _check_list("params", params, params, dt, dev)
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+            raise ValueError(f"AdamW: betas={tuple(betas)} in [0, 1), eps={eps} >= 0 wanted")
+        if masters is not None:
+            _check_list("masters", masters, params, torch.float32, dev)
+        if state is None:
+            state = adamw_state(params, state_bits)
+        m, v, scales = state
+        if not m or m[0].dtype not in (torch.float32, torch.float8_e4m3fn):
+            raise ValueError("AdamW: moments are float32 or float8_e4m3fn / float8_e5m2")
+        state_bits = 32 if m[0].dtype == torch.float32 else 8
+        _check_list("exp_avgs", m, params, MOMENT_DTYPES[state_bits][0], dev)
+        _check_list("exp_avg_sqs", v, params, MOMENT_DTYPES[state_bits][1], dev)
+        flat_scales: List[torch.Tensor] = []
+        if state_bits == 8:
+            if scales is None or len(scales) != len(params):
+                raise ValueError("AdamW: 8-bit moments need one (scale_m, scale_v) pair per parameter")
+            for i, (p, pair) in enumerate(zip(params, scales)):
+                for s in pair:
+                    if s.dtype != torch.float32 or s.device != dev or not s.is_contiguous() or s.numel() != -(-p.numel() // BLOCK):
+                        raise ValueError(f"AdamW: scales[{i}]: expected {-(-p.numel() // BLOCK)} contiguous float32 values on {dev}")
+                flat_scales += pair
+        elif scales is not None:
+            raise ValueError("AdamW: scales belong to 8-bit moments")
+        _check_disjoint(params + list(m) + list(v) + list(masters or []) + flat_scales)
+        self.params, self.masters, self.exp_avgs, self.exp_avg_sqs, self.scales = params, masters, m, v, scales
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
+        self.device = dev
+        self._table = (_lib.NkAdamwTensor * len(params))()
+        for i, p in enumerate(params):
+            sm, sv = scales[i] if scales is not None else (None, None)
+            self._table[i] = _lib.NkAdamwTensor(p.data_ptr(), None, m[i].data_ptr(), v[i].data_ptr(),
+                                                masters[i].data_ptr() if masters is not None else None,
+                                                sm.data_ptr() if sm is not None else None,
+                                                sv.data_ptr() if sv is not None else None, p.numel())
+        # the `grad` words of the table, one per tensor
+        self._grads = (C.c_int64 * (_TENSOR_WORDS * len(params))).from_buffer(self._table)
+        self._numels = [p.numel() for p in params]
+        self._opts = _lib.NkAdamwOpts()
+        self._opts.param_dtype, self._opts.state_bits = _lib.DTYPES[dt], state_bits
+        self._opts.beta1, self._opts.beta2, self._opts.eps = self.betas[0], self.betas[1], self.eps
+
+    def step(self, grads: Optional[Sequence[torch.Tensor]] = None, *, lr: Optional[float] = None, step: Optional[int] = None,
+             grad_scale: float = 1.0, seed: Optional[int] = None, step_state: Optional[int] = None) -> None:
+        """One update.  ``grads``: one contiguous tensor per parameter, all fp32 or all of the parameters' dtype
+        (default: the parameters' ``.grad``, which must exist).  ``step`` (from 1; default: one more than the
+        last) sets the bias corrections, ``seed`` the stochastic rounding of 8-bit moments (default: the
+        optimiser's, moved on by the step).  ``step_state``: device address of an ``nk_step_state`` to read the
+        step-dependent scalars from when the kernel runs (graph replay)."""
+        n = len(self.params)
+        if grads is None:
+            grads = [p.grad for p in self._sources]
+            if any(g is None for g in grads):
+                raise ValueError("AdamW.step: a parameter has no .grad")
+        if len(grads) != n:
+            raise ValueError(f"grads: {len(grads)} tensors for {n} parameters")
+        gd, dev, words, numels = grads[0].dtype, self.device, self._grads, self._numels
+        if gd != torch.float32 and gd != self.params[0].dtype:
+            raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self.params[0].dtype})")
+        for i, g in enumerate(grads):
+            if g.dtype != gd or g.numel() != numels[i] or g.device != dev or not g.is_contiguous():
+                raise ValueError(f"grads[{i}]: expected {numels[i]} contiguous {gd} values on {dev}")
+            words[_TENSOR_WORDS * i + 1] = g.data_ptr()
+        step = self.steps + 1 if step is None else int(step)
+        if step < 1:
+            raise ValueError(f"step={step}: from 1")
+        o = self._opts
+        o.grad_dtype, o.step, o.lr, o.weight_decay = _lib.DTYPES[gd], step, self.lr if lr is None else float(lr), self.weight_decay
+        o.grad_scale = float(grad_scale)
+        o.seed = (self.seed + 0x9E3779B1 * step if seed is None else int(seed)) & 0xFFFFFFFF
+        o.state = step_state
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if torch.cuda.current_device() == dev.index:
+            _lib.check(self._L.nk_adamw_step(self._table, n, o, stream))
+        else:
+            with torch.cuda.device(dev):
+                _lib.check(self._L.nk_adamw_step(self._table, n, o, stream))
+        self.steps = step
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, *, scales=None, masters: Optional[Sequence[torch.Tensor]] = None,
+               grad_scale: float = 1.0, seed: int = 0) -> None:
+    """One AdamW update of ``params`` in place (see :class:`AdamW` for the arguments)."""
+    AdamW(params, lr, betas, eps, weight_decay, masters=masters, state=(exp_avgs, exp_avg_sqs, scales)).step(
+        grads, step=step, grad_scale=grad_scale, seed=seed)
