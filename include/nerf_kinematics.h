@@ -213,6 +213,41 @@ int nk_adam_step(float* params, const float* grad, float* exp_avg, float* exp_av
 /* Element types of the operators below that take more than fp32. */
 enum { NK_F32 = 0, NK_BF16 = 1, NK_F16 = 2 };
 
+/* Gated linear recurrence along axis T of x [B, T, C], forward and backward:
+ *     h_t = a_t * h_(t-1) + x_t        (reverse: h_t = a_t * h_(t+1) + x_t, from the last step to the first)
+ * a is [B, T, gates]; gate j is shared by the C / gates consecutive channels from j * C / gates on.  The
+ * front-to-back compositing of raw2outputs is the case a = 1 - alpha, x = alpha * colour, reverse, one gate.
+ * States and sums are fp32; h is rounded once to its type.  h0 [B, C] (NULL = zero) is the state before the
+ * first step, h_last [B, C] (NULL = unwanted) the one after the last.  Gates are meant to decay (|a| <= 1);
+ * growing ones work as long as the product of the gates over any stretch stays in the range of fp32.
+ *   lengths   NULL, or B device ints: sequence b has clamp(lengths[b], 0, T) steps.  Rows behind it are not read;
+ *             the outputs there (h, d_a, d_x) are zero, and a reversed sequence starts at its own last step.
+ * a, x and d_h may be strided over B and T, with unit channel stride; strides
+ * in elements, zero allowed.  h, d_a and d_x are contiguous.                                         */
+typedef struct nk_scan_opts {
+    int64_t B, T, C, gates;
+    int32_t dtype;                /* of x, h, d_h, d_x: NK_F32 | NK_BF16 | NK_F16              */
+    int32_t gate_dtype;           /* of a, d_a: the same, or NK_F32                           */
+    int32_t reverse;
+    int32_t reserved;
+    int64_t a_stride_b, a_stride_t, x_stride_b, x_stride_t;
+    int64_t g_stride_b, g_stride_t;       /* of d_h (backward call)                       */
+    const int32_t* lengths;       /* device, or NULL                                          */
+} nk_scan_opts;
+/* 256-byte aligned scratch either call may need (it holds nothing between calls); 0 is common. */
+int64_t nk_gated_scan_workspace_bytes(const nk_scan_opts* opts /*host*/, int backward);
+/* states: NULL, or nk_gated_scan_states_bytes() bytes that receive the fp32 state in front of every 32nd step
+ * for the backward call.                                                                             */
+int64_t nk_gated_scan_states_bytes(const nk_scan_opts* opts /*host*/);
+int nk_gated_scan_fwd(const nk_scan_opts* opts /*host*/, const void* a, const void* x, const float* h0, void* h,
+                      float* h_last, float* states, void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients from d_h (NULL = zero) and d_h_last (NULL = zero); a, x, h0, lengths and states as in the forward
+ * call (x and states may be NULL when d_a is).  d_a, d_x and d_h0 are written, not accumulated; each
+ * may be NULL when unwanted.  d_a sums over the channels of its gate in a fixed order.               */
+int nk_gated_scan_bwd(const nk_scan_opts* opts /*host*/, const void* a, const void* x, const float* states,
+                      const float* h0, const void* d_h, const float* d_h_last, void* d_a, void* d_x, float* d_h0,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 /* AdamW (torch.optim.AdamW's update, decoupled weight decay) over many tensors in one launch per 56 of
  * them.  No counterpart in the reference, whose optimiser is Adam on fp32 parameters.
  *   param       n elements of opts->param_dtype, updated in place

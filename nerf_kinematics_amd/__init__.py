@@ -9,6 +9,7 @@ from .model import Arch, NeRFModel, ARCH_RUN_NERF, ARCH_LEGO_CKPT, ARCH_WHEEL_CK
 from .render import (get_rays, stratified_z, run_network, raw2outputs, raw2outputs_backward,  # noqa: F401
                      sample_pdf, render_rays, make_opts, alloc_activations, mlp_backward, mse_loss,
                      adam_step)
+from .scan import gated_scan  # noqa: F401
 from .optim import AdamW, adamw_state, adamw_step, decode_moment, encode_moment  # noqa: F401
 
 __version__ = "0.1.0"

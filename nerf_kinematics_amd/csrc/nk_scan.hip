@@ -1,0 +1,754 @@
+// Gated linear recurrence along a long axis and its backward pass.
+//
+//   forward    h_s = a_s h_(s-1) + x_s,   h_(-1) = h0                       (s: order of processing)
+//   backward   d_s = g_s + e_(s+1),  e_s = a_s d_s,  e_(len) = d_last       (g = dL/dh)
+//              dL/dx_s = d_s,  dL/da_s = sum over the channels of a gate of d_s h_(s-1),  dL/dh0 = e_0
+//
+// Both directions are compositions of maps s -> A s + H, which are associative: the steps of a column (one
+// channel, or four neighbouring ones, of one sequence) are cut into runs, each run is reduced to its (A, H),
+// the (A, H) of the runs in front are composed onto the state at the start, and every run is then walked
+// again from its own start state, out of registers.  State, products and sums are fp32 throughout.
+//
+// A workgroup holds 2^LC columns x (256 >> LC) runs of SC_U steps ("a tile") and walks along the sequence
+// tile by tile, so every input is read once.  The forward pass of a training step keeps the fp32 state in
+// front of every 32nd step; the backward pass walks the tiles from the last to the first and rebuilds the
+// states inside a tile from these and x, which costs no more bytes than reading h and keeps dL/da free
+// of the rounding of h.
+//
+// Where there are too few columns to fill the chip the sequence itself is cut into stretches (grid.y): a
+// first launch reduces every stretch to its (A, H), the second composes those in front of its own and walks.
+#include "nk_common.h"
+
+namespace {
+
+enum { SC_THREADS = 256, SC_U = 8, SC_KEEP = 32 };
+#ifndef NK_SCAN_LC
+#define NK_SCAN_LC 4
+#endif
+#ifndef NK_SCAN_FEW
+#define NK_SCAN_FEW 512
+#endif
+#ifndef NK_SCAN_FILL
+#define NK_SCAN_FILL 1024
+#endif
+#ifndef NK_SCAN_CACHE
+#define NK_SCAN_CACHE 96
+#endif
+
+struct ScanArgs {
+    const void* a; const void* x; const void* g;    // g: dL/dh (backward)
+    const float* h0; const float* first;            // first: state the walk starts from (h0, d_last, or what the block before left)
+    void* o; void* d_a;                             // o: h or dL/dx
+    float* last;                                    // state behind the walk (h_last, dL/dh0)
+    float* states;                                  // [B][ceil(T / 32)][C]: state in front of step 32 k
+    float* sums;                                    // [stretch][2][columns * VC]: A, H of every stretch
+    float* gate_part;                               // [part][B * T * J]: partial sums of dL/da of a wide gate
+    const int32_t* lengths;
+    int64_t C, a_sb, a_st, x_sb, x_st, g_sb, g_st;
+    int64_t cols, B, J;
+    int32_t T, begin, end, stretch;                 // steps [begin, end) of this launch, steps per stretch
+    int32_t G, LG, per_b, LC, reverse;              // channels per gate, columns per gate, columns per sequence
+};
+
+template <typename T, int VC> struct Pack { T v[VC]; };
+template <typename T, int VC> NK_D Pack<T, VC> ld(const T* p) {
+    Pack<T, VC> r;
+    if constexpr (VC == 1) r.v[0] = *p;
+    else {
+        typedef __attribute__((ext_vector_type(VC))) T vec;
+        const vec w = *(const vec*)p;
+#pragma unroll
+        for (int k = 0; k < VC; ++k) r.v[k] = w[k];
+    }
+    return r;
+}
+template <typename T, int VC> NK_D void st(T* p, const float* v) {
+    if constexpr (VC == 1) *p = (T)v[0];
+    else {
+        typedef __attribute__((ext_vector_type(VC))) T vec;
+        vec w;
+#pragma unroll
+        for (int k = 0; k < VC; ++k) w[k] = (T)v[k];
+        *(vec*)p = w;
+    }
+}
+
+// A s + H on a state; a state of exactly zero gives H even where the product of the gates has left the
+// range of fp32
+NK_D float apply(float A, float H, float s) { return s == 0.0f ? H : fmaf(A, s, H); }
+
+// What a thread works on: its column and which run of a tile.
+struct Place {
+    int64_t b, c, gate, col;    // sequence, first channel, gate, column
+    int k;                      // which column of the gate
+    int run;
+    int len;                    // live steps of the sequence; 0 for columns that only round a gate up
+    bool on;                    // has channels
+};
+template <int VC, bool SHARED> NK_D Place place(const ScanArgs& A) {
+    Place p;
+    const int lcol = 1 << A.LC;
+    p.run = threadIdx.x >> A.LC;
+    p.col = (int64_t)blockIdx.x * lcol + (threadIdx.x & (lcol - 1));
+    p.b = p.col / A.per_b;
+    const int r = (int)(p.col - p.b * A.per_b);
+    p.on = p.col < A.cols;
+    if (SHARED) {
+        const int j = r / A.LG;
+        p.k = r - j * A.LG;
+        p.gate = j; p.c = (int64_t)j * A.G + (int64_t)p.k * VC;
+        p.on = p.on && p.k * VC < A.G;
+    } else {
+        p.k = 0; p.c = (int64_t)r * VC; p.gate = p.c;
+    }
+    p.len = !p.on ? 0 : A.lengths ? max(0, min(A.T, A.lengths[p.b])) : A.T;
+    return p;
+}
+
+// Steps s0 .. s0 + SC_U - 1 of a column; `fill` where s reaches `lim`.  base: the row of step s0.
+template <typename T, int VC>
+NK_D void fetch(Pack<T, VC> (&r)[SC_U], const T* base, int64_t step, int s0, int lim, float fill) {
+    if (__all(s0 + SC_U <= lim)) {
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u) r[u] = ld<T, VC>(base + u * step);
+    } else {
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u) {
+#pragma unroll
+            for (int v = 0; v < VC; ++v) r[u].v[v] = (T)fill;
+            if (s0 + u < lim) r[u] = ld<T, VC>(base + u * step);
+        }
+    }
+}
+// row of step s of a sequence of len steps
+NK_D int64_t time_of(int s, int len, int reverse) { return reverse ? len - 1 - s : s; }
+
+// Largest live length of the workgroup's columns.
+NK_D int longest(const Place& p, const ScanArgs& A) {
+    if (!A.lengths) return A.T;
+    __shared__ int most;
+    if (threadIdx.x == 0) most = 0;
+    __syncthreads();
+    if (p.len > 0) atomicMax(&most, p.len);
+    __syncthreads();
+    return most;
+}
+
+template <int VC> struct Buf { float v[4][3 * VC][64]; };
+
+// Runs of a tile in ascending order.  In: (Ar, Hr) of this thread's run and `carry`, the state in front of the
+// tile.  Out: s, the state in front of this run; carry, the one behind the tile.  Runs of one wavefront are
+// composed with lane shuffles, wavefronts through LDS (`buf` alternates, so one barrier a tile is enough).
+template <int VC>
+NK_D void compose_up(const float* Ain, const float* Hin, float* carry, float* s, int LC, Buf<VC>& buf) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lcol = 1 << LC, cl = lane & (lcol - 1);
+    if (LC == 8) {          // every thread has a column of its own
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { s[v] = carry[v]; carry[v] = apply(Ain[v], Hin[v], carry[v]); }
+        return;
+    }
+    float Ar[VC], Hr[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) { Ar[v] = Ain[v]; Hr[v] = Hin[v]; }
+    for (int off = lcol; off < 64; off <<= 1) {         // inclusive over the runs of the wavefront
+#pragma unroll
+        for (int v = 0; v < VC; ++v) {
+            const float A0 = __shfl_up(Ar[v], off, 64), H0 = __shfl_up(Hr[v], off, 64);
+            if (lane >= off) { Hr[v] = apply(Ar[v], Hr[v], H0); Ar[v] *= A0; }
+        }
+    }
+    if (LC >= 6 || lane >= 64 - lcol) {
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { buf.v[wave][v][cl] = Ar[v]; buf.v[wave][VC + v][cl] = Hr[v]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < VC; ++v) {
+        float c = carry[v];
+        s[v] = c;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            c = apply(buf.v[w][v][cl], buf.v[w][VC + v][cl], c);
+            if (w + 1 == wave) s[v] = c;
+        }
+        carry[v] = c;
+        if (LC < 6) {
+            const float A0 = __shfl_up(Ar[v], lcol, 64), H0 = __shfl_up(Hr[v], lcol, 64);
+            if (lane >= lcol) s[v] = apply(A0, H0, s[v]);
+        }
+    }
+}
+
+// The backward pass's two compositions with one barrier: (A, H) ascending from the kept state `hs` in front of
+// the tile (out: h, the state in front of this run), and (A, E) descending from `carry` behind the tile
+// (out: e, what this run starts from; carry, in front of the tile).
+template <int VC>
+NK_D void compose_both(const float* Ain, const float* Hin, const float* Ein, const float* hs, float* carry, float* h, float* e,
+                       int LC, Buf<VC>& buf) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lcol = 1 << LC, cl = lane & (lcol - 1);
+    if (LC == 8) {
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { h[v] = hs[v]; e[v] = carry[v]; carry[v] = apply(Ain[v], Ein[v], carry[v]); }
+        return;
+    }
+    float Au[VC], Hr[VC], Ad[VC], Er[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) { Au[v] = Ad[v] = Ain[v]; Hr[v] = Hin[v]; Er[v] = Ein[v]; }
+    for (int off = lcol; off < 64; off <<= 1) {
+#pragma unroll
+        for (int v = 0; v < VC; ++v) {
+            const float A0 = __shfl_up(Au[v], off, 64), H0 = __shfl_up(Hr[v], off, 64);
+            const float A1 = __shfl_down(Ad[v], off, 64), E1 = __shfl_down(Er[v], off, 64);
+            if (lane >= off) { Hr[v] = apply(Au[v], Hr[v], H0); Au[v] *= A0; }
+            if (lane + off < 64) { Er[v] = apply(Ad[v], Er[v], E1); Ad[v] *= A1; }
+        }
+    }
+    if (LC >= 6 || lane >= 64 - lcol) {
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { buf.v[wave][v][cl] = Au[v]; buf.v[wave][VC + v][cl] = Hr[v]; }
+    }
+    if (LC >= 6 || lane < lcol) {
+#pragma unroll
+        for (int v = 0; v < VC; ++v) buf.v[wave][2 * VC + v][cl] = Er[v];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < VC; ++v) {
+        float c = hs[v], d = carry[v];
+        h[v] = c; e[v] = d;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            c = apply(buf.v[w][v][cl], buf.v[w][VC + v][cl], c);
+            if (w + 1 == wave) h[v] = c;
+        }
+#pragma unroll
+        for (int w = 3; w >= 0; --w) {
+            d = apply(buf.v[w][v][cl], buf.v[w][2 * VC + v][cl], d);
+            if (w - 1 == wave) e[v] = d;
+        }
+        carry[v] = d;
+        if (LC < 6) {
+            const float A0 = __shfl_up(Au[v], lcol, 64), H0 = __shfl_up(Hr[v], lcol, 64);
+            const float A1 = __shfl_down(Ad[v], lcol, 64), E1 = __shfl_down(Er[v], lcol, 64);
+            if (lane >= lcol) h[v] = apply(A0, H0, h[v]);
+            if (lane + lcol < 64) e[v] = apply(A1, E1, e[v]);
+        }
+    }
+}
+
+// state at the start of stretch y of this launch: the (A, H) of the stretches walked before it composed
+// onto the given one (ascending in the forward pass, descending in the backward pass)
+template <int VC, bool BWD> NK_D void stretch_start(const ScanArgs& A, const Place& p, float* carry) {
+    const int n = BWD ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+#pragma unroll 4
+    for (int q = 0; q < n; ++q) {
+        const int y = BWD ? gridDim.y - 1 - q : q;
+        const float* w = A.sums + (int64_t)y * 2 * A.cols * VC + p.col * VC;
+#pragma unroll
+        for (int v = 0; v < VC; ++v) carry[v] = apply(w[v], w[A.cols * VC + v], carry[v]);
+    }
+}
+
+// First launch of a split sequence: (A, H) of a stretch, or (A, E) of the backward pass.  Nothing has to be
+// written in order here, so a thread takes one long run of the stretch and the runs are composed once.
+template <typename T, typename GT, int VC, bool SHARED, bool BWD>
+__global__ __launch_bounds__(SC_THREADS) void k_scan_sum(const ScanArgs A) {
+    __shared__ Buf<VC> buf[2];
+    const Place p = place<VC, SHARED>(A);
+    constexpr int GV = SHARED ? 1 : VC;
+    const int y = blockIdx.y + (BWD ? 1 : 0);        // the stretch walked last needs no sum
+    const int per = A.stretch / (SC_THREADS >> A.LC), lo = A.begin + y * A.stretch + p.run * per;
+    const int hi = min(min(lo + per, A.end), p.len);
+    float Ar[VC], Hr[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = 0.0f; }
+    const int64_t as = A.reverse ? -A.a_st : A.a_st, xs = A.reverse ? -A.x_st : A.x_st;
+    const GT* ab = (const GT*)A.a + p.b * A.a_sb + p.gate;
+    const T* xb = (const T*)A.x + p.b * A.x_sb + p.c;
+    const int rows = hi - lo, turns = rows > 0 ? (rows + SC_U - 1) / SC_U : 0;
+    for (int q = 0; q < turns; ++q) {
+        const int s0 = lo + (BWD ? turns - 1 - q : q) * SC_U;
+        const int64_t t0 = time_of(s0, p.len, A.reverse);
+        Pack<GT, GV> ra[SC_U];
+        Pack<T, VC> rx[SC_U];
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, hi, 1.0f);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, A.x ? hi : 0, 0.0f);
+#pragma unroll
+        for (int w = 0; w < SC_U; ++w) {
+            const int u = BWD ? SC_U - 1 - w : w;
+#pragma unroll
+            for (int v = 0; v < VC; ++v) {
+                const float a = (float)ra[u].v[SHARED ? 0 : v], x = (float)rx[u].v[v];
+                Hr[v] = BWD ? a * (x + Hr[v]) : fmaf(a, Hr[v], x);
+                Ar[v] *= a;
+            }
+        }
+    }
+    // H from a start of zero, A from a start of one without summands
+    float zero[VC], one[VC], H[VC], s[VC], e[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) { zero[v] = H[v] = 0.0f; one[v] = 1.0f; }
+    if (BWD) {
+        compose_both<VC>(Ar, zero, Hr, zero, H, s, e, A.LC, buf[0]);
+        compose_both<VC>(Ar, zero, zero, zero, one, s, e, A.LC, buf[1]);
+    } else {
+        compose_up<VC>(Ar, Hr, H, s, A.LC, buf[0]);
+        compose_up<VC>(Ar, zero, one, s, A.LC, buf[1]);
+    }
+    if (p.on && p.run == 0) {
+        float* w = A.sums + (int64_t)y * 2 * A.cols * VC + p.col * VC;
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { w[v] = one[v]; w[A.cols * VC + v] = H[v]; }
+    }
+}
+
+template <typename T, typename GT, int VC, bool SHARED>
+__global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
+    __shared__ Buf<VC> buf[2];
+    constexpr int GV = SHARED ? 1 : VC;
+    const Place p = place<VC, SHARED>(A);
+    const int tile = (SC_THREADS >> A.LC) * SC_U;
+    const int begin = A.begin + blockIdx.y * A.stretch, end = min(A.end, begin + A.stretch);
+    const int stop = min(end, longest(p, A));           // behind it every column is dead
+    float carry[VC], s[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) carry[v] = 0.0f;
+    if (p.on) {
+        if (A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
+        stretch_start<VC, false>(A, p, carry);
+    }
+    const int64_t as = A.reverse ? -A.a_st : A.a_st, xs = A.reverse ? -A.x_st : A.x_st, os = A.reverse ? -A.C : A.C;
+    const GT* ab = (const GT*)A.a + p.b * A.a_sb + p.gate;
+    const T* xb = (const T*)A.x + p.b * A.x_sb + p.c;
+    T* ob = (T*)A.o + p.b * A.T * A.C + p.c;
+    const int kept = (A.T + SC_KEEP - 1) / SC_KEEP;
+    const int lim = min(p.len, end);
+    Pack<GT, GV> ra[SC_U];
+    Pack<T, VC> rx[SC_U];
+    int s0 = begin + p.run * SC_U;
+    {
+        const int64_t t0 = time_of(s0, p.len, A.reverse);
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, lim, 0.0f);
+    }
+    int flip = 0, at = begin;
+    for (; at < stop; at += tile, s0 += tile, flip ^= 1) {
+        Pack<GT, GV> na[SC_U];
+        Pack<T, VC> nx[SC_U];
+        {       // the next tile's loads are in flight while this one is composed and written
+            const int s1 = s0 + tile;
+            const int64_t t1 = time_of(s1, p.len, A.reverse);
+            fetch<GT, GV>(na, ab + t1 * A.a_st, as, s1, lim, 1.0f);
+            fetch<T, VC>(nx, xb + t1 * A.x_st, xs, s1, lim, 0.0f);
+        }
+        float Ar[VC], Hr[VC];
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = 0.0f; }
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u)
+#pragma unroll
+            for (int v = 0; v < VC; ++v) {
+                const float a = (float)ra[u].v[SHARED ? 0 : v];
+                Hr[v] = fmaf(a, Hr[v], (float)rx[u].v[v]);
+                Ar[v] *= a;
+            }
+        compose_up<VC>(Ar, Hr, carry, s, A.LC, buf[flip]);
+        if (A.states && (s0 & (SC_KEEP - 1)) == 0 && s0 < lim) st<float, VC>(A.states + ((int64_t)p.b * kept + s0 / SC_KEEP) * A.C + p.c, s);
+        T* o = ob + time_of(s0, p.len, A.reverse) * A.C;
+        const bool whole = __all(s0 + SC_U <= lim);
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u) {
+#pragma unroll
+            for (int v = 0; v < VC; ++v) s[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], s[v], (float)rx[u].v[v]);
+            if (whole || s0 + u < lim) st<T, VC>(o + u * os, s);
+            else if (p.on && s0 + u < end) {
+                float z[VC];
+#pragma unroll
+                for (int v = 0; v < VC; ++v) z[v] = 0.0f;
+                st<T, VC>(ob + (int64_t)(s0 + u) * A.C, z);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u) { ra[u] = na[u]; rx[u] = nx[u]; }
+    }
+    float z[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) z[v] = 0.0f;
+    if (p.on) for (int t = at + p.run; t < end; t += SC_THREADS >> A.LC) st<T, VC>(ob + (int64_t)t * A.C, z);
+    if (p.on && p.run == 0 && A.last && end == A.end)
+        for (int v = 0; v < VC; ++v) A.last[p.b * A.C + p.c + v] = carry[v];
+}
+
+// Sums of SC_U values over the `wide` (a power of two) neighbouring lanes of a gate: while a lane holds more
+// than one value it trades half of them with its partner, so U values cost about U shuffles instead of
+// U log2(wide).  On return the lane holds sums of steps u0 .. u0 + n - 1, all of them if `mine`.
+NK_D void gate_sums(float (&v)[SC_U], int wide, int k, int* u0, int* n, bool* mine) {
+    int off = wide >> 1, held = SC_U, first = 0;
+    if (off > 0) {
+        const bool up = (k & off) != 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float keep = up ? v[4 + i] : v[i], send = up ? v[i] : v[4 + i];
+            v[i] = keep + __shfl_xor(send, off, 64);
+        }
+        first += up ? 4 : 0; held = 4; off >>= 1;
+    }
+    if (off > 0) {
+        const bool up = (k & off) != 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float keep = up ? v[2 + i] : v[i], send = up ? v[i] : v[2 + i];
+            v[i] = keep + __shfl_xor(send, off, 64);
+        }
+        first += up ? 2 : 0; held = 2; off >>= 1;
+    }
+    if (off > 0) {
+        const bool up = (k & off) != 0;
+        const float keep = up ? v[1] : v[0], send = up ? v[0] : v[1];
+        v[0] = keep + __shfl_xor(send, off, 64);
+        first += up ? 1 : 0; held = 1; off >>= 1;
+    }
+    *mine = (k & (2 * off - (off > 0 ? 1 : 0))) == 0;
+    for (; off > 0; off >>= 1) v[0] += __shfl_xor(v[0], off, 64);
+    *u0 = first; *n = held;
+}
+
+template <typename T, typename GT, int VC, bool SHARED>
+__global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
+    __shared__ Buf<VC> buf[2];
+    constexpr int GV = SHARED ? 1 : VC;
+    const Place p = place<VC, SHARED>(A);
+    const int tile = (SC_THREADS >> A.LC) * SC_U;
+    const int begin = A.begin + blockIdx.y * A.stretch, end = min(A.end, begin + A.stretch);
+    const int stop = min(end, longest(p, A));
+    float carry[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) carry[v] = 0.0f;
+    if (p.on) {
+        if (A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
+        stretch_start<VC, true>(A, p, carry);
+    }
+    const bool gates = A.d_a != nullptr;
+    const int64_t as = A.reverse ? -A.a_st : A.a_st, xs = A.reverse ? -A.x_st : A.x_st, gs = A.reverse ? -A.g_st : A.g_st;
+    const GT* ab = (const GT*)A.a + p.b * A.a_sb + p.gate;
+    const T* xb = (const T*)A.x + p.b * A.x_sb + p.c;
+    const T* gb = (const T*)A.g + p.b * A.g_sb + p.c;
+    T* ob = (T*)A.o + p.b * A.T * A.C + p.c;
+    const int kept = (A.T + SC_KEEP - 1) / SC_KEEP;
+    const int lim = min(p.len, end);
+    // the gate's share of a row of dL/da: `wide` lanes hold it, `parts` such shares make it
+    const int wide = min(min(A.LG, 1 << A.LC), 64);
+    GT* db = (GT*)A.d_a + (SHARED ? p.b * A.T * A.J + p.gate : p.b * A.T * A.C + p.c);
+    float* pb = A.gate_part + (int64_t)(p.k / wide) * A.B * A.T * A.J + p.b * A.T * A.J + p.gate;
+    const bool part = A.LG > wide;
+    const int64_t drow = SHARED ? A.J : A.C;
+    const int tiles = stop > begin ? (stop - begin + tile - 1) / tile : 0;
+    int flip = 0;
+    // rows behind the last tile with a live step
+    {
+        float z[VC];
+#pragma unroll
+        for (int v = 0; v < VC; ++v) z[v] = 0.0f;
+        for (int t = begin + tiles * tile + p.run; t < end; t += SC_THREADS >> A.LC) {
+            if (p.on && A.o) st<T, VC>(ob + (int64_t)t * A.C, z);
+            if (gates && p.col < A.cols) {
+                if (!SHARED) st<GT, VC>(db + t * drow, z);
+                else if (part) { if ((p.k & (wide - 1)) == 0) pb[t * drow] = 0.0f; }
+                else if (p.k == 0) db[t * drow] = (GT)0.0f;
+            }
+        }
+    }
+    for (int q = tiles - 1; q >= 0; --q, flip ^= 1) {
+        const int at = begin + q * tile, s0 = at + p.run * SC_U;
+        const int64_t t0 = time_of(s0, p.len, A.reverse);
+        Pack<GT, GV> ra[SC_U];
+        Pack<T, VC> rx[SC_U], rg[SC_U];
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
+        fetch<T, VC>(rg, gb + t0 * A.g_st, gs, s0, A.g ? lim : 0, 0.0f);
+        float hs[VC], h[VC], e[VC];
+#pragma unroll
+        for (int v = 0; v < VC; ++v) hs[v] = 0.0f;
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, gates ? lim : 0, 0.0f);
+        if (gates) {
+            const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
+                                        : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
+            if (p.on && from && at < lim) for (int v = 0; v < VC; ++v) hs[v] = from[v];
+        }
+        float Ar[VC], Hr[VC], Er[VC];
+#pragma unroll
+        for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = Er[v] = 0.0f; }
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u)
+#pragma unroll
+            for (int v = 0; v < VC; ++v) {
+                const float a = (float)ra[u].v[SHARED ? 0 : v];
+                Hr[v] = fmaf(a, Hr[v], (float)rx[u].v[v]);
+                Ar[v] *= a;
+            }
+#pragma unroll
+        for (int u = SC_U - 1; u >= 0; --u)
+#pragma unroll
+            for (int v = 0; v < VC; ++v) Er[v] = (float)ra[u].v[SHARED ? 0 : v] * ((float)rg[u].v[v] + Er[v]);
+        compose_both<VC>(Ar, Hr, Er, hs, carry, h, e, A.LC, buf[flip]);
+        float prev[SC_U][VC], sum[SC_U];
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u)
+#pragma unroll
+            for (int v = 0; v < VC; ++v) { prev[u][v] = h[v]; h[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], h[v], (float)rx[u].v[v]); }
+        const bool whole = __all(s0 + SC_U <= lim);
+        T* o = ob + t0 * A.C;
+        const int64_t os = A.reverse ? -A.C : A.C, ds = A.reverse ? -drow : drow;
+#pragma unroll
+        for (int u = SC_U - 1; u >= 0; --u) {
+            float d[VC], dg[VC];
+            const bool live = whole || s0 + u < lim;
+            sum[u] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < VC; ++v) {
+                d[v] = (float)rg[u].v[v] + e[v];
+                e[v] = (float)ra[u].v[SHARED ? 0 : v] * d[v];
+                if (!live) d[v] = 0.0f;
+                dg[v] = live ? d[v] * prev[u][v] : 0.0f;
+                sum[u] += dg[v];
+            }
+            if (live) {
+                if (A.o) st<T, VC>(o + u * os, d);
+                if (!SHARED && gates) st<GT, VC>(db + t0 * drow + u * ds, dg);
+            } else if (p.on && s0 + u < end) {      // behind the sequence: zeros, in place
+                if (A.o) st<T, VC>(ob + (int64_t)(s0 + u) * A.C, d);
+                if (!SHARED && gates) st<GT, VC>(db + (int64_t)(s0 + u) * drow, dg);
+            }
+        }
+        if (SHARED && gates) {
+            int u0, n;
+            bool mine;
+            gate_sums(sum, wide, p.k, &u0, &n, &mine);
+            // the live steps of the sequence, whether or not this lane has channels
+            const int len = p.col >= A.cols ? 0 : A.lengths ? max(0, min(A.T, A.lengths[p.b])) : A.T;
+            if (mine && p.col < A.cols) {
+#pragma unroll
+                for (int i = 0; i < SC_U; ++i)
+                    if (i < n && s0 + u0 + i < end) {
+                        const int sx = s0 + u0 + i;
+                        const int64_t row = sx < len ? time_of(sx, len, A.reverse) : sx;
+                        if (part) pb[row * drow] = sum[i]; else db[row * drow] = (GT)sum[i];
+                    }
+            }
+        }
+    }
+    if (p.on && p.run == 0 && A.last && begin == A.begin)
+        for (int v = 0; v < VC; ++v) A.last[p.b * A.C + p.c + v] = carry[v];
+}
+
+// dL/da of gates wider than a wavefront's share of a tile: the parts are added in one order
+template <typename GT>
+__global__ __launch_bounds__(256) void k_gate_sum(const float* __restrict__ part, GT* __restrict__ d_a, int64_t n, int parts) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.0f;
+    for (int k = 0; k < parts; ++k) s += part[(int64_t)k * n + i];
+    d_a[i] = (GT)s;
+}
+
+struct Shape {
+    int VC, LC, S, parts, blocks;           // blocks: launches along the sequence
+    int64_t cols;
+    int32_t stretch, block;
+    int32_t G, LG, per_b;
+    bool shared;
+    int64_t carry_bytes, sums_bytes, part_bytes;
+};
+
+inline int ceil_log2(int64_t x) { int k = 0; while (((int64_t)1 << k) < x) ++k; return k; }
+inline int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
+
+// The variant for a shape.  `vec`: addresses and strides allow four channels per load.
+void shape_of(const nk_scan_opts* o, bool vec, int bwd, Shape* s) {
+    s->G = (int32_t)(o->C / o->gates);
+    s->shared = s->G > 1;
+    s->VC = vec && (s->shared ? s->G : o->C) % 4 == 0 ? 4 : 1;
+    const int64_t unit = s->shared ? (s->G + s->VC - 1) / s->VC : (o->C + s->VC - 1) / s->VC;
+    const int64_t all = (s->shared ? o->gates : 1) * o->B * unit;
+    // 16 columns x 16 runs (a row of a tile is 128 bytes of bf16 at four channels a column), 64 x 4 at one
+    int LC = s->VC == 4 ? NK_SCAN_LC : 6;
+    while (LC > 2 && ((int64_t)1 << LC) > all) --LC;
+    const int runs_wanted = ceil_log2((o->T + SC_U - 1) / SC_U);
+    if (runs_wanted < 8 - LC) LC = 8 - runs_wanted;
+    if (LC == 7) LC = 6;
+    s->LC = LC;
+    const int lcol = 1 << LC;
+    if (s->shared) {
+        const int64_t p2 = (int64_t)1 << ceil_log2(unit);
+        s->LG = (int32_t)(p2 <= lcol ? p2 : (unit + lcol - 1) / lcol * lcol);
+        s->per_b = (int32_t)(s->LG * o->gates);
+    } else {
+        s->LG = 1;
+        s->per_b = (int32_t)unit;
+    }
+    s->cols = o->B * s->per_b;
+    const int wide = lcol < 64 ? lcol : 64;
+    s->parts = s->shared && s->LG > wide ? s->LG / wide : 1;
+    const int64_t groups = (s->cols + lcol - 1) / lcol, tile = (int64_t)(SC_THREADS >> LC) * SC_U;
+    const int64_t tiles = (o->T + tile - 1) / tile;
+    int64_t S = 1;
+    s->block = (int32_t)(tiles * tile);
+    if (groups < NK_SCAN_FEW && tiles > 1) {
+        // the second launch of a split block finds what the first one read in the 256 MB cache behind the L2s
+        const int64_t row = o->B * (o->C * elem(o->dtype) + o->gates * elem(o->gate_dtype));
+        int64_t fit = ((int64_t)NK_SCAN_CACHE << 20) / (row * tile);
+        if (fit < 1) fit = 1;
+        const int64_t blocks = (tiles + fit - 1) / fit;
+        const int64_t per = (tiles + blocks - 1) / blocks;
+        s->block = (int32_t)(per * tile);
+        S = (NK_SCAN_FILL + groups - 1) / groups;
+        if (S > per) S = per;
+        s->stretch = (int32_t)((per + S - 1) / S * tile);
+    } else {
+        s->stretch = s->block;
+    }
+    s->S = (s->block + s->stretch - 1) / s->stretch;
+    s->blocks = (int)((o->T + s->block - 1) / s->block);
+    s->carry_bytes = s->blocks > 1 ? up256(o->B * o->C * 4) : 0;
+    s->sums_bytes = s->S > 1 ? up256((int64_t)s->S * 2 * s->cols * s->VC * 4) : 0;
+    s->part_bytes = bwd && s->parts > 1 ? (int64_t)s->parts * o->B * o->T * o->gates * 4 : 0;
+}
+
+int check(const nk_scan_opts* o, const char* who) {
+    if (!o) NK_FAIL(NK_ERR_ARG, "%s: null options", who);
+    if (o->B < 0 || o->T < 0 || o->C < 1 || o->gates < 1 || o->C % o->gates != 0)
+        NK_FAIL(NK_ERR_ARG, "%s: B=%lld T=%lld C=%lld gates=%lld (gates divides C)", who, (long long)o->B, (long long)o->T, (long long)o->C, (long long)o->gates);
+    if (o->dtype < NK_F32 || o->dtype > NK_F16 || (o->gate_dtype != o->dtype && o->gate_dtype != NK_F32))
+        NK_FAIL(NK_ERR_UNSUPPORTED, "%s: dtype %d with gates of dtype %d (the same, or fp32)", who, o->dtype, o->gate_dtype);
+    const int64_t most = (int64_t)1 << 29;
+    if (o->C > most || o->T > most || o->B > most || o->B * o->C > ((int64_t)1 << 34))
+        NK_FAIL(NK_ERR_UNSUPPORTED, "%s: B, T, C up to 2^29 and B * C up to 2^34", who);
+    if (o->a_stride_b < 0 || o->a_stride_t < 0 || o->x_stride_b < 0 || o->x_stride_t < 0 || o->g_stride_b < 0 || o->g_stride_t < 0)
+        NK_FAIL(NK_ERR_ARG, "%s: negative stride", who);
+    return NK_OK;
+}
+
+template <typename T, typename GT, int VC, bool SHARED, bool BWD>
+void launch(ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
+    const unsigned groups = (unsigned)((s.cols + (1 << s.LC) - 1) >> s.LC);
+    float* last = A.last;
+    const int64_t n = s.carry_bytes / 4;        // two buffers in turn: a block's first stretches read what its last one replaces
+    for (int q = 0; q < s.blocks; ++q) {
+        const int k = BWD ? s.blocks - 1 - q : q;
+        A.begin = k * s.block;
+        A.end = (int)((int64_t)A.begin + s.block < A.T ? A.begin + s.block : A.T);
+        A.stretch = s.stretch;
+        const int S = (A.end - A.begin + s.stretch - 1) / s.stretch;
+        A.last = q + 1 < s.blocks ? carry + (q & 1) * n : last;
+        if (S > 1) {
+            ScanArgs B = A;
+            if (BWD) { B.x = A.g; B.x_sb = A.g_sb; B.x_st = A.g_st; }
+            hipLaunchKernelGGL((k_scan_sum<T, GT, VC, SHARED, BWD>), dim3(groups, S - 1), dim3(SC_THREADS), 0, st, B);
+        }
+        if constexpr (BWD) hipLaunchKernelGGL((k_scan_bwd<T, GT, VC, SHARED>), dim3(groups, S), dim3(SC_THREADS), 0, st, A);
+        else hipLaunchKernelGGL((k_scan_fwd<T, GT, VC, SHARED>), dim3(groups, S), dim3(SC_THREADS), 0, st, A);
+        A.first = carry + (q & 1) * n;
+    }
+}
+
+template <typename T, typename GT, bool BWD>
+void launch_vc(ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
+    if (s.VC == 4) { if (s.shared) launch<T, GT, 4, true, BWD>(A, s, carry, st); else launch<T, GT, 4, false, BWD>(A, s, carry, st); }
+    else { if (s.shared) launch<T, GT, 1, true, BWD>(A, s, carry, st); else launch<T, GT, 1, false, BWD>(A, s, carry, st); }
+}
+template <bool BWD>
+int launch_types(const nk_scan_opts* o, ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
+    const bool g32 = o->gate_dtype == NK_F32;
+    if (o->dtype == NK_F32) launch_vc<float, float, BWD>(A, s, carry, st);
+    else if (o->dtype == NK_BF16) { if (g32) launch_vc<__bf16, float, BWD>(A, s, carry, st); else launch_vc<__bf16, __bf16, BWD>(A, s, carry, st); }
+    else { if (g32) launch_vc<_Float16, float, BWD>(A, s, carry, st); else launch_vc<_Float16, _Float16, BWD>(A, s, carry, st); }
+    NK_CHECK_LAUNCH("k_scan");
+    if (BWD && s.parts > 1 && A.d_a) {
+        const int64_t n = o->B * o->T * o->gates;
+        const dim3 grid((unsigned)((n + 255) / 256));
+        if (g32) hipLaunchKernelGGL(k_gate_sum<float>, grid, dim3(256), 0, st, A.gate_part, (float*)A.d_a, n, s.parts);
+        else if (o->dtype == NK_BF16) hipLaunchKernelGGL(k_gate_sum<__bf16>, grid, dim3(256), 0, st, A.gate_part, (__bf16*)A.d_a, n, s.parts);
+        else hipLaunchKernelGGL(k_gate_sum<_Float16>, grid, dim3(256), 0, st, A.gate_part, (_Float16*)A.d_a, n, s.parts);
+        NK_CHECK_LAUNCH("k_gate_sum");
+    }
+    return NK_OK;
+}
+
+// four channels per load: every row of every tensor starts on a multiple of four elements
+bool can_vec(const nk_scan_opts* o, const void* a, const void* x, const void* g, const void* out, const void* d_a, const void* states) {
+    const int64_t e = elem(o->dtype) * 4, ge = elem(o->gate_dtype) * 4;
+    if (((uintptr_t)x % e) || ((uintptr_t)g % e) || ((uintptr_t)out % e) || ((uintptr_t)states % 16) || o->C % 4) return false;
+    if ((x && (o->x_stride_b % 4 || o->x_stride_t % 4)) || (g && (o->g_stride_b % 4 || o->g_stride_t % 4))) return false;
+    if (o->gates != o->C) return true;
+    return ((uintptr_t)a % ge) == 0 && ((uintptr_t)d_a % ge) == 0 && o->a_stride_b % 4 == 0 && o->a_stride_t % 4 == 0;
+}
+
+ScanArgs args_of(const nk_scan_opts* o, const Shape& s, void* ws, float** carry) {
+    ScanArgs A = {};
+    A.lengths = o->lengths; A.T = (int32_t)o->T; A.C = o->C; A.B = o->B; A.J = o->gates;
+    A.a_sb = o->a_stride_b; A.a_st = o->a_stride_t; A.x_sb = o->x_stride_b; A.x_st = o->x_stride_t;
+    A.g_sb = o->g_stride_b; A.g_st = o->g_stride_t;
+    A.cols = s.cols; A.G = s.G; A.LG = s.LG; A.per_b = s.per_b; A.LC = s.LC; A.reverse = o->reverse != 0;
+    *carry = (float*)ws;
+    A.sums = (float*)((char*)ws + 2 * s.carry_bytes);
+    A.gate_part = (float*)((char*)ws + 2 * s.carry_bytes + s.sums_bytes);
+    return A;
+}
+
+int64_t bytes_of(const Shape& s) { return 2 * s.carry_bytes + s.sums_bytes + s.part_bytes; }
+
+}  // namespace
+
+extern "C" int64_t nk_gated_scan_workspace_bytes(const nk_scan_opts* o, int backward) {
+    const int rc = check(o, "nk_gated_scan_workspace_bytes");
+    if (rc < 0) return rc;
+    if (o->B == 0 || o->T == 0) return 0;
+    int64_t most = 0;
+    for (int vec = 0; vec < 2; ++vec) {         // which of the two variants runs depends on the addresses
+        Shape s;
+        shape_of(o, vec != 0, backward, &s);
+        if (bytes_of(s) > most) most = bytes_of(s);
+    }
+    return most;
+}
+
+extern "C" int64_t nk_gated_scan_states_bytes(const nk_scan_opts* o) {
+    const int rc = check(o, "nk_gated_scan_states_bytes");
+    if (rc < 0) return rc;
+    return o->B * ((o->T + SC_KEEP - 1) / SC_KEEP) * o->C * 4;
+}
+
+extern "C" int nk_gated_scan_fwd(const nk_scan_opts* o, const void* a, const void* x, const float* h0, void* h, float* h_last,
+                                 float* states, void* workspace, int64_t workspace_bytes, void* stream) {
+    int rc = check(o, "nk_gated_scan_fwd");
+    if (rc < 0) return rc;
+    if (o->B == 0) return NK_OK;
+    if (o->T == 0) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_fwd: T = 0 (the state does not change: nothing to launch)");
+    if (!a || !x || !h) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_fwd: null pointer");
+    Shape s;
+    shape_of(o, can_vec(o, a, x, nullptr, h, nullptr, states), 0, &s);
+    if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
+        NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_fwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
+    float* carry;
+    ScanArgs A = args_of(o, s, workspace, &carry);
+    A.a = a; A.x = x; A.first = h0; A.o = h; A.last = h_last; A.states = states;
+    return launch_types<false>(o, A, s, carry, nk_stream(stream));
+}
+
+extern "C" int nk_gated_scan_bwd(const nk_scan_opts* o, const void* a, const void* x, const float* states, const float* h0,
+                                 const void* d_h, const float* d_h_last, void* d_a, void* d_x, float* d_h0, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+    int rc = check(o, "nk_gated_scan_bwd");
+    if (rc < 0) return rc;
+    if (o->B == 0) return NK_OK;
+    if (o->T == 0) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_bwd: T = 0");
+    if (!a || (d_a && (!x || !states)) || (!d_a && !d_x && !d_h0)) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_bwd: null pointer");
+    Shape s;
+    shape_of(o, can_vec(o, a, d_a ? x : nullptr, d_h, d_x, d_a, states), 1, &s);
+    if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
+        NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_bwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
+    float* carry;
+    ScanArgs A = args_of(o, s, workspace, &carry);
+    A.a = a; A.x = x; A.g = d_h; A.h0 = h0; A.states = (float*)states; A.first = d_h_last; A.o = d_x; A.d_a = d_a; A.last = d_h0;
+    return launch_types<true>(o, A, s, carry, nk_stream(stream));
+}

@@ -60,6 +60,13 @@ class NkRenderOut(C.Structure):
                                           "rgb_coarse", "disp_coarse", "acc_coarse", "depth_coarse")]
 
 
+class NkScanOpts(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("B", "T", "C", "gates")]
+                + [(n, C.c_int32) for n in ("dtype", "gate_dtype", "reverse", "reserved")]
+                + [(n, C.c_int64) for n in ("a_stride_b", "a_stride_t", "x_stride_b", "x_stride_t", "g_stride_b",
+                                              "g_stride_t")] + [("lengths", C.c_void_p)])
+
+
 class NkAdamwTensor(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "master", "scale_m", "scale_v")] + [("n", C.c_int64)]
 
@@ -87,6 +94,10 @@ SIGNATURES = {
     "nk_sample_training_rays_dev": (C.c_int, [_P, _I32, _P, _I64, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
     "nk_set_step_state": (C.c_int, [C.POINTER(NkStepState), _P, _P]),
     "nk_adam_step_dev": (C.c_int, [_P, _P, _P, _P, _I64, _P, C.c_double, C.c_double, C.c_double, _F, _P]),
+    "nk_gated_scan_workspace_bytes": (_I64, [C.POINTER(NkScanOpts), C.c_int]),
+    "nk_gated_scan_fwd": (C.c_int, [C.POINTER(NkScanOpts), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "nk_gated_scan_states_bytes": (_I64, [C.POINTER(NkScanOpts)]),
+    "nk_gated_scan_bwd": (C.c_int, [C.POINTER(NkScanOpts), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "nk_adamw_step": (C.c_int, [C.POINTER(NkAdamwTensor), _I32, C.POINTER(NkAdamwOpts), _P]),
     "nk_stratified_z": (C.c_int, [_P, _I64, _PO, _P, _P]),
     "nk_act_bytes": (_I64, [_PA, _I64, _I32]),

@@ -1,0 +1,141 @@
+"""Gated linear recurrence along a long axis, differentiable (``nk_gated_scan_fwd`` / ``_bwd``).
+
+Stands beside :func:`~nerf_kinematics_amd.render.raw2outputs`: alpha compositing along a ray is the
+recurrence with ``a = 1 - alpha``, ``x = alpha * colour``, walked from the far sample to the near one with one
+gate for all channels; here the channels, the length and the gates are free.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import lib as _lib
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B, T, n] with unit stride along n and no negative strides (a copy where it has neither)."""
+    if (t.shape[2] > 1 and t.stride(2) != 1) or t.stride(0) < 0 or t.stride(1) < 0:
+        return t.contiguous()
+    return t
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _call(dev, fn, *args) -> None:
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, stream))
+
+
+def _opts(a, x, g, lengths, reverse) -> "_lib.NkScanOpts":
+    B, T, C = x.shape
+    sg = (0, 0) if g is None else g.stride()
+    return _lib.NkScanOpts(B, T, C, a.shape[2], _lib.DTYPES[x.dtype], _lib.DTYPES[a.dtype], int(reverse), 0,
+                           a.stride(0), a.stride(1), x.stride(0), x.stride(1), sg[0], sg[1], _ptr(lengths))
+
+
+def _workspace(L, o, backward, dev):
+    n = _lib.check(L.nk_gated_scan_workspace_bytes(o, backward))
+    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n      # torch's blocks are 512-byte aligned
+
+
+def _forward(a, x, h0, lengths, reverse, training):
+    L = _lib.load()
+    B, T, C = x.shape
+    dev = x.device
+    if B == 0 or T == 0:        # no step: the state passes through
+        return x.new_empty(B, T, C), (h0.clone() if h0 is not None else torch.zeros(B, C, dtype=torch.float32, device=dev)), None
+    h = torch.empty(B, T, C, dtype=x.dtype, device=dev)
+    last = torch.empty(B, C, dtype=torch.float32, device=dev)
+    o = _opts(a, x, None, lengths, reverse)
+    states = None
+    if training:
+        states = torch.empty(_lib.check(L.nk_gated_scan_states_bytes(o)) // 4, dtype=torch.float32, device=dev)
+    ws, n = _workspace(L, o, 0, dev)
+    _call(dev, L.nk_gated_scan_fwd, o, a.data_ptr(), x.data_ptr(), _ptr(h0), h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), n)
+    return h, last, states
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, x, h0, lengths, reverse):
+        # the states in front of every 32nd step serve the gates' gradient alone
+        h, last, states = _forward(a, x, h0, lengths, reverse, ctx.needs_input_grad[0])
+        ctx.save_for_backward(a, x, h0, lengths, states)
+        ctx.reverse = reverse
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_h, d_last):
+        a, x, h0, lengths, states = ctx.saved_tensors
+        want_a, want_x, want_0 = ctx.needs_input_grad[:3]
+        B, T, C = x.shape
+        dev = x.device
+        if d_h is None and d_last is None:
+            return None, None, None, None, None
+        if d_last is not None:
+            d_last = d_last.contiguous()
+        if B == 0 or T == 0:
+            z = lambda t, want: torch.zeros_like(t) if want else None
+            d_0 = None
+            if want_0:
+                d_0 = d_last.clone() if d_last is not None else torch.zeros_like(h0)
+            return z(a, want_a), z(x, want_x), d_0, None, None
+        L = _lib.load()
+        g = _rows(d_h) if d_h is not None else None
+        o = _opts(a, x, g, lengths, ctx.reverse)
+        d_a = torch.empty(B, T, a.shape[2], dtype=a.dtype, device=dev) if want_a else None
+        d_x = torch.empty(B, T, C, dtype=x.dtype, device=dev) if want_x else None
+        d_0 = torch.empty(B, C, dtype=torch.float32, device=dev) if want_0 else None
+        ws, n = _workspace(L, o, 1, dev)
+        _call(dev, L.nk_gated_scan_bwd, o, a.data_ptr(), x.data_ptr(), _ptr(states), _ptr(h0), _ptr(g), _ptr(d_last),
+              _ptr(d_a), _ptr(d_x), _ptr(d_0), _ptr(ws), n)
+        return d_a, d_x, d_0, None, None
+
+
+def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *, lengths: Optional[torch.Tensor] = None,
+               reverse: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``h_t = a_t * h_(t-1) + x_t`` along axis 1 of ``x`` [B, T, C]; returns ``(h, h_last)``.
+
+    ``a`` is [B, T, J] with J dividing C: gate j serves the C / J consecutive channels from ``j * C / J`` on (J = 1:
+    one gate per step; J = C: one per channel), of ``x``'s dtype or float32.  ``x`` and ``h`` are float32,
+    bfloat16 or float16; the state is float32: ``h0`` [B, C] (default zero) and ``h_last`` [B, C].  ``reverse`` walks
+    from the last step to the first.  ``lengths`` [B] int32 cuts sequence b short: rows behind it are not read and
+    ``h`` and all gradients are zero there; values outside 0..T are clamped.
+
+    Differentiable in ``a``, ``x`` and ``h0`` (first order), through both results.  For one step at a time pass T = 1
+    and the last state as ``h0``.  A training call also keeps the float32 state in front of every 32nd step.
+    """
+    if not isinstance(x, torch.Tensor) or x.dtype not in _lib.DTYPES or x.dim() != 3:
+        raise ValueError("x: expected a [B, T, C] tensor of float32, bfloat16 or float16")
+    B, T, C = x.shape
+    if not isinstance(a, torch.Tensor) or a.dim() != 3 or tuple(a.shape[:2]) != (B, T) or a.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"a: expected a [{B}, {T}, J] tensor of {x.dtype} or float32")
+    J = a.shape[2]
+    if C < 1 or J < 1 or C % J:
+        raise ValueError(f"a: {J} gates for {C} channels (a divisor of them)")
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("x: expected a GPU tensor (there is no CPU implementation)")
+    if a.device != dev:
+        raise ValueError(f"a: expected a tensor on {dev}")
+    if h0 is not None:
+        if h0.dtype != torch.float32 or tuple(h0.shape) != (B, C) or h0.device != dev:
+            raise ValueError(f"h0: expected a float32 tensor of shape {(B, C)} on {dev}")
+        h0 = h0.contiguous()
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or lengths.device != dev:
+            raise ValueError(f"lengths: expected an int32 tensor of shape {(B,)} on {dev}")
+        lengths = lengths.contiguous()
+    a, x = _rows(a), _rows(x)
+    if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _GatedScan.apply(a, x, h0, lengths, bool(reverse))
+    return _forward(a, x, h0, lengths, bool(reverse), False)[:2]
