@@ -248,6 +248,35 @@ int nk_gated_scan_bwd(const nk_scan_opts* opts /*host*/, const void* a, const vo
                       const float* h0, const void* d_h, const float* d_h_last, void* d_a, void* d_x, float* d_h0,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Softmax cross entropy of a linear head, forward and backward, without holding the logits
+ * z = hidden weight^T (hidden [N, D], weight [V, D], one type; products in fp32):
+ *     loss_n = log(sum_v exp z_(n,v)) - z_(n, target_n)
+ * target: device int64, 0 .. V-1 or ignore_index (loss 0, no gradient; such a row of hidden may hold
+ * anything).  Any other value makes the token's loss and the gradients NaN; nothing is read out of range.
+ * NK_REDUCE_MEAN divides by the number of tokens that are not ignored (0 if there are none).
+ * hidden and weight have unit stride along D and the given row strides (in elements); rows that do not start
+ * on 16 bytes are copied into the workspace first, the weight piece by piece.                       */
+enum { NK_REDUCE_NONE = 0, NK_REDUCE_MEAN = 1, NK_REDUCE_SUM = 2 };
+typedef struct nk_xent_opts {
+    int64_t N, D, V;
+    int64_t hidden_stride, weight_stride;
+    int64_t ignore_index;
+    int32_t dtype;                /* NK_F32 | NK_BF16 | NK_F16                                */
+    int32_t reduction;            /* NK_REDUCE_*                                              */
+    int64_t piece;                /* rows of the vocabulary per piece of the backward call, rounded up to 256;
+                                     0: as many as keep a piece's gradients (2 N piece elements) near 256 MB */
+} nk_xent_opts;
+/* Scratch of a call on these operands (256-byte aligned; it holds nothing between calls). */
+int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int backward);
+/* loss [N] and lse [N] (kept for the backward call) are always written; reduced [1] receives the mean or sum. */
+int nk_linear_xent_fwd(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, const int64_t* target,
+                       float* loss, float* lse, float* reduced, void* workspace, int64_t workspace_bytes, void* stream);
+/* d_loss: [N] (NK_REDUCE_NONE) or [1].  d_hidden [N, D] and d_weight [V, D] (contiguous, the operands' type) are
+ * written, not accumulated; either may be NULL when unwanted.                                        */
+int nk_linear_xent_bwd(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, const int64_t* target,
+                       const float* lse, const float* d_loss, void* d_hidden, void* d_weight, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 /* AdamW (torch.optim.AdamW's update, decoupled weight decay) over many tensors in one launch per 56 of
  * them.  No counterpart in the reference, whose optimiser is Adam on fp32 parameters.
  *   param       n elements of opts->param_dtype, updated in place

@@ -10,6 +10,7 @@ from .render import (get_rays, stratified_z, run_network, raw2outputs, raw2outpu
                      sample_pdf, render_rays, make_opts, alloc_activations, mlp_backward, mse_loss,
                      adam_step)
 from .scan import gated_scan  # noqa: F401
+from .xent import linear_cross_entropy  # noqa: F401
 from .optim import AdamW, adamw_state, adamw_step, decode_moment, encode_moment  # noqa: F401
 
 __version__ = "0.1.0"

@@ -1,0 +1,739 @@
+// Softmax cross entropy of a linear head, without ever holding the logits:
+//
+//   z_(n,v) = <hidden_n, weight_v>        loss_n = lse_n - z_(n,t_n),  lse_n = log sum_v exp z_(n,v)
+//   dz_(n,v) = c_n (exp(z_(n,v) - lse_n) - [v = t_n])      d_hidden = dz weight,  d_weight = dz^T hidden
+//
+// Forward: one product weight x hidden^T on the matrix cores whose tiles end in registers; a tile leaves
+// the maximum and the sum of exponentials of its vocabulary rows for every token (8 bytes per token and tile),
+// a second kernel joins them.  Backward: the vocabulary is walked in pieces; per piece the logits are
+// computed again, turned into dz (rounded once to the operands' type: the two products that follow take it as
+// a matrix operand) and multiplied into d_weight's rows of the piece and onto d_hidden's fp32 sums.
+//
+// All products have the form C[m][n] = sum_k A[m][k] B[n][k] with k contiguous in both operands; where the
+// mathematics wants the other order (weight^T, hidden^T) a piece is transposed once by a copy, and dz is
+// written in both orders by the tile that computes it.
+#include "nk_common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+#ifndef NK_XENT_PIECE_MB
+#define NK_XENT_PIECE_MB 256
+#endif
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// ---- operand types: 16 bytes of k per lane and fragment --------------------------------------
+template <typename T> struct Op;
+template <> struct Op<__bf16> {
+    static constexpr float SCALE = 1.0f;    // dz is multiplied by this before it is rounded
+    NK_D static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Op<_Float16> {
+    // softmax values of a large vocabulary fall below fp16's smallest normal value (2^-14): 2^14 of headroom
+    // keeps |dz| <= 1 at most 16 384 and makes 2^-28 the smallest normal one
+    static constexpr float SCALE = 16384.0f;
+    NK_D static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Op<float> {
+    static constexpr float SCALE = 1.0f;
+    // element j of every lane's four is one 16x16x4 product; any order of k serves as long as A and B agree
+    NK_D static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ---- the tile product -------------------------------------------------------------------------
+// A workgroup computes BM x BN of C with WGM x WGN wavefronts, each TM x TN tiles of 16 x 16.  k advances
+// by 128 bytes of every row; the rows of a step are loaded straight into LDS (16 bytes a lane, 8 rows a
+// wavefront and instruction) STAGES - 1 steps ahead.  Row r keeps its eight 16-byte chunks in the order
+// chunk ^ (r & 7), so that the 16 rows a fragment read touches fall on different banks; the order is made by the
+// source address, the LDS side of such a load being fixed.  Rows behind the matrix and the end of k
+// are outside the buffer resource's range and arrive as zeros.
+struct Mat { const char* p; int64_t rows, stride; };      // stride in bytes, a multiple of 16, as is p
+
+template <int BM_, int BN_, int WGM_, int WGN_, int STAGES_> struct Cfg {
+    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_;
+    static constexpr int WAVES = WGM * WGN, THREADS = WAVES * 64;
+    static constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16;
+    static constexpr int STAGE_BYTES = (BM + BN) * 128, LDS = STAGE_BYTES * STAGES;
+    static constexpr int PIECES = (BM + BN) / 8 / WAVES;     // load instructions per wavefront and step
+};
+
+NK_D void lds_load(uint32_t lds_at, u32x4 srd, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds_at), "v"(voff), "s"(srd), "s"(soff) : "memory");
+}
+template <int N> NK_D void wait_loads_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory"); }
+
+NK_D u32x4 resource(const char* p, int64_t bytes) {
+    const uint64_t a = (uint64_t)p;
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xFFFF;
+    r[2] = __builtin_amdgcn_readfirstlane((int)(bytes < 0 ? 0 : bytes > 0x7FFFFFFF ? 0x7FFFFFFF : bytes));
+    r[3] = 0x00027000;
+    return r;
+}
+
+template <typename T, class C>
+NK_D void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds, f32x4 (&acc)[C::TM][C::TN]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / C::WGN, wn = wave % C::WGN;
+    u32x4 ra = resource(A.p + m0 * A.stride, (A.rows - m0) * A.stride);
+    u32x4 rb = resource(B.p + n0 * B.stride, (B.rows - n0) * B.stride);
+    asm volatile("s_nop 4" : "+s"(ra), "+s"(rb));       // scalars written by the vector unit, read by loads issued from asm
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(NK_LDS char*)lds;
+    // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
+    const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
+    uint32_t voff[C::PIECES];
+#pragma unroll
+    for (int i = 0; i < C::PIECES; ++i) {
+        const int r8 = wave * C::PIECES + i;                 // group of eight rows: A's first, then B's
+        const bool isa = r8 < C::BM / 8;
+        const int row = (isa ? r8 : r8 - C::BM / 8) * 8 + lrow;
+        voff[i] = (uint32_t)row * (uint32_t)(isa ? A.stride : B.stride) + lchunk * 16;
+    }
+    const int steps = (int)((kbytes + 127) / 128);
+    const bool ragged = (kbytes & 127) != 0;
+    auto issue = [&](int s, int slot) {
+        const bool cut = ragged && s == steps - 1 && (int64_t)s * 128 + lchunk * 16 >= kbytes;      // behind the end of k
+#pragma unroll
+        for (int i = 0; i < C::PIECES; ++i) {
+            const int r8 = wave * C::PIECES + i;
+            const uint32_t at = lds0 + slot * C::STAGE_BYTES + r8 * 1024;
+            const uint32_t v = cut ? 0x80000000u : voff[i];
+            if (r8 < C::BM / 8) lds_load(at, ra, v, (uint32_t)s * 128);
+            else lds_load(at, rb, v, (uint32_t)s * 128);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    const int pre = C::STAGES - 1;
+    for (int s = 0; s < pre && s < steps; ++s) issue(s, s);
+    int slot = 0, fill = pre % C::STAGES;
+    const int frow = lane & 15, fchunk = lane >> 4;
+    const char* fa = lds + (wm * C::TM * 16 + frow) * 128;
+    const char* fb = lds + (C::BM + wn * C::TN * 16 + frow) * 128;
+    const int x0 = (fchunk ^ (frow & 7)) * 16, x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
+    for (int s = 0; s < steps; ++s) {
+        // this step's loads have landed when at most those of the steps behind it are outstanding
+        if (s + pre <= steps) wait_loads_and_meet<(C::STAGES - 2) * C::PIECES>();
+        else wait_loads_and_meet<0>();
+        if (s + pre < steps) issue(s + pre, fill);
+        const char* pa = fa + slot * C::STAGE_BYTES;
+        const char* pb = fb + slot * C::STAGE_BYTES;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 a[C::TM], b[C::TN];
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048 + (h ? x1 : x0));
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048 + (h ? x1 : x0));
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
+        }
+        slot = slot + 1 == C::STAGES ? 0 : slot + 1;
+        fill = fill + 1 == C::STAGES ? 0 : fill + 1;
+    }
+    wait_loads_and_meet<0>();           // the LDS of the last step is free for the epilogue
+}
+
+// Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn; every XCD gets a contiguous
+// range of tiles, walked in patches of 8 rows of tiles, so that what its L2 holds is used again.
+NK_D void tile_of(int64_t id, int64_t mt, int64_t nt, int64_t* m, int64_t* n) {
+    const int64_t total = mt * nt;
+    const int64_t per = total / 8, extra = total % 8, x = id % 8;
+    const int64_t t = x * per + (x < extra ? x : extra) + id / 8;
+    const int64_t band = 8 * nt, b = t / band, left = mt - b * 8, h = left < 8 ? left : 8;
+    const int64_t r = t - b * band;
+    *m = b * 8 + r % h;
+    *n = r / h;
+}
+
+// ---- forward ----------------------------------------------------------------------------------
+struct LseArgs {
+    Mat w, h;
+    int64_t kbytes, v0, V, N;              // rows v0 .. of the vocabulary are w's rows 0 ..
+    const int64_t* target;
+    float2* part; int64_t part0;            // [tile of vocabulary][token]: maximum, sum of exponentials
+    float* zt;                              // logit of the target
+};
+
+template <typename T, class C>
+__global__ __launch_bounds__(C::THREADS) void k_xent_lse(const LseArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    int64_t mi, ni;
+    tile_of(blockIdx.x, (g.w.rows + C::BM - 1) / C::BM, (g.N + C::BN - 1) / C::BN, &mi, &ni);
+    f32x4 acc[C::TM][C::TN];
+    tile_product<T, C>(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
+    float2* meet = (float2*)lds;            // [WGM][BN]
+    const int64_t row0 = mi * C::BM + wm * C::TM * 16 + 4 * (lane >> 4);       // of w; rows row0 + 16 i + e
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+        const int col = wn * C::TN * 16 + j * 16 + (lane & 15);
+        const int64_t n = ni * C::BN + col;
+        const int64_t t = n < g.N ? g.target[n] - g.v0 : -1;
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t v = row0 + 16 * i + e;
+                if (v >= g.w.rows) acc[i][j][e] = -__builtin_inff();
+                else if (v == t) g.zt[n] = acc[i][j][e];
+                m = fmaxf(m, acc[i][j][e]);
+            }
+        const float ms = m == -__builtin_inff() ? 0.0f : m;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - ms) * LOG2E);
+#pragma unroll
+        for (int off = 16; off < 64; off <<= 1) {
+            const float mo = __shfl_xor(m, off, 64), so = __shfl_xor(s, off, 64);
+            const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
+            s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
+            m = mn;
+        }
+        if (lane < 16) meet[wm * C::BN + col] = make_float2(m, s);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < C::BN; c += C::THREADS) {
+        const int64_t n = ni * C::BN + c;
+        if (n >= g.N) break;
+        float m = meet[c].x, s = meet[c].y;
+#pragma unroll
+        for (int w = 1; w < C::WGM; ++w) {
+            const float mo = meet[w * C::BN + c].x, so = meet[w * C::BN + c].y;
+            const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
+            s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
+            m = mn;
+        }
+        g.part[(g.part0 + mi) * g.N + n] = make_float2(m, s);
+    }
+}
+
+// lse and loss of 16 tokens: 16 threads a token take the tiles in turn, then meet
+__global__ __launch_bounds__(256) void k_xent_join(const float2* __restrict__ part, int64_t tiles, int64_t N, int64_t V,
+                                                   const int64_t* __restrict__ target, int64_t ignore, const float* __restrict__ zt,
+                                                   float* __restrict__ lse, float* __restrict__ loss) {
+    __shared__ float2 meet[16][17];
+    const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int64_t n = (int64_t)blockIdx.x * 16 + c;
+    float m = -__builtin_inff(), s = 0.0f;
+    if (n < N)
+        for (int64_t t = q; t < tiles; t += 16) {
+            const float2 p = part[t * N + n];
+            const float mn = fmaxf(m, p.x), mz = mn == -__builtin_inff() ? 0.0f : mn;
+            s = s * expf(m - mz) + p.y * expf(p.x - mz);
+            m = mn;
+        }
+    meet[q][c] = make_float2(m, s);
+    __syncthreads();
+    if (q == 0 && n < N) {
+        for (int k = 1; k < 16; ++k) {
+            const float2 p = meet[k][c];
+            const float mn = fmaxf(m, p.x), mz = mn == -__builtin_inff() ? 0.0f : mn;
+            s = s * expf(m - mz) + p.y * expf(p.x - mz);
+            m = mn;
+        }
+        const float l = m + logf(s);
+        const int64_t t = target[n];
+        lse[n] = l;
+        loss[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : l - zt[n];
+    }
+}
+
+// sum (and mean over the tokens that count) in one order: one workgroup
+__global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ loss, const int64_t* __restrict__ target, int64_t N,
+                                                      int64_t ignore, int mean, float* __restrict__ out) {
+    __shared__ double sums[16];
+    __shared__ int64_t counts[16];
+    double s = 0.0;
+    int64_t k = 0;
+    for (int64_t n = threadIdx.x; n < N; n += 1024) { s += (double)loss[n]; k += target[n] != ignore; }
+    for (int off = 32; off > 0; off >>= 1) { s += __shfl_xor(s, off, 64); k += __shfl_xor((int)k, off, 64); }
+    if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = s; counts[threadIdx.x >> 6] = k; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) { s += sums[w]; k += counts[w]; }
+        out[0] = (float)(mean ? s / (double)(k > 0 ? k : 1) : s);
+    }
+}
+
+// ---- backward ---------------------------------------------------------------------------------
+// Row factors of dz and the factor that is left for the end: the products see dz with |c| <= 1.
+//   mean / sum: c = 1 for tokens that count, rest = d_loss / count or d_loss
+//   none:       c = d_loss_n / rest with rest the power of two above the largest |d_loss|
+__global__ __launch_bounds__(1024) void k_xent_factors(const int64_t* __restrict__ target, int64_t N, int64_t V, int64_t ignore, int reduction,
+                                                       const float* __restrict__ d_loss, float* __restrict__ c, float* __restrict__ rest) {
+    __shared__ int64_t counts[16];
+    __shared__ uint32_t peaks[16];
+    __shared__ float unit;
+    int64_t k = 0;
+    uint32_t peak = 0;
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+        const bool on = target[n] != ignore;
+        k += on;
+        if (reduction == NK_REDUCE_NONE && on) peak = max(peak, __float_as_uint(d_loss[n]) & 0x7FFFFFFFu);
+    }
+    for (int off = 32; off > 0; off >>= 1) { k += __shfl_xor((int)k, off, 64); peak = max(peak, (uint32_t)__shfl_xor((int)peak, off, 64)); }
+    if ((threadIdx.x & 63) == 0) { counts[threadIdx.x >> 6] = k; peaks[threadIdx.x >> 6] = peak; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) { k += counts[w]; peak = max(peak, peaks[w]); }
+        if (reduction == NK_REDUCE_NONE) {
+            const int e = min(max((int)(peak >> 23) + 1, 27), 227);          // 2^-100 .. 2^100; infinities and NaN stay in c
+            unit = __uint_as_float((uint32_t)(254 - e) << 23);
+            *rest = __uint_as_float((uint32_t)e << 23);
+        } else {
+            unit = 1.0f;
+            *rest = reduction == NK_REDUCE_MEAN ? d_loss[0] / (float)(k > 0 ? k : 1) : d_loss[0];
+        }
+    }
+    __syncthreads();
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+        const int64_t t = target[n];
+        c[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : reduction == NK_REDUCE_NONE ? d_loss[n] * unit : 1.0f;
+    }
+}
+
+struct DzArgs {
+    Mat w, h;
+    int64_t kbytes, v0, N;
+    const int64_t* target;
+    const float* lse; const float* c;
+    void* dz; int64_t dz_ld;                // [token][row of the piece]
+    void* dzt; int64_t dzt_ld;              // [row of the piece][token], zero up to dzt_ld
+};
+
+// 4 x 4 transpose of 16-bit values over the four lanes of a quad: in, p = elements 0..3 of this lane's column;
+// out, element (lane & 3) of the quad's four columns
+NK_D u32x2 quad_transpose(u32x2 p, int lane) {
+    const bool b0 = lane & 1, b1 = lane & 2;
+    const uint32_t x = b1 ? p[1] : p[0];
+    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)(b1 ? p[0] : p[1]), 0x4E, 0xF, 0xF, true);      // from lane ^ 2
+    // x: elements 2 b1, 2 b1 + 1 of this column; y: of column ^ 2
+    const uint32_t lo = (x & 0xFFFFu) | (y << 16), hi = (x >> 16) | (y & 0xFFFF0000u);
+    uint32_t keep = b0 ? hi : lo;                                                                              // columns own, own ^ 2
+    uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(b0 ? lo : hi), 0xB1, 0xF, 0xF, true);              // columns own ^ 1, own ^ 3
+    if (b1) { keep = (keep >> 16) | (keep << 16); got = (got >> 16) | (got << 16); }
+    const uint32_t even = b0 ? got : keep, odd = b0 ? keep : got;
+    return u32x2{(even & 0xFFFFu) | (odd << 16), (even >> 16) | (odd & 0xFFFF0000u)};
+}
+
+template <typename T, class C>
+__global__ __launch_bounds__(C::THREADS) void k_xent_dz(const DzArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    int64_t mi, ni;
+    // up to the padded token count: those columns of dzt have to be zero
+    tile_of(blockIdx.x, (g.w.rows + C::BM - 1) / C::BM, (g.dzt_ld + C::BN - 1) / C::BN, &mi, &ni);
+    f32x4 acc[C::TM][C::TN];
+    tile_product<T, C>(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
+    const int64_t row0 = mi * C::BM + wm * C::TM * 16 + 4 * (lane >> 4);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+        const int64_t n = ni * C::BN + wn * C::TN * 16 + j * 16 + (lane & 15);
+        const bool in = n < g.N;
+        const int64_t t = in ? g.target[n] - g.v0 : -1;
+        const float lse = in ? g.lse[n] : 0.0f, c = in ? g.c[n] : 0.0f, cs = c * Op<T>::SCALE;
+        T* dz = (T*)g.dz + n * g.dz_ld;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+            const int64_t v = row0 + 16 * i;
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float p = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
+                if (v + e == t) p -= 1.0f;
+                d[e] = (c == 0.0f || v + e >= g.w.rows) ? 0.0f : p * cs;
+            }
+            if constexpr (sizeof(T) == 2) {
+                typedef __attribute__((ext_vector_type(4))) T vec;
+                vec w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (T)d[e];
+                const u32x2 p = __builtin_bit_cast(u32x2, w);
+                if (in && v < g.dz_ld) *(u32x2*)(dz + v) = p;
+                const u32x2 q = quad_transpose(p, lane);
+                const int64_t n4 = n - (lane & 3), vt = v + (lane & 3);
+                if (n4 < g.dzt_ld && vt < g.w.rows) *(u32x2*)((T*)g.dzt + vt * g.dzt_ld + n4) = q;
+            } else {
+                if (in && v < g.dz_ld) *(float4*)(dz + v) = make_float4(d[0], d[1], d[2], d[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n < g.dzt_ld && v + e < g.w.rows) ((T*)g.dzt)[(v + e) * g.dzt_ld + n] = (T)d[e];
+            }
+        }
+    }
+}
+
+struct ProductArgs {
+    Mat a, b;
+    int64_t k0, kbytes, kslice;             // bytes of k: slice z takes k0 + z * kslice .. (kslice a multiple of 128)
+    int64_t M, N;
+    void* out; int64_t ld;                  // [n][m]
+    float* sums; int add;                   // fp32 sums [slice][n][m] instead; add: onto what is there
+    const float* rest; float scale;
+};
+
+// C[m][n] -> out[n][m]: a lane holds four consecutive m of one n
+template <typename T, class C, bool SUMS>
+__global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    int64_t mi, ni;
+    tile_of(blockIdx.x, (g.M + C::BM - 1) / C::BM, (g.N + C::BN - 1) / C::BN, &mi, &ni);
+    const int64_t at = blockIdx.y * g.kslice, left = g.kbytes - at;
+    Mat a = g.a, b = g.b;
+    a.p += at; b.p += at;
+    f32x4 acc[C::TM][C::TN];
+    tile_product<T, C>(a, b, mi * C::BM, ni * C::BN, left < 0 ? 0 : left < g.kslice ? left : g.kslice, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
+    const float f = SUMS ? 1.0f : *g.rest * g.scale;
+    const bool vec = SUMS ? (g.M & 3) == 0 : (g.ld & 3) == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+        const int64_t n = ni * C::BN + wn * C::TN * 16 + j * 16 + (lane & 15);
+        if (n >= g.N) continue;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+            const int64_t m = mi * C::BM + wm * C::TM * 16 + i * 16 + 4 * (lane >> 4);
+            if (m >= g.M) continue;
+            if (SUMS) {
+                float* s = g.sums + (blockIdx.y * g.N + n) * g.M + m;
+                if (vec) {
+                    f32x4 o = acc[i][j];
+                    if (g.add) o += *(f32x4*)s;
+                    *(f32x4*)s = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (m + e < g.M) s[e] = acc[i][j][e] + (g.add ? s[e] : 0.0f);
+                }
+            } else {
+                T* o = (T*)g.out + n * g.ld + m;
+                if (vec && m + 4 <= g.M) {
+                    typedef __attribute__((ext_vector_type(4))) T vt;
+                    vt w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = (T)(acc[i][j][e] * f);
+                    *(vt*)o = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (m + e < g.M) o[e] = (T)(acc[i][j][e] * f);
+                }
+            }
+        }
+    }
+}
+
+// d_hidden from its fp32 sums; tokens that do not count have none
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ sums, int slices, int64_t N, int64_t D, const float* __restrict__ c,
+                                                     const float* __restrict__ rest, float scale, T* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= N * D) return;
+    float s = 0.0f;
+    for (int k = 0; k < slices; ++k) s += sums[(int64_t)k * N * D + i];
+    out[i] = (T)(c[i / D] == 0.0f ? 0.0f : s * (*rest * scale));
+}
+
+// dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, T* __restrict__ dst, int64_t dst_ld) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * dst_ld) return;
+    const int64_t r = i / dst_ld, c = i - r * dst_ld;
+    dst[i] = c < cols ? src[r * ld + c] : (T)0.0f;
+}
+
+// dst[c][0 .. dst_ld) = src[0 .. rows)[c], zeros behind; rows with factor c = 0 are left out as zeros (their
+// values may be anything)
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_transpose(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
+                                                        const float* __restrict__ factor, T* __restrict__ dst, int64_t dst_ld) {
+    __shared__ T tile[64][64 + 4 / sizeof(T)];
+    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int k = y; k < 64; k += 4) {
+        const int64_t r = r0 + k, c = c0 + x;
+        T v = (T)0.0f;
+        if (r < rows && c < cols && !(factor && factor[r] == 0.0f)) v = src[r * ld + c];
+        tile[k][x] = v;
+    }
+    __syncthreads();
+    for (int k = y; k < 64; k += 4) {
+        const int64_t c = c0 + k, r = r0 + x;
+        if (c < cols && r < dst_ld) dst[c * dst_ld + r] = tile[x][k];
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------
+typedef Cfg<256, 256, 2, 4, 2> Large;
+typedef Cfg<128, 128, 2, 2, 2> Middle;
+typedef Cfg<128, 32, 4, 1, 4> Few;
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
+
+template <auto K, typename ARGS>
+int start(const ARGS& args, int64_t blocks, int slices, int threads, hipStream_t st, const char* name) {
+    if (blocks > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+    hipLaunchKernelGGL(K, dim3((unsigned)blocks, (unsigned)slices), dim3(threads), 0, st, args);
+    NK_CHECK_LAUNCH(name);
+    return NK_OK;
+}
+
+// Which tile: 0 large, 1 middle, 2 few columns.
+int tile_kind(int64_t M, int64_t N) {
+    if (N <= 32) return 2;
+    return cdiv(M, 256) * cdiv(N, 256) >= 224 ? 0 : 1;
+}
+int kind_bm(int kind) { return kind == 0 ? 256 : 128; }
+
+struct Plan {
+    int64_t Dp, Np, piece;                  // padded k of the logits' product; tokens padded to a step; vocabulary rows per piece
+    bool pad_h, pad_w;
+    int kind, slices;
+    int64_t parts, zt, h, w, c, rest, wt, ht, dz, dzt, sums, total;
+};
+
+int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int backward, Plan* p, const char* who) {
+    if (!o) NK_FAIL(NK_ERR_ARG, "%s: null options", who);
+    if (o->N < 0 || o->D < 1 || o->V < 1) NK_FAIL(NK_ERR_ARG, "%s: N=%lld D=%lld V=%lld", who, (long long)o->N, (long long)o->D, (long long)o->V);
+    if (o->dtype < NK_F32 || o->dtype > NK_F16) NK_FAIL(NK_ERR_ARG, "%s: unknown dtype %d", who, o->dtype);
+    if (o->reduction < NK_REDUCE_NONE || o->reduction > NK_REDUCE_SUM) NK_FAIL(NK_ERR_ARG, "%s: unknown reduction %d", who, o->reduction);
+    if (o->hidden_stride < o->D || o->weight_stride < o->D) NK_FAIL(NK_ERR_ARG, "%s: row strides below D", who);
+    if (o->piece < 0) NK_FAIL(NK_ERR_ARG, "%s: piece < 0", who);
+    const int es = elem(o->dtype);
+    // 256 rows of an operand are addressed with 31 bits
+    if (o->D > (1 << 20) || o->hidden_stride * es > (1 << 22) || o->weight_stride * es > (1 << 22) || o->N > (1 << 24) || o->V > (1 << 26))
+        NK_FAIL(NK_ERR_UNSUPPORTED, "%s: D up to 2^20, row strides up to 2^22 bytes, N up to 2^24, V up to 2^26", who);
+    const int64_t step = 128 / es;          // elements of k per step
+    p->Dp = up(o->D, step);
+    auto aligned = [&](const void* q, int64_t stride) { return ((uintptr_t)q & 15) == 0 && (stride * es) % 16 == 0 && (o->D * es) % 16 == 0; };
+    p->pad_h = !aligned(hidden, o->hidden_stride); p->pad_w = !aligned(weight, o->weight_stride);
+    p->Np = up(o->N, step);
+    int64_t piece;
+    if (backward) {
+        piece = o->piece ? up(o->piece, 256) : up((int64_t)(NK_XENT_PIECE_MB / 2 << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
+        if (piece < 2048 && !o->piece) piece = 2048;
+    } else {
+        piece = p->pad_w ? (o->piece ? up(o->piece, 256) : 16384) : up(o->V, 256);
+    }
+    if (piece > up(o->V, 256)) piece = up(o->V, 256);
+    p->piece = piece;
+    int64_t off = 0;
+    auto take = [&](int64_t bytes) { const int64_t at = off; off = up(off + bytes, 1024); return at; };
+    p->h = take(p->pad_h ? o->N * p->Dp * es : 0);
+    p->w = take(p->pad_w ? piece * p->Dp * es : 0);
+    p->kind = tile_kind(piece < o->V ? piece : o->V, o->N);
+    p->slices = 1;
+    if (!backward) {
+        p->parts = take(cdiv(o->V, piece) * (piece / kind_bm(p->kind)) * o->N * 8);
+        p->zt = take(o->N * 4);
+    } else {
+        p->c = take(o->N * 4);
+        p->rest = take(4);
+        p->wt = take(o->D * piece * es);
+        p->ht = take(o->D * p->Np * es);
+        p->dz = take(o->N * piece * es);
+        p->dzt = take(piece * p->Np * es);
+        // d_hidden has few tiles: cut its k (the piece) until they fill the chip
+        const int64_t tiles = cdiv(o->D, 128) * cdiv(o->N, o->N <= 32 ? 32 : 128), most = piece / (8 * step);
+        int64_t s = tiles >= 256 || tiles < 1 ? 1 : cdiv(512, tiles);
+        if (s > most) s = most;
+        if (s > 16) s = 16;
+        p->slices = (int)(s < 1 ? 1 : s);
+        p->sums = take((int64_t)p->slices * o->N * o->D * 4);
+    }
+    p->total = off;
+    return NK_OK;
+}
+
+template <typename T> int lse_launch(int kind, const LseArgs& g, hipStream_t st) {
+    const int64_t M = g.w.rows, N = g.N;
+    if (kind == 0) return start<k_xent_lse<T, Large>>(g, cdiv(M, 256) * cdiv(N, 256), 1, Large::THREADS, st, "k_xent_lse");
+    if (kind == 1) return start<k_xent_lse<T, Middle>>(g, cdiv(M, 128) * cdiv(N, 128), 1, Middle::THREADS, st, "k_xent_lse");
+    return start<k_xent_lse<T, Few>>(g, cdiv(M, 128) * cdiv(N, 32), 1, Few::THREADS, st, "k_xent_lse");
+}
+template <typename T> int dz_launch(int kind, const DzArgs& g, hipStream_t st) {
+    const int64_t M = g.w.rows;
+    if (kind == 0) return start<k_xent_dz<T, Large>>(g, cdiv(M, 256) * cdiv(g.dzt_ld, 256), 1, Large::THREADS, st, "k_xent_dz");
+    if (kind == 1) return start<k_xent_dz<T, Middle>>(g, cdiv(M, 128) * cdiv(g.dzt_ld, 128), 1, Middle::THREADS, st, "k_xent_dz");
+    return start<k_xent_dz<T, Few>>(g, cdiv(M, 128) * cdiv(g.dzt_ld, 32), 1, Few::THREADS, st, "k_xent_dz");
+}
+template <typename T, bool SUMS> int product_launch(const ProductArgs& g, int slices, hipStream_t st) {
+    const int kind = g.N <= 32 ? 2 : cdiv(g.M, 256) * cdiv(g.N, 256) * slices >= 224 ? 0 : 1;
+    if (kind == 0) return start<k_xent_product<T, Large, SUMS>>(g, cdiv(g.M, 256) * cdiv(g.N, 256), slices, Large::THREADS, st, "k_xent_product");
+    if (kind == 1) return start<k_xent_product<T, Middle, SUMS>>(g, cdiv(g.M, 128) * cdiv(g.N, 128), slices, Middle::THREADS, st, "k_xent_product");
+    return start<k_xent_product<T, Few, SUMS>>(g, cdiv(g.M, 128) * cdiv(g.N, 32), slices, Few::THREADS, st, "k_xent_product");
+}
+
+template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t dst_ld, hipStream_t st) {
+    const int64_t n = rows * dst_ld;
+    if (cdiv(n, 256) > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "k_xent_pad: too large");
+    hipLaunchKernelGGL(k_xent_pad<T>, dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, (const T*)src, ld, rows, cols, (T*)dst, dst_ld);
+    NK_CHECK_LAUNCH("k_xent_pad");
+    return NK_OK;
+}
+template <typename T> int transpose(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* factor, void* dst, int64_t dst_ld, hipStream_t st) {
+    hipLaunchKernelGGL(k_xent_transpose<T>, dim3((unsigned)cdiv(dst_ld, 64), (unsigned)cdiv(cols, 64)), dim3(256), 0, st, (const T*)src, ld, rows, cols,
+                       factor, (T*)dst, dst_ld);
+    NK_CHECK_LAUNCH("k_xent_transpose");
+    return NK_OK;
+}
+
+template <typename T>
+int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse, float* reduced,
+            char* ws, hipStream_t st) {
+    const int es = sizeof(T);
+    int rc;
+    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es};
+    if (p.pad_h) {
+        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, ws + p.h, p.Dp, st)) < 0) return rc;
+        h = Mat{ws + p.h, o->N, p.Dp * es};
+    }
+    int64_t tiles = 0;
+    for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
+        const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
+        const char* src = (const char*)weight + v0 * o->weight_stride * es;
+        Mat w = {src, rows, o->weight_stride * es};
+        if (p.pad_w) {
+            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, ws + p.w, p.Dp, st)) < 0) return rc;
+            w = Mat{ws + p.w, rows, p.Dp * es};
+        }
+        const LseArgs g = {w, h, o->D * es, v0, o->V, o->N, target, (float2*)(ws + p.parts), tiles, (float*)(ws + p.zt)};
+        if ((rc = lse_launch<T>(p.kind, g, st)) < 0) return rc;
+        tiles += cdiv(rows, kind_bm(p.kind));
+    }
+    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)cdiv(o->N, 16)), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V, target,
+                       o->ignore_index, (const float*)(ws + p.zt), lse, loss);
+    NK_CHECK_LAUNCH("k_xent_join");
+    if (o->reduction != NK_REDUCE_NONE) {
+        hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, loss, target, o->N, o->ignore_index, o->reduction == NK_REDUCE_MEAN, reduced);
+        NK_CHECK_LAUNCH("k_xent_reduce");
+    }
+    return NK_OK;
+}
+
+template <typename T>
+int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void* weight, const int64_t* target, const float* lse, const float* d_loss,
+             void* d_hidden, void* d_weight, char* ws, hipStream_t st) {
+    const int es = sizeof(T);
+    const float unscale = 1.0f / Op<T>::SCALE;
+    float* c = (float*)(ws + p.c);
+    float* rest = (float*)(ws + p.rest);
+    int rc;
+    hipLaunchKernelGGL(k_xent_factors, dim3(1), dim3(1024), 0, st, target, o->N, o->V, o->ignore_index, o->reduction, d_loss, c, rest);
+    NK_CHECK_LAUNCH("k_xent_factors");
+    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es};
+    if (p.pad_h) {
+        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, ws + p.h, p.Dp, st)) < 0) return rc;
+        h = Mat{ws + p.h, o->N, p.Dp * es};
+    }
+    if (d_weight && (rc = transpose<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.ht, p.Np, st)) < 0) return rc;
+    const int64_t slice = up(cdiv(p.piece, p.slices), 128 / es) * es;
+    for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
+        const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
+        const char* src = (const char*)weight + v0 * o->weight_stride * es;
+        Mat w = {src, rows, o->weight_stride * es};
+        if (p.pad_w) {
+            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, ws + p.w, p.Dp, st)) < 0) return rc;
+            w = Mat{ws + p.w, rows, p.Dp * es};
+        }
+        const int64_t kv = up(rows, 128 / es);          // columns of dz that the product takes: zeros behind `rows`
+        const DzArgs g = {w, h, o->D * es, v0, o->N, target, lse, c, ws + p.dz, kv, ws + p.dzt, p.Np};
+        if ((rc = dz_launch<T>(tile_kind(rows, o->N), g, st)) < 0) return rc;
+        if (d_weight) {
+            ProductArgs q = {};
+            q.a = Mat{ws + p.ht, o->D, p.Np * es}; q.b = Mat{ws + p.dzt, rows, p.Np * es};
+            q.kbytes = q.kslice = p.Np * es; q.M = o->D; q.N = rows;
+            q.out = (char*)d_weight + v0 * o->D * es; q.ld = o->D; q.rest = rest; q.scale = unscale;
+            if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+        }
+        if (d_hidden) {
+            if ((rc = transpose<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.wt, kv, st)) < 0) return rc;
+            ProductArgs q = {};
+            q.a = Mat{ws + p.wt, o->D, kv * es}; q.b = Mat{ws + p.dz, o->N, kv * es};
+            q.kbytes = kv * es; q.kslice = slice; q.M = o->D; q.N = o->N;
+            q.sums = (float*)(ws + p.sums); q.add = v0 > 0;
+            if ((rc = product_launch<T, true>(q, p.slices, st)) < 0) return rc;
+        }
+    }
+    if (d_hidden) {
+        const int64_t n = o->N * o->D;
+        if (cdiv(n, 256) > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_linear_xent_bwd: too large");
+        hipLaunchKernelGGL(k_xent_finish<T>, dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c, rest,
+                           unscale, (T*)d_hidden);
+        NK_CHECK_LAUNCH("k_xent_finish");
+    }
+    return NK_OK;
+}
+
+int check_ws(const Plan& p, const void* ws, int64_t bytes, const char* who) {
+    if (bytes < p.total || (p.total > 0 && (!ws || ((uintptr_t)ws & 255))))
+        NK_FAIL(NK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who, (long long)bytes, (long long)p.total);
+    return NK_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* o, const void* hidden, const void* weight, int backward) {
+    Plan p;
+    const int rc = plan_of(o, hidden, weight, backward, &p, "nk_linear_xent_workspace_bytes");
+    return rc < 0 ? rc : p.total;
+}
+
+extern "C" int nk_linear_xent_fwd(const nk_xent_opts* o, const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,
+                                  float* reduced, void* workspace, int64_t workspace_bytes, void* stream) {
+    Plan p;
+    int rc = plan_of(o, hidden, weight, 0, &p, "nk_linear_xent_fwd");
+    if (rc < 0) return rc;
+    if (o->reduction != NK_REDUCE_NONE && !reduced) NK_FAIL(NK_ERR_ARG, "nk_linear_xent_fwd: the reduction needs `reduced`");
+    if (o->N > 0 && (!hidden || !weight || !target || !loss || !lse)) NK_FAIL(NK_ERR_ARG, "nk_linear_xent_fwd: null pointer");
+    if ((rc = check_ws(p, workspace, workspace_bytes, "nk_linear_xent_fwd")) < 0) return rc;
+    const hipStream_t st = nk_stream(stream);
+    if (o->N == 0) {
+        if (o->reduction != NK_REDUCE_NONE) {
+            hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, loss, target, (int64_t)0, o->ignore_index, 0, reduced);
+            NK_CHECK_LAUNCH("k_xent_reduce");
+        }
+        return NK_OK;
+    }
+    char* ws = (char*)workspace;
+    if (o->dtype == NK_BF16) return forward<__bf16>(o, p, hidden, weight, target, loss, lse, reduced, ws, st);
+    if (o->dtype == NK_F16) return forward<_Float16>(o, p, hidden, weight, target, loss, lse, reduced, ws, st);
+    return forward<float>(o, p, hidden, weight, target, loss, lse, reduced, ws, st);
+}
+
+extern "C" int nk_linear_xent_bwd(const nk_xent_opts* o, const void* hidden, const void* weight, const int64_t* target, const float* lse,
+                                  const float* d_loss, void* d_hidden, void* d_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+    Plan p;
+    int rc = plan_of(o, hidden, weight, 1, &p, "nk_linear_xent_bwd");
+    if (rc < 0) return rc;
+    if (o->N < 1) NK_FAIL(NK_ERR_ARG, "nk_linear_xent_bwd: no tokens");
+    if (!hidden || !weight || !target || !lse || !d_loss || (!d_hidden && !d_weight)) NK_FAIL(NK_ERR_ARG, "nk_linear_xent_bwd: null pointer");
+    if ((rc = check_ws(p, workspace, workspace_bytes, "nk_linear_xent_bwd")) < 0) return rc;
+    const hipStream_t st = nk_stream(stream);
+    char* ws = (char*)workspace;
+    if (o->dtype == NK_BF16) return backward<__bf16>(o, p, hidden, weight, target, lse, d_loss, d_hidden, d_weight, ws, st);
+    if (o->dtype == NK_F16) return backward<_Float16>(o, p, hidden, weight, target, lse, d_loss, d_hidden, d_weight, ws, st);
+    return backward<float>(o, p, hidden, weight, target, lse, d_loss, d_hidden, d_weight, ws, st);
+}

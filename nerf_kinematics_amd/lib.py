@@ -67,6 +67,14 @@ class NkScanOpts(C.Structure):
                                               "g_stride_t")] + [("lengths", C.c_void_p)])
 
 
+class NkXentOpts(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("N", "D", "V", "hidden_stride", "weight_stride", "ignore_index")]
+                + [("dtype", C.c_int32), ("reduction", C.c_int32), ("piece", C.c_int64)])
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
 class NkAdamwTensor(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "master", "scale_m", "scale_v")] + [("n", C.c_int64)]
 
@@ -94,6 +102,9 @@ SIGNATURES = {
     "nk_sample_training_rays_dev": (C.c_int, [_P, _I32, _P, _I64, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
     "nk_set_step_state": (C.c_int, [C.POINTER(NkStepState), _P, _P]),
     "nk_adam_step_dev": (C.c_int, [_P, _P, _P, _P, _I64, _P, C.c_double, C.c_double, C.c_double, _F, _P]),
+    "nk_linear_xent_workspace_bytes": (_I64, [C.POINTER(NkXentOpts), _P, _P, C.c_int]),
+    "nk_linear_xent_fwd": (C.c_int, [C.POINTER(NkXentOpts), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "nk_linear_xent_bwd": (C.c_int, [C.POINTER(NkXentOpts), _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "nk_gated_scan_workspace_bytes": (_I64, [C.POINTER(NkScanOpts), C.c_int]),
     "nk_gated_scan_fwd": (C.c_int, [C.POINTER(NkScanOpts), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "nk_gated_scan_states_bytes": (_I64, [C.POINTER(NkScanOpts)]),

@@ -1,0 +1,101 @@
+"""Softmax cross entropy of a linear head without the logits, differentiable (``nk_linear_xent_fwd`` / ``_bwd``).
+
+Stands beside :func:`~nerf_kinematics_amd.render.mse_loss`: the loss of a field that answers with one of many
+labels instead of a colour.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import lib as _lib
+from .scan import _call, _ptr
+
+
+def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
+    N, D = hidden.shape
+    return _lib.NkXentOpts(N, D, weight.shape[0], hidden.stride(0), weight.stride(0), ignore_index, _lib.DTYPES[hidden.dtype],
+                           reduction, piece)
+
+
+def _workspace(L, o, hidden, weight, backward):
+    n = _lib.check(L.nk_linear_xent_workspace_bytes(o, hidden.data_ptr(), weight.data_ptr(), backward))
+    return torch.empty(n, dtype=torch.uint8, device=hidden.device), n
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` with unit stride along its rows, which do not overlap (a copy where they do)."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _forward(hidden, weight, target, o, reduction):
+    L = _lib.load()
+    N, dev = hidden.shape[0], hidden.device
+    loss, lse = torch.empty(2, N, dtype=torch.float32, device=dev).unbind(0)
+    total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
+    ws, n = _workspace(L, o, hidden, weight, 0)
+    _call(dev, L.nk_linear_xent_fwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(), lse.data_ptr(),
+          _ptr(total), ws.data_ptr(), n)
+    return (loss if total is None else total), lse
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, ignore_index, reduction, piece):
+        o = _opts(hidden, weight, ignore_index, reduction, piece)
+        loss, lse = _forward(hidden, weight, target, o, reduction)
+        ctx.save_for_backward(hidden, weight, target, lse)
+        ctx.opts = o
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss):
+        hidden, weight, target, lse = ctx.saved_tensors
+        dev = hidden.device
+        want_h, want_w = ctx.needs_input_grad[:2]
+        d_hidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
+        if hidden.shape[0] == 0:
+            return d_hidden, torch.zeros_like(weight) if want_w else None, None, None, None, None
+        d_weight = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
+        d_loss = d_loss.contiguous()
+        L = _lib.load()
+        ws, n = _workspace(L, ctx.opts, hidden, weight, 1)
+        _call(dev, L.nk_linear_xent_bwd, ctx.opts, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
+              d_loss.data_ptr(), _ptr(d_hidden), _ptr(d_weight), ws.data_ptr(), n)
+        return d_hidden, d_weight, None, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean", piece: int = 0) -> torch.Tensor:
+    """``cross_entropy(hidden @ weight.T, target)`` as float32, without holding the logits.
+
+    ``hidden`` [N, D] and ``weight`` [V, D] share a dtype (float32, bfloat16 or float16); ``target`` [N] is int64.
+    Tokens whose target is ``ignore_index`` have loss 0 and no gradient, whatever their row of ``hidden``
+    holds; any other target outside 0..V-1 makes its loss and the gradients NaN.  ``reduction`` is "mean" (over the
+    tokens that are not ignored; 0 without any), "sum" or "none" ([N] losses).
+
+    Differentiable in ``hidden`` and ``weight`` (first order).  The backward pass walks the vocabulary in pieces
+    of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB) and rounds the logit
+    gradients once to the operands' dtype between its products; sums are float32.
+    """
+    if reduction not in _lib.REDUCTIONS:
+        raise ValueError(f"reduction={reduction!r}: expected one of {sorted(_lib.REDUCTIONS)}")
+    if not isinstance(hidden, torch.Tensor) or hidden.dim() != 2 or hidden.dtype not in _lib.DTYPES or hidden.shape[1] < 1:
+        raise ValueError("hidden: expected a [N, D] tensor of float32, bfloat16 or float16")
+    N, D = hidden.shape
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != D or weight.shape[0] < 1 or weight.dtype != hidden.dtype:
+        raise ValueError(f"weight: expected a [V, {D}] tensor of {hidden.dtype}")
+    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64 or tuple(target.shape) != (N,):
+        raise ValueError(f"target: expected an int64 tensor of shape {(N,)}")
+    if piece < 0:
+        raise ValueError(f"piece={piece} (>= 0)")
+    dev = hidden.device
+    if dev.type != "cuda":
+        raise ValueError("hidden: expected a GPU tensor (there is no CPU implementation)")
+    if weight.device != dev or target.device != dev:
+        raise ValueError(f"weight, target: expected tensors on {dev}")
+    hidden, weight, target = _rows(hidden), _rows(weight), target.contiguous()
+    r = _lib.REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), r, int(piece))
+    return _forward(hidden, weight, target, _opts(hidden, weight, int(ignore_index), r, int(piece)), r)[0]
