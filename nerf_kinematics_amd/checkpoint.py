@@ -132,7 +132,7 @@ def state_from_checkpoint(ck: dict, arch_coarse: Arch, arch_fine: Optional[Arch]
 
 
 def checkpoint_from_state(s: TrainState, arch_coarse: Arch, arch_fine: Optional[Arch],
-                          betas=(0.9, 0.999), eps: float = 1e-8) -> dict:
+                          betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0) -> dict:
     ck = {"iter": int(s.iteration), "model_coarse_state_dict": split_flat(arch_coarse, s.coarse),
           "model_fine_state_dict": split_flat(arch_fine, s.fine) if s.fine is not None else None}
     archs = [arch_coarse] + ([arch_fine] if s.fine is not None else [])
@@ -148,7 +148,7 @@ def checkpoint_from_state(s: TrainState, arch_coarse: Arch, arch_fine: Optional[
                     entry["exp_avg_sq"] = s.exp_avg_sq[k][off:off + n].view(*shape).clone()
                 state[idx] = entry
                 off += n; idx += 1
-    group = {"lr": float(s.lr), "betas": tuple(betas), "eps": float(eps), "weight_decay": 0, "amsgrad": False,
+    group = {"lr": float(s.lr), "betas": tuple(betas), "eps": float(eps), "weight_decay": weight_decay, "amsgrad": False,
              "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
              "params": list(range(idx))}
     ck["optimizer_state_dict"] = {"state": state if s.exp_avg else {}, "param_groups": [group]}

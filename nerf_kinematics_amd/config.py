@@ -22,9 +22,10 @@ _RENDER_DEFAULT = {
     "chunksize": 131072, "lindisp": False, "num_coarse": 64, "num_fine": 64, "perturb": False,
     "radiance_field_noise_std": 0.0, "white_background": False,
 }
-# Two keys the reference's files do not have, both experiments that are off unless a file names them:
-#   nerf.train.act_format            "bf16" | "fp8" | "fp8bf8": format of the tensors saved for backward
-#   nerf.validation.skip_empty_eps   > 0: renders skip the fine network where the coarse pass saw nothing
+# Keys the reference's files do not have, all off unless a file names them:
+#   nerf.train.act_format            "bf16" | "fp8" | "fp8bf8": format of the tensors saved for backward (experiment)
+#   nerf.validation.skip_empty_eps   > 0: renders skip the fine network where the coarse pass saw nothing (experiment)
+#   optimizer.type: AdamW            with weight_decay (0.01) and state_bits (32 | 8: format of the moments)
 ACT_FORMATS = ("bf16", "fp8", "fp8bf8")
 DEFAULTS: Dict[str, Any] = {
     "dataset": {"type": "blender", "basedir": "cache/nerf_synthetic/lego", "cachedir": None, "near": 2, "far": 6,
@@ -91,8 +92,14 @@ def validate(cfg: dict) -> dict:
             raise ConfigError(f"nerf.{block}.num_coarse must be >= 2")
         if int(r["num_fine"]) < 0:
             raise ConfigError(f"nerf.{block}.num_fine must be >= 0")
-    if cfg["optimizer"].get("type", "Adam") != "Adam":
-        raise ConfigError(f"optimizer.type: only Adam is supported, got {cfg['optimizer']['type']!r}")
+    opt = cfg["optimizer"]
+    if opt.get("type", "Adam") not in ("Adam", "AdamW"):
+        raise ConfigError(f"optimizer.type: Adam or AdamW, got {opt['type']!r}")
+    if opt.get("type", "Adam") == "AdamW":
+        if int(opt.get("state_bits", 32)) not in (32, 8):
+            raise ConfigError(f"optimizer.state_bits: 32 or 8, got {opt['state_bits']!r}")
+        if not float(opt.get("weight_decay", 0.01)) >= 0.0:
+            raise ConfigError(f"optimizer.weight_decay: >= 0, got {opt['weight_decay']!r}")
     if cfg["dataset"]["type"] not in ("blender", "robot", "transforms", "teacher", "forward_grid"):
         raise ConfigError(f"dataset.type: unknown dataset type {cfg['dataset']['type']!r}")
     return cfg

@@ -205,7 +205,7 @@ extern "C" int nk_adamw_step(const nk_adamw_tensor* tensors, int32_t count, cons
     if (!o->state) {
         a.step_size = (float)(o->lr / (1.0 - pow(o->beta1, (double)o->step)));
         a.bc2_sqrt = (float)sqrt(1.0 - pow(o->beta2, (double)o->step));
-        a.decay = (float)(1.0 - o->lr * o->weight_decay);
+        a.decay = 1.0f - (float)(o->lr * o->weight_decay);         // as the kernel forms it from *state
     }
     a.gscale = o->grad_scale; a.seed = o->seed; a.st = o->state;
     int32_t k = 0;

@@ -69,12 +69,13 @@ def encode_moment(values: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tenso
     b = torch.nn.functional.pad(values.reshape(-1).float(), (0, -n % BLOCK)).view(-1, BLOCK)
     frac, e = torch.frexp(b.abs().amax(1, keepdim=True))
     e = torch.where(frac == 0, torch.full_like(e, -100), e - (frac == 0.5).to(e.dtype) - top).clamp_min(-100)
-    scaled = torch.ldexp(b, -e)
+    pow2 = lambda k: ((k.to(torch.int32) + 127) << 23).view(torch.float32)      # exact, which torch.ldexp is not on every device
+    scaled = b * pow2(-e)
     codes = scaled.to(dtype)
     if dtype == torch.float8_e5m2:       # a second moment stays positive
         least = torch.full_like(scaled, 2.0 ** -16).to(dtype)
         codes = torch.where((scaled > 0) & (codes.float() == 0), least.view(torch.uint8), codes.view(torch.uint8)).view(dtype)
-    return codes.reshape(-1)[:n].clone(), torch.ldexp(torch.ones_like(b[:, 0]), e[:, 0])
+    return codes.reshape(-1)[:n].clone(), pow2(e[:, 0])
 
 
 class AdamW:

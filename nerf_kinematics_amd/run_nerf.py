@@ -225,7 +225,8 @@ def main(argv=None) -> int:
         if rank == 0 and ((i % int(exp["save_every"]) == 0 and i > 0) or last):
             lv = float(loss)
             path = os.path.join(logdir, ckpt.checkpoint_name(i))
-            ckpt.save_checkpoint(path, tr.export_state(lv, mse2psnr(lv)), arch_c, arch_f, betas=opts.betas, eps=opts.eps)
+            ckpt.save_checkpoint(path, tr.export_state(lv, mse2psnr(lv)), arch_c, arch_f, betas=opts.betas, eps=opts.eps,
+                                 weight_decay=opts.weight_decay if opts.optimizer == "AdamW" else 0)
             print(f"saved {path}", flush=True)
     if log:
         log.close()

@@ -20,6 +20,7 @@ import torch
 
 from . import lib as _lib
 from .model import Arch, NeRFModel
+from .optim import AdamW, decode_moment, encode_moment
 from .render import make_opts, _ptr, _stream
 
 
@@ -42,6 +43,10 @@ class TrainOpts:
     # format of the tensors saved for backward (experiment, no counterpart in the reference):
     # "bf16" (default), "fp8" = e4m3 activations, "fp8bf8" = e4m3 activations and e5m2 dZ
     act_format: str = "bf16"
+    # "Adam" (the reference's) or "AdamW": decoupled weight decay, moments in 32 or 8 bits
+    optimizer: str = "Adam"
+    weight_decay: float = 0.01
+    state_bits: int = 32
 
     @staticmethod
     def from_config(cfg: dict) -> "TrainOpts":
@@ -54,7 +59,8 @@ class TrainOpts:
                          white_background=bool(t.get("white_background", False)), lr=float(o.get("lr", 5e-4)),
                          lr_decay=int(s.get("lr_decay", 250)), lr_decay_factor=float(s.get("lr_decay_factor", 0.1)),
                          seed=int(cfg.get("experiment", {}).get("randomseed", 42)),
-                         act_format=str(t.get("act_format", "bf16")))
+                         act_format=str(t.get("act_format", "bf16")), optimizer=str(o.get("type", "Adam")),
+                         weight_decay=float(o.get("weight_decay", 0.01)), state_bits=int(o.get("state_bits", 32)))
 
 
 def lr_at(iteration: int, o: TrainOpts) -> float:
@@ -89,8 +95,15 @@ class Trainer:
         self._grad_loss = torch.zeros(n_pad + 64, dtype=torch.float32, device=self.device)
         self.grad = self._grad_loss[:nc_pad + nf]
         self.loss = self._grad_loss[n_pad:n_pad + 1]
-        self.exp_avg = torch.zeros_like(self.params)
-        self.exp_avg_sq = torch.zeros_like(self.params)
+        if opts.optimizer not in ("Adam", "AdamW"):
+            raise ValueError(f"optimizer={opts.optimizer!r}: Adam or AdamW")
+        self._adamw = None
+        if opts.optimizer == "AdamW":       # both networks as one tensor of the multi-tensor step
+            self._adamw = AdamW([self.params], opts.lr, opts.betas, opts.eps, opts.weight_decay, state_bits=opts.state_bits)
+            self.exp_avg, self.exp_avg_sq = self._adamw.exp_avgs[0], self._adamw.exp_avg_sqs[0]
+        else:
+            self.exp_avg = torch.zeros_like(self.params)
+            self.exp_avg_sq = torch.zeros_like(self.params)
         self.coarse = NeRFModel(arch_coarse, self.params[:nc])
         self.fine = NeRFModel(arch_fine, self.params[nc_pad:]) if use_fine else None
         self._nc, self._nc_pad = nc, nc_pad
@@ -183,10 +196,15 @@ class Trainer:
                 self.comm_events.append(timed)
             self.iteration += 1
             self.opt_steps += 1
-            _lib.check(L.nk_adam_step(self.params.data_ptr(), self.grad.data_ptr(), self.exp_avg.data_ptr(),
-                                      self.exp_avg_sq.data_ptr(), self.params.numel(), self.opt_steps,
-                                      lr_at(self.iteration - 1, self.opts), self.opts.betas[0], self.opts.betas[1],
-                                      self.opts.eps, 1.0 / self.world, st))
+            lr = lr_at(self.iteration - 1, self.opts)
+            if self._adamw is not None:
+                # the rounding of 8-bit moments is the same on every rank: their replicas stay equal
+                self._adamw.step([self.grad], lr=lr, step=self.opt_steps, grad_scale=1.0 / self.world,
+                                 seed=self.opts.seed + 0x9E3779B1 * self.iteration)
+            else:
+                _lib.check(L.nk_adam_step(self.params.data_ptr(), self.grad.data_ptr(), self.exp_avg.data_ptr(),
+                                          self.exp_avg_sq.data_ptr(), self.params.numel(), self.opt_steps, lr, self.opts.betas[0],
+                                          self.opts.betas[1], self.opts.eps, 1.0 / self.world, st))
             self.coarse.pack()
             if self.fine is not None:
                 self.fine.pack()
@@ -202,6 +220,17 @@ class Trainer:
     def _rank(self) -> int:
         return torch.distributed.get_rank(self.pg) if self.world > 1 else 0
 
+    def optimizer_tensors(self) -> list:
+        """Every tensor an optimiser step changes."""
+        more = list(self._adamw.scales[0]) if self._adamw is not None and self._adamw.scales is not None else []
+        return [self.params, self.exp_avg, self.exp_avg_sq] + more
+
+    def _moments(self):
+        """Both moments as fp32 (8-bit ones decoded)."""
+        if self._adamw is not None and self._adamw.state_bits == 8:
+            return tuple(decode_moment(c, u) for c, u in zip((self.exp_avg, self.exp_avg_sq), self._adamw.scales[0]))
+        return self.exp_avg, self.exp_avg_sq
+
     # -- checkpoints ----------------------------------------------------------------------------
     def export_state(self, loss: float = float("nan"), psnr: float = float("nan")):
         """Everything a reference-layout checkpoint carries, copied to the CPU.  ``iter`` is the index
@@ -212,9 +241,10 @@ class Trainer:
         cpu = lambda t: t.detach().to("cpu", copy=True)
         fine = self.fine is not None
         cut = lambda t: [cpu(t[:nc])] + ([cpu(t[ncp:])] if fine else [])
+        exp_avg, exp_avg_sq = self._moments()
         return TrainState(iteration=self.iteration - 1, coarse=cpu(self.params[:nc]),
-                          fine=cpu(self.params[ncp:]) if fine else None, exp_avg=cut(self.exp_avg),
-                          exp_avg_sq=cut(self.exp_avg_sq), opt_step=self.opt_steps,
+                          fine=cpu(self.params[ncp:]) if fine else None, exp_avg=cut(exp_avg),
+                          exp_avg_sq=cut(exp_avg_sq), opt_step=self.opt_steps,
                           lr=lr_at(max(self.iteration - 1, 0), self.opts), loss=loss, psnr=psnr)
 
     def import_state(self, s) -> None:
@@ -226,11 +256,17 @@ class Trainer:
         self.params[:nc] = s.coarse.to(self.device)
         if self.fine is not None:
             self.params[ncp:] = s.fine.to(self.device)
-        self.exp_avg.zero_(); self.exp_avg_sq.zero_()
+        m, v = torch.zeros_like(self.params), torch.zeros_like(self.params)
         if s.exp_avg:
-            self.exp_avg[:nc] = s.exp_avg[0].to(self.device); self.exp_avg_sq[:nc] = s.exp_avg_sq[0].to(self.device)
+            m[:nc] = s.exp_avg[0].to(self.device); v[:nc] = s.exp_avg_sq[0].to(self.device)
             if self.fine is not None:
-                self.exp_avg[ncp:] = s.exp_avg[1].to(self.device); self.exp_avg_sq[ncp:] = s.exp_avg_sq[1].to(self.device)
+                m[ncp:] = s.exp_avg[1].to(self.device); v[ncp:] = s.exp_avg_sq[1].to(self.device)
+        if self._adamw is not None and self._adamw.state_bits == 8:
+            for t, codes, scale in zip((m, v), (self.exp_avg, self.exp_avg_sq), self._adamw.scales[0]):
+                c, u = encode_moment(t, codes.dtype)
+                codes.copy_(c); scale.copy_(u)
+        else:
+            self.exp_avg.copy_(m); self.exp_avg_sq.copy_(v)
         self.iteration = int(s.iteration) + 1
         self.opt_steps = int(s.opt_step) if s.exp_avg else 0
         self.coarse.pack()
@@ -319,10 +355,10 @@ class GraphedStep:
                 # one eager pass of the kernels first would advance the parameters, so instead the
                 # launch-time set-up that capture forbids (function attributes) is done by a throw-away
                 # pass on scratch copies of everything the step writes
-                keep = [t.clone() for t in (trainer.params, trainer.exp_avg, trainer.exp_avg_sq)]
+                keep = [t.clone() for t in trainer.optimizer_tensors()]
                 self._launch(side.cuda_stream)
                 side.synchronize()
-                for t, k in zip((trainer.params, trainer.exp_avg, trainer.exp_avg_sq), keep):
+                for t, k in zip(trainer.optimizer_tensors(), keep):
                     t.copy_(k)
                 trainer.coarse.pack()
                 if trainer.fine is not None:
@@ -344,6 +380,7 @@ class GraphedStep:
         b1, b2 = tr.opts.betas
         st.adam_step_size = lr_at(it, tr.opts) / (1.0 - b1 ** step)
         st.adam_bc2_sqrt = math.sqrt(1.0 - b2 ** step)
+        st.adamw_decay = lr_at(it, tr.opts) * tr.opts.weight_decay if tr._adamw is not None else 0.0
 
     def _launch(self, st: int) -> None:
         """The launch sequence of one iteration on stream `st` (captured once, or issued eagerly)."""
@@ -364,9 +401,12 @@ class GraphedStep:
         gc, gf = tr.grad_views()
         _lib.check(L.nk_render_rays_bwd(tr.coarse._c, tr.coarse.packed.data_ptr(), fc, fp, rb, R, self.ropts, tr.ws_ptr,
                                         tr.ws_bytes, _ptr(tr.d_rgb_f), tr.d_rgb_c.data_ptr(), gc.data_ptr(), _ptr(gf), st))
-        _lib.check(L.nk_adam_step_dev(tr.params.data_ptr(), tr.grad.data_ptr(), tr.exp_avg.data_ptr(),
-                                      tr.exp_avg_sq.data_ptr(), tr.params.numel(), sp, tr.opts.betas[0], tr.opts.betas[1],
-                                      tr.opts.eps, 1.0, st))
+        if tr._adamw is not None:
+            tr._adamw.step([tr.grad], step_state=sp)
+        else:
+            _lib.check(L.nk_adam_step_dev(tr.params.data_ptr(), tr.grad.data_ptr(), tr.exp_avg.data_ptr(),
+                                          tr.exp_avg_sq.data_ptr(), tr.params.numel(), sp, tr.opts.betas[0], tr.opts.betas[1],
+                                          tr.opts.eps, 1.0, st))
         for m in (tr.coarse, tr.fine):
             if m is not None:
                 _lib.check(L.nk_pack_weights(m._c, m.flat.data_ptr(), m.packed.data_ptr(), st))
