@@ -157,6 +157,20 @@ def load() -> C.CDLL:
     return lib
 
 
+def launch(dev, fn, *args) -> None:
+    """Call a launching entry point (stream last) on the current torch stream of the GPU `dev`."""
+    index = dev.index
+    # the raw handle of the current stream, without the stream object around it
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc < 0:
+        check(rc)
+
+
 def check(rc: int) -> int:
     """Raise on a negative nk_status (sizes are returned through the same channel)."""
     if rc < 0:

@@ -22,23 +22,32 @@ MOMENT_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, to
 _TENSOR_WORDS = C.sizeof(_lib.NkAdamwTensor) // 8
 
 
-def _check_list(name: str, tensors: Sequence[torch.Tensor], like: Sequence[torch.Tensor], dtype: torch.dtype, device) -> None:
-    if len(tensors) != len(like):
-        raise ValueError(f"{name}: {len(tensors)} tensors for {len(like)} parameters")
-    for i, (t, p) in enumerate(zip(tensors, like)):
+def _check_list(name: str, tensors: Sequence[torch.Tensor], numels: Sequence[int], dtype: torch.dtype, device, spans: list) -> List[int]:
+    """Checks a list against the parameters' element counts; returns the addresses, adds the extents to `spans`."""
+    if len(tensors) != len(numels):
+        raise ValueError(f"{name}: {len(tensors)} tensors for {len(numels)} parameters")
+    size, out = dtype.itemsize, []
+    for i, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
             raise ValueError(f"{name}[{i}]: expected a {dtype} tensor on {device}")
-        if t.numel() != p.numel():
-            raise ValueError(f"{name}[{i}]: {t.numel()} elements, the parameter has {p.numel()}")
+        if t.numel() != numels[i]:
+            raise ValueError(f"{name}[{i}]: {t.numel()} elements, expected {numels[i]}")
         if not t.is_contiguous():
             raise ValueError(f"{name}[{i}]: must be contiguous")
+        at = t.data_ptr()
+        out.append(at)
+        if numels[i]:
+            spans.append((at, at + numels[i] * size))
+    return out
 
 
-def _check_disjoint(tensors: List[torch.Tensor]) -> None:
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
+def _check_disjoint(spans: list) -> None:
+    spans.sort()
+    end = 0
+    for a, b in spans:
+        if a < end:
             raise ValueError("parameters, masters and moments must not overlap in memory (the same tensor twice?)")
+        end = b
 
 
 def adamw_state(params: Sequence[torch.Tensor], state_bits: int = 32):
@@ -90,8 +99,7 @@ class AdamW:
                  weight_decay: float = 1e-2, *, state_bits: int = 32, masters: Optional[Sequence[torch.Tensor]] = None,
                  state=None, seed: int = 0):
         self._L = _lib.load()
-        self._sources = list(params)
-        params = [p.detach() for p in params]
+        params = list(params)
         if not params:
             raise ValueError("AdamW: no parameters")
         dt, dev = params[0].dtype, params[0].device
@@ -99,45 +107,38 @@ class AdamW:
             raise ValueError(f"AdamW: parameters of dtype {dt} (float32, bfloat16 or float16)")
         if dev.type != "cuda":
             raise ValueError("AdamW: expected GPU tensors (there is no CPU implementation)")
-        _check_list("params", params, params, dt, dev)
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
             raise ValueError(f"AdamW: betas={tuple(betas)} in [0, 1), eps={eps} >= 0 wanted")
-        if masters is not None:
-            _check_list("masters", masters, params, torch.float32, dev)
+        numels, spans, n = [p.numel() for p in params], [], len(params)
+        none = [0] * n
+        at_p = _check_list("params", params, numels, dt, dev, spans)
+        at_w = none if masters is None else _check_list("masters", masters, numels, torch.float32, dev, spans)
         if state is None:
             state = adamw_state(params, state_bits)
         m, v, scales = state
         if not m or m[0].dtype not in (torch.float32, torch.float8_e4m3fn):
             raise ValueError("AdamW: moments are float32 or float8_e4m3fn / float8_e5m2")
         state_bits = 32 if m[0].dtype == torch.float32 else 8
-        _check_list("exp_avgs", m, params, MOMENT_DTYPES[state_bits][0], dev)
-        _check_list("exp_avg_sqs", v, params, MOMENT_DTYPES[state_bits][1], dev)
-        flat_scales: List[torch.Tensor] = []
+        at_m = _check_list("exp_avgs", m, numels, MOMENT_DTYPES[state_bits][0], dev, spans)
+        at_v = _check_list("exp_avg_sqs", v, numels, MOMENT_DTYPES[state_bits][1], dev, spans)
+        at_sm = at_sv = none
         if state_bits == 8:
-            if scales is None or len(scales) != len(params):
+            if scales is None:
                 raise ValueError("AdamW: 8-bit moments need one (scale_m, scale_v) pair per parameter")
-            for i, (p, pair) in enumerate(zip(params, scales)):
-                for s in pair:
-                    if s.dtype != torch.float32 or s.device != dev or not s.is_contiguous() or s.numel() != -(-p.numel() // BLOCK):
-                        raise ValueError(f"AdamW: scales[{i}]: expected {-(-p.numel() // BLOCK)} contiguous float32 values on {dev}")
-                flat_scales += pair
+            blocks = [-(-k // BLOCK) for k in numels]
+            at_sm = _check_list("scale_m", [s[0] for s in scales], blocks, torch.float32, dev, spans)
+            at_sv = _check_list("scale_v", [s[1] for s in scales], blocks, torch.float32, dev, spans)
         elif scales is not None:
             raise ValueError("AdamW: scales belong to 8-bit moments")
-        _check_disjoint(params + list(m) + list(v) + list(masters or []) + flat_scales)
+        _check_disjoint(spans)
         self.params, self.masters, self.exp_avgs, self.exp_avg_sqs, self.scales = params, masters, m, v, scales
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
         self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
         self.device = dev
-        self._table = (_lib.NkAdamwTensor * len(params))()
-        for i, p in enumerate(params):
-            sm, sv = scales[i] if scales is not None else (None, None)
-            self._table[i] = _lib.NkAdamwTensor(p.data_ptr(), None, m[i].data_ptr(), v[i].data_ptr(),
-                                                masters[i].data_ptr() if masters is not None else None,
-                                                sm.data_ptr() if sm is not None else None,
-                                                sv.data_ptr() if sv is not None else None, p.numel())
-        # the `grad` words of the table, one per tensor
-        self._grads = (C.c_int64 * (_TENSOR_WORDS * len(params))).from_buffer(self._table)
-        self._numels = [p.numel() for p in params]
+        # nk_adamw_tensor, word by word: param, grad (filled in by step), exp_avg, exp_avg_sq, master, scales, n
+        self._words = (C.c_int64 * (_TENSOR_WORDS * n))(*[w for row in zip(at_p, none, at_m, at_v, at_w, at_sm, at_sv, numels) for w in row])
+        self._table = C.cast(self._words, C.POINTER(_lib.NkAdamwTensor))
+        self._numels = numels
         self._opts = _lib.NkAdamwOpts()
         self._opts.param_dtype, self._opts.state_bits = _lib.DTYPES[dt], state_bits
         self._opts.beta1, self._opts.beta2, self._opts.eps = self.betas[0], self.betas[1], self.eps
@@ -151,18 +152,20 @@ class AdamW:
         step-dependent scalars from when the kernel runs (graph replay)."""
         n = len(self.params)
         if grads is None:
-            grads = [p.grad for p in self._sources]
+            grads = [p.grad for p in self.params]
             if any(g is None for g in grads):
                 raise ValueError("AdamW.step: a parameter has no .grad")
         if len(grads) != n:
             raise ValueError(f"grads: {len(grads)} tensors for {n} parameters")
-        gd, dev, words, numels = grads[0].dtype, self.device, self._grads, self._numels
+        gd, dev, words, numels = grads[0].dtype, self.device, self._words, self._numels
         if gd != torch.float32 and gd != self.params[0].dtype:
             raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self.params[0].dtype})")
-        for i, g in enumerate(grads):
-            if g.dtype != gd or g.numel() != numels[i] or g.device != dev or not g.is_contiguous():
-                raise ValueError(f"grads[{i}]: expected {numels[i]} contiguous {gd} values on {dev}")
-            words[_TENSOR_WORDS * i + 1] = g.data_ptr()
+        at = 1
+        for g, k in zip(grads, numels):
+            if g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
+                raise ValueError(f"grads[{at // _TENSOR_WORDS}]: expected {k} contiguous {gd} values on {dev}")
+            words[at] = g.data_ptr()
+            at += _TENSOR_WORDS
         step = self.steps + 1 if step is None else int(step)
         if step < 1:
             raise ValueError(f"step={step}: from 1")
@@ -171,12 +174,7 @@ class AdamW:
         o.grad_scale = float(grad_scale)
         o.seed = (self.seed + 0x9E3779B1 * step if seed is None else int(seed)) & 0xFFFFFFFF
         o.state = step_state
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if torch.cuda.current_device() == dev.index:
-            _lib.check(self._L.nk_adamw_step(self._table, n, o, stream))
-        else:
-            with torch.cuda.device(dev):
-                _lib.check(self._L.nk_adamw_step(self._table, n, o, stream))
+        _lib.launch(dev, self._L.nk_adamw_step, self._table, n, o)
         self.steps = step
 
 

@@ -13,36 +13,33 @@ import torch
 from . import lib as _lib
 
 
+_KEEP = 32              # the forward pass of a training step keeps the state in front of every 32nd step
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, T, n] with unit stride along n and no negative strides (a copy where it has neither)."""
-    if (t.shape[2] > 1 and t.stride(2) != 1) or t.stride(0) < 0 or t.stride(1) < 0:
-        return t.contiguous()
-    return t
+    sb, st, sc = t.stride()
+    return t if (sc == 1 or t.shape[2] == 1) and sb >= 0 and st >= 0 else t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _call(dev, fn, *args) -> None:
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(*args, stream))
-    else:
-        with torch.cuda.device(dev):
-            _lib.check(fn(*args, stream))
-
-
 def _opts(a, x, g, lengths, reverse) -> "_lib.NkScanOpts":
     B, T, C = x.shape
-    sg = (0, 0) if g is None else g.stride()
-    return _lib.NkScanOpts(B, T, C, a.shape[2], _lib.DTYPES[x.dtype], _lib.DTYPES[a.dtype], int(reverse), 0,
-                           a.stride(0), a.stride(1), x.stride(0), x.stride(1), sg[0], sg[1], _ptr(lengths))
+    ab, at, _ = a.stride()
+    xb, xt, _ = x.stride()
+    gb, gt, _ = (0, 0, 0) if g is None else g.stride()
+    return _lib.NkScanOpts(B, T, C, a.shape[2], _lib.DTYPES[x.dtype], _lib.DTYPES[a.dtype], reverse, 0, ab, at, xb, xt, gb, gt,
+                           _ptr(lengths))
 
 
 def _workspace(L, o, backward, dev):
-    n = _lib.check(L.nk_gated_scan_workspace_bytes(o, backward))
-    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n      # torch's blocks are 512-byte aligned
+    n = L.nk_gated_scan_workspace_bytes(o, backward)
+    if n == 0:
+        return None, 0
+    return torch.empty(_lib.check(n), dtype=torch.uint8, device=dev), n         # torch's blocks are 512-byte aligned
 
 
 def _forward(a, x, h0, lengths, reverse, training):
@@ -51,21 +48,19 @@ def _forward(a, x, h0, lengths, reverse, training):
     dev = x.device
     if B == 0 or T == 0:        # no step: the state passes through
         return x.new_empty(B, T, C), (h0.clone() if h0 is not None else torch.zeros(B, C, dtype=torch.float32, device=dev)), None
-    h = torch.empty(B, T, C, dtype=x.dtype, device=dev)
-    last = torch.empty(B, C, dtype=torch.float32, device=dev)
+    h = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    last = torch.empty((B, C), dtype=torch.float32, device=dev)
     o = _opts(a, x, None, lengths, reverse)
-    states = None
-    if training:
-        states = torch.empty(_lib.check(L.nk_gated_scan_states_bytes(o)) // 4, dtype=torch.float32, device=dev)
+    states = torch.empty(B * (-(-T // _KEEP)) * C, dtype=torch.float32, device=dev) if training else None
     ws, n = _workspace(L, o, 0, dev)
-    _call(dev, L.nk_gated_scan_fwd, o, a.data_ptr(), x.data_ptr(), _ptr(h0), h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), n)
+    _lib.launch(dev, L.nk_gated_scan_fwd, o, a.data_ptr(), x.data_ptr(), _ptr(h0), h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), n)
     return h, last, states
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, x, h0, lengths, reverse):
-        # the states in front of every 32nd step serve the gates' gradient alone
+        # the kept states serve the gates' gradient alone
         h, last, states = _forward(a, x, h0, lengths, reverse, ctx.needs_input_grad[0])
         ctx.save_for_backward(a, x, h0, lengths, states)
         ctx.reverse = reverse
@@ -92,12 +87,12 @@ class _GatedScan(torch.autograd.Function):
         L = _lib.load()
         g = _rows(d_h) if d_h is not None else None
         o = _opts(a, x, g, lengths, ctx.reverse)
-        d_a = torch.empty(B, T, a.shape[2], dtype=a.dtype, device=dev) if want_a else None
-        d_x = torch.empty(B, T, C, dtype=x.dtype, device=dev) if want_x else None
-        d_0 = torch.empty(B, C, dtype=torch.float32, device=dev) if want_0 else None
+        d_a = torch.empty(a.shape, dtype=a.dtype, device=dev) if want_a else None
+        d_x = torch.empty((B, T, C), dtype=x.dtype, device=dev) if want_x else None
+        d_0 = torch.empty((B, C), dtype=torch.float32, device=dev) if want_0 else None
         ws, n = _workspace(L, o, 1, dev)
-        _call(dev, L.nk_gated_scan_bwd, o, a.data_ptr(), x.data_ptr(), _ptr(states), _ptr(h0), _ptr(g), _ptr(d_last),
-              _ptr(d_a), _ptr(d_x), _ptr(d_0), _ptr(ws), n)
+        _lib.launch(dev, L.nk_gated_scan_bwd, o, a.data_ptr(), x.data_ptr(), _ptr(states), _ptr(h0), _ptr(g), _ptr(d_last),
+                    _ptr(d_a), _ptr(d_x), _ptr(d_0), _ptr(ws), n)
         return d_a, d_x, d_0, None, None
 
 
@@ -122,6 +117,7 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     J = a.shape[2]
     if C < 1 or J < 1 or C % J:
         raise ValueError(f"a: {J} gates for {C} channels (a divisor of them)")
+    reverse = bool(reverse)
     dev = x.device
     if dev.type != "cuda":
         raise ValueError("x: expected a GPU tensor (there is no CPU implementation)")
@@ -137,5 +133,5 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
         lengths = lengths.contiguous()
     a, x = _rows(a), _rows(x)
     if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(a, x, h0, lengths, bool(reverse))
-    return _forward(a, x, h0, lengths, bool(reverse), False)[:2]
+        return _GatedScan.apply(a, x, h0, lengths, int(reverse))
+    return _forward(a, x, h0, lengths, int(reverse), False)[:2]

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _call, _ptr
+from .scan import _ptr
 
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
@@ -19,7 +19,7 @@ def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
 
 def _workspace(L, o, hidden, weight, backward):
     n = _lib.check(L.nk_linear_xent_workspace_bytes(o, hidden.data_ptr(), weight.data_ptr(), backward))
-    return torch.empty(n, dtype=torch.uint8, device=hidden.device), n
+    return torch.empty(n, dtype=torch.uint8, device=hidden.device), n         # torch's blocks are 512-byte aligned
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -30,11 +30,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _forward(hidden, weight, target, o, reduction):
     L = _lib.load()
     N, dev = hidden.shape[0], hidden.device
-    loss, lse = torch.empty(2, N, dtype=torch.float32, device=dev).unbind(0)
+    loss, lse = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
     total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     ws, n = _workspace(L, o, hidden, weight, 0)
-    _call(dev, L.nk_linear_xent_fwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(), lse.data_ptr(),
-          _ptr(total), ws.data_ptr(), n)
+    _lib.launch(dev, L.nk_linear_xent_fwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
+                lse.data_ptr(), _ptr(total), ws.data_ptr(), n)
     return (loss if total is None else total), lse
 
 
@@ -60,8 +60,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d_loss = d_loss.contiguous()
         L = _lib.load()
         ws, n = _workspace(L, ctx.opts, hidden, weight, 1)
-        _call(dev, L.nk_linear_xent_bwd, ctx.opts, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
-              d_loss.data_ptr(), _ptr(d_hidden), _ptr(d_weight), ws.data_ptr(), n)
+        _lib.launch(dev, L.nk_linear_xent_bwd, ctx.opts, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
+                    d_loss.data_ptr(), _ptr(d_hidden), _ptr(d_weight), ws.data_ptr(), n)
         return d_hidden, d_weight, None, None, None, None
 
 
