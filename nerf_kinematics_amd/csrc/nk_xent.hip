@@ -65,7 +65,8 @@ template <int BM_, int BN_, int WGM_, int WGN_, int STAGES_> struct Cfg {
     static constexpr int WAVES = WGM * WGN, THREADS = WAVES * 64;
     static constexpr int TM = BM / WGM / 16, TN = BN / WGN / 16;
     static constexpr int STAGE_BYTES = (BM + BN) * 128, LDS = STAGE_BYTES * STAGES;
-    static constexpr int PIECES = (BM + BN) / 8 / WAVES;     // load instructions per wavefront and step
+    static constexpr int PA = BM / 8 / WAVES, PB = BN / 8 / WAVES, PIECES = PA + PB;    // load instructions per wavefront and step
+    static_assert(PA * 8 * WAVES == BM && PB * 8 * WAVES == BN, "every wavefront loads the same share of A and of B");
 };
 
 NK_D void lds_load(uint32_t lds_at, u32x4 srd, uint32_t voff, uint32_t soff) {
@@ -88,67 +89,82 @@ template <typename T, class C>
 NK_D void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds, f32x4 (&acc)[C::TM][C::TN]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / C::WGN, wn = wave % C::WGN;
-    u32x4 ra = resource(A.p + m0 * A.stride, (A.rows - m0) * A.stride);
-    u32x4 rb = resource(B.p + n0 * B.stride, (B.rows - n0) * B.stride);
+    // the last byte that a row of this stretch of k may be read to; rows and steps behind it arrive as zeros
+    const int64_t row_bytes = (kbytes + 15) & ~(int64_t)15;
+    u32x4 ra = resource(A.p + m0 * A.stride, (A.rows - m0 - 1) * A.stride + row_bytes);
+    u32x4 rb = resource(B.p + n0 * B.stride, (B.rows - n0 - 1) * B.stride + row_bytes);
     asm volatile("s_nop 4" : "+s"(ra), "+s"(rb));       // scalars written by the vector unit, read by loads issued from asm
     const uint32_t lds0 = (uint32_t)(uintptr_t)(NK_LDS char*)lds;
     // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
     const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
-    uint32_t voff[C::PIECES];
+    uint32_t va[C::PA], vb[C::PB];
 #pragma unroll
-    for (int i = 0; i < C::PIECES; ++i) {
-        const int r8 = wave * C::PIECES + i;                 // group of eight rows: A's first, then B's
-        const bool isa = r8 < C::BM / 8;
-        const int row = (isa ? r8 : r8 - C::BM / 8) * 8 + lrow;
-        voff[i] = (uint32_t)row * (uint32_t)(isa ? A.stride : B.stride) + lchunk * 16;
-    }
+    for (int i = 0; i < C::PA; ++i) va[i] = (uint32_t)((wave * C::PA + i) * 8 + lrow) * (uint32_t)A.stride + lchunk * 16;
+#pragma unroll
+    for (int i = 0; i < C::PB; ++i) vb[i] = (uint32_t)((wave * C::PB + i) * 8 + lrow) * (uint32_t)B.stride + lchunk * 16;
     const int steps = (int)((kbytes + 127) / 128);
-    const bool ragged = (kbytes & 127) != 0;
+    // Loads of a step, behind the end of k as well (out of range: no memory is touched), so that the loop has
+    // no branches and the number of loads in flight is always the same.
+    const int last = (int)((kbytes - lchunk * 16 + 127) / 128);       // steps in which this lane's chunk is inside k
     auto issue = [&](int s, int slot) {
-        const bool cut = ragged && s == steps - 1 && (int64_t)s * 128 + lchunk * 16 >= kbytes;      // behind the end of k
+        const uint32_t out = s < last ? 0u : 0x80000000u;
+        const uint32_t at = lds0 + slot * C::STAGE_BYTES;
 #pragma unroll
-        for (int i = 0; i < C::PIECES; ++i) {
-            const int r8 = wave * C::PIECES + i;
-            const uint32_t at = lds0 + slot * C::STAGE_BYTES + r8 * 1024;
-            const uint32_t v = cut ? 0x80000000u : voff[i];
-            if (r8 < C::BM / 8) lds_load(at, ra, v, (uint32_t)s * 128);
-            else lds_load(at, rb, v, (uint32_t)s * 128);
-        }
+        for (int i = 0; i < C::PA; ++i) lds_load(at + (wave * C::PA + i) * 1024, ra, va[i] | out, (uint32_t)s * 128);
+#pragma unroll
+        for (int i = 0; i < C::PB; ++i) lds_load(at + C::BM * 128 + (wave * C::PB + i) * 1024, rb, vb[i] | out, (uint32_t)s * 128);
     };
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int pre = C::STAGES - 1;
-    for (int s = 0; s < pre && s < steps; ++s) issue(s, s);
-    int slot = 0, fill = pre % C::STAGES;
     const int frow = lane & 15, fchunk = lane >> 4;
     const char* fa = lds + (wm * C::TM * 16 + frow) * 128;
     const char* fb = lds + (C::BM + wn * C::TN * 16 + frow) * 128;
     const int x0 = (fchunk ^ (frow & 7)) * 16, x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
-    for (int s = 0; s < steps; ++s) {
-        // this step's loads have landed when at most those of the steps behind it are outstanding
-        if (s + pre <= steps) wait_loads_and_meet<(C::STAGES - 2) * C::PIECES>();
-        else wait_loads_and_meet<0>();
-        if (s + pre < steps) issue(s + pre, fill);
-        const char* pa = fa + slot * C::STAGE_BYTES;
-        const char* pb = fb + slot * C::STAGE_BYTES;
+    u32x4 a0[C::TM], b0[C::TN], a1[C::TM], b1[C::TN];
+    auto read = [&](u32x4 (&a)[C::TM], u32x4 (&b)[C::TN], int slot, int x) {
+        const char* pa = fa + slot * C::STAGE_BYTES + x;
+        const char* pb = fb + slot * C::STAGE_BYTES + x;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 a[C::TM], b[C::TN];
+        for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048);
 #pragma unroll
-            for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048 + (h ? x1 : x0));
+        for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048);
+    };
+    auto multiply = [&](const u32x4 (&a)[C::TM], const u32x4 (&b)[C::TN]) {
 #pragma unroll
-            for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048 + (h ? x1 : x0));
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int i = 0; i < C::TM; ++i)
+            for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
+        // one LDS read between every few products (0x100: LDS read, 0x008: matrix product)
 #pragma unroll
-                for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
+        for (int q = 0; q < C::TM + C::TN; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, C::TM * C::TN / (C::TM + C::TN), 0);
         }
-        slot = slot + 1 == C::STAGES ? 0 : slot + 1;
-        fill = fill + 1 == C::STAGES ? 0 : fill + 1;
+    };
+    constexpr int S = C::STAGES;
+#pragma unroll
+    for (int s = 0; s < S; ++s) issue(s, s);
+    wait_loads_and_meet<(S - 1) * C::PIECES>();
+    read(a0, b0, 0, x0);
+    int slot = 0;
+    for (int s = 0; s < steps; ++s) {
+        const int next = slot + 1 == S ? 0 : slot + 1;
+        // the second half of the step's fragments arrives while the first is multiplied
+        read(a1, b1, slot, x1);
+        multiply(a0, b0);
+        __builtin_amdgcn_sched_barrier(0);
+        // everyone has read this step; the next one has landed when at most the loads behind it are outstanding
+        wait_loads_and_meet<(S - 2) * C::PIECES>();
+        issue(s + S, slot);
+        __builtin_amdgcn_sched_barrier(0);
+        read(a0, b0, next, x0);
+        multiply(a1, b1);
+        __builtin_amdgcn_sched_barrier(0);
+        slot = next;
     }
-    wait_loads_and_meet<0>();           // the LDS of the last step is free for the epilogue
+    wait_loads_and_meet<0>();           // nothing is in flight into LDS any more: it is free for the epilogue
 }
 
 // Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn; every XCD gets a contiguous
@@ -484,7 +500,10 @@ __global__ __launch_bounds__(256) void k_xent_transpose(const T* __restrict__ sr
 }
 
 // ---- host -------------------------------------------------------------------------------------
-typedef Cfg<256, 256, 2, 4, 2> Large;
+#ifndef LARGE_WAVES
+#define LARGE_WAVES 8
+#endif
+typedef Cfg<256, 256, 2, LARGE_WAVES / 2, 2> Large;
 typedef Cfg<128, 128, 2, 2, 2> Middle;
 typedef Cfg<128, 32, 4, 1, 4> Few;
 
