@@ -85,86 +85,107 @@ NK_D u32x4 resource(const char* p, int64_t bytes) {
     return r;
 }
 
-template <typename T, class C>
-NK_D void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds, f32x4 (&acc)[C::TM][C::TN]) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / C::WGN, wn = wave % C::WGN;
-    // the last byte that a row of this stretch of k may be read to; rows and steps behind it arrive as zeros
-    const int64_t row_bytes = (kbytes + 15) & ~(int64_t)15;
-    u32x4 ra = resource(A.p + m0 * A.stride, (A.rows - m0 - 1) * A.stride + row_bytes);
-    u32x4 rb = resource(B.p + n0 * B.stride, (B.rows - n0 - 1) * B.stride + row_bytes);
-    asm volatile("s_nop 4" : "+s"(ra), "+s"(rb));       // scalars written by the vector unit, read by loads issued from asm
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(NK_LDS char*)lds;
-    // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
-    const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
+// One tile's product in two parts: begin() starts the loads of the first steps, run() does the rest.  The
+// LDS of the operands has to be idle at begin().
+template <typename T, class C> struct TileProduct {
+    u32x4 ra, rb;
     uint32_t va[C::PA], vb[C::PB];
-#pragma unroll
-    for (int i = 0; i < C::PA; ++i) va[i] = (uint32_t)((wave * C::PA + i) * 8 + lrow) * (uint32_t)A.stride + lchunk * 16;
-#pragma unroll
-    for (int i = 0; i < C::PB; ++i) vb[i] = (uint32_t)((wave * C::PB + i) * 8 + lrow) * (uint32_t)B.stride + lchunk * 16;
-    const int steps = (int)((kbytes + 127) / 128);
+    uint32_t lds0;
+    int steps, last, wave;
+    char* lds;
+
     // Loads of a step, behind the end of k as well (out of range: no memory is touched), so that the loop has
     // no branches and the number of loads in flight is always the same.
-    const int last = (int)((kbytes - lchunk * 16 + 127) / 128);       // steps in which this lane's chunk is inside k
-    auto issue = [&](int s, int slot) {
+    NK_D void issue(int s, int slot) {
         const uint32_t out = s < last ? 0u : 0x80000000u;
         const uint32_t at = lds0 + slot * C::STAGE_BYTES;
 #pragma unroll
         for (int i = 0; i < C::PA; ++i) lds_load(at + (wave * C::PA + i) * 1024, ra, va[i] | out, (uint32_t)s * 128);
 #pragma unroll
         for (int i = 0; i < C::PB; ++i) lds_load(at + C::BM * 128 + (wave * C::PB + i) * 1024, rb, vb[i] | out, (uint32_t)s * 128);
-    };
+    }
+
+    NK_D void begin(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds_) {
+        const int lane = threadIdx.x & 63;
+        lds = lds_;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        // the last byte that a row of this stretch of k may be read to; rows and steps behind it arrive as zeros
+        const int64_t row_bytes = (kbytes + 15) & ~(int64_t)15;
+        ra = resource(A.p + m0 * A.stride, (A.rows - m0 - 1) * A.stride + row_bytes);
+        rb = resource(B.p + n0 * B.stride, (B.rows - n0 - 1) * B.stride + row_bytes);
+        asm volatile("s_nop 4" : "+s"(ra), "+s"(rb));       // scalars written by the vector unit, read by loads issued from asm
+        lds0 = (uint32_t)(uintptr_t)(NK_LDS char*)lds;
+        // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
+        const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::PA; ++i) va[i] = (uint32_t)((wave * C::PA + i) * 8 + lrow) * (uint32_t)A.stride + lchunk * 16;
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int frow = lane & 15, fchunk = lane >> 4;
-    const char* fa = lds + (wm * C::TM * 16 + frow) * 128;
-    const char* fb = lds + (C::BM + wn * C::TN * 16 + frow) * 128;
-    const int x0 = (fchunk ^ (frow & 7)) * 16, x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
-    u32x4 a0[C::TM], b0[C::TN], a1[C::TM], b1[C::TN];
-    auto read = [&](u32x4 (&a)[C::TM], u32x4 (&b)[C::TN], int slot, int x) {
-        const char* pa = fa + slot * C::STAGE_BYTES + x;
-        const char* pb = fb + slot * C::STAGE_BYTES + x;
+        for (int i = 0; i < C::PB; ++i) vb[i] = (uint32_t)((wave * C::PB + i) * 8 + lrow) * (uint32_t)B.stride + lchunk * 16;
+        steps = (int)((kbytes + 127) / 128);
+        last = (int)((kbytes - lchunk * 16 + 127) / 128);       // steps in which this lane's chunk is inside k
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048);
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048);
-    };
-    auto multiply = [&](const u32x4 (&a)[C::TM], const u32x4 (&b)[C::TN]) {
+        for (int s = 0; s < C::STAGES; ++s) issue(s, s);
+    }
+
+    NK_D void run(f32x4 (&acc)[C::TM][C::TN]) {
+        const int lane = threadIdx.x & 63, wm = wave / C::WGN, wn = wave % C::WGN;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
-        // one LDS read between every few products (0x100: LDS read, 0x008: matrix product)
+            for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+        const int frow = lane & 15, fchunk = lane >> 4;
+        const char* fa = lds + (wm * C::TM * 16 + frow) * 128;
+        const char* fb = lds + (C::BM + wn * C::TN * 16 + frow) * 128;
+        const int x0 = (fchunk ^ (frow & 7)) * 16, x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
+        u32x4 a0[C::TM], b0[C::TN], a1[C::TM], b1[C::TN];
+        auto read = [&](u32x4 (&a)[C::TM], u32x4 (&b)[C::TN], int slot, int x) {
+            const char* pa = fa + slot * C::STAGE_BYTES + x;
+            const char* pb = fb + slot * C::STAGE_BYTES + x;
 #pragma unroll
-        for (int q = 0; q < C::TM + C::TN; ++q) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, C::TM * C::TN / (C::TM + C::TN), 0);
+            for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048);
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048);
+        };
+        auto multiply = [&](const u32x4 (&a)[C::TM], const u32x4 (&b)[C::TN]) {
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
+            // one LDS read between every few products (0x100: LDS read, 0x008: matrix product)
+#pragma unroll
+            for (int q = 0; q < C::TM + C::TN; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, C::TM * C::TN / (C::TM + C::TN), 0);
+            }
+        };
+        constexpr int S = C::STAGES;
+        wait_loads_and_meet<(S - 1) * C::PIECES>();
+        read(a0, b0, 0, x0);
+        int slot = 0;
+        for (int s = 0; s < steps; ++s) {
+            const int next = slot + 1 == S ? 0 : slot + 1;
+            // the second half of the step's fragments arrives while the first is multiplied
+            read(a1, b1, slot, x1);
+            multiply(a0, b0);
+            __builtin_amdgcn_sched_barrier(0);
+            // everyone has read this step; the next one has landed when at most the loads behind it are outstanding
+            wait_loads_and_meet<(S - 2) * C::PIECES>();
+            issue(s + S, slot);
+            __builtin_amdgcn_sched_barrier(0);
+            read(a0, b0, next, x0);
+            multiply(a1, b1);
+            __builtin_amdgcn_sched_barrier(0);
+            slot = next;
         }
-    };
-    constexpr int S = C::STAGES;
-#pragma unroll
-    for (int s = 0; s < S; ++s) issue(s, s);
-    wait_loads_and_meet<(S - 1) * C::PIECES>();
-    read(a0, b0, 0, x0);
-    int slot = 0;
-    for (int s = 0; s < steps; ++s) {
-        const int next = slot + 1 == S ? 0 : slot + 1;
-        // the second half of the step's fragments arrives while the first is multiplied
-        read(a1, b1, slot, x1);
-        multiply(a0, b0);
-        __builtin_amdgcn_sched_barrier(0);
-        // everyone has read this step; the next one has landed when at most the loads behind it are outstanding
-        wait_loads_and_meet<(S - 2) * C::PIECES>();
-        issue(s + S, slot);
-        __builtin_amdgcn_sched_barrier(0);
-        read(a0, b0, next, x0);
-        multiply(a1, b1);
-        __builtin_amdgcn_sched_barrier(0);
-        slot = next;
+        wait_loads_and_meet<0>();           // nothing is in flight into LDS any more: it is free
     }
-    wait_loads_and_meet<0>();           // nothing is in flight into LDS any more: it is free for the epilogue
+};
+
+template <typename T, class C>
+NK_D void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds, f32x4 (&acc)[C::TM][C::TN]) {
+    TileProduct<T, C> p;
+    p.begin(A, B, m0, n0, kbytes, lds);
+    p.run(acc);
 }
 
 // Workgroup -> tile.  Consecutive workgroups go to the eight XCDs in turn; every XCD gets a contiguous
@@ -188,87 +209,102 @@ struct LseArgs {
     float* zt;                              // logit of the target
 };
 
+// The workgroups stay and take tiles in turn: the loads of the next tile's first steps are under way while
+// this one's registers are reduced.
 template <typename T, class C>
 __global__ __launch_bounds__(C::THREADS) void k_xent_lse(const LseArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
-    int64_t mi, ni;
-    tile_of(blockIdx.x, (g.w.rows + C::BM - 1) / C::BM, (g.N + C::BN - 1) / C::BN, &mi, &ni);
-    f32x4 acc[C::TM][C::TN];
-    tile_product<T, C>(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds, acc);
+    __shared__ float2 meet[C::WGM][C::BN];
+    const int64_t mt = (g.w.rows + C::BM - 1) / C::BM, nt = (g.N + C::BN - 1) / C::BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
-    float2* meet = (float2*)lds;            // [WGM][BN]
-    const int64_t row0 = mi * C::BM + wm * C::TM * 16 + 4 * (lane >> 4);       // of w; rows row0 + 16 i + e
+    int64_t mi, ni;
+    tile_of(blockIdx.x, mt, nt, &mi, &ni);
+    TileProduct<T, C> p;
+    p.begin(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds);
+    for (int64_t tile = blockIdx.x; tile < mt * nt; tile += gridDim.x) {
+        f32x4 acc[C::TM][C::TN];
+        p.run(acc);
+        const int64_t m_at = mi, n_at = ni;
+        if (tile + gridDim.x < mt * nt) {
+            tile_of(tile + gridDim.x, mt, nt, &mi, &ni);
+            p.begin(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds);
+        }
+        const int64_t row0 = m_at * C::BM + wm * C::TM * 16 + 4 * (lane >> 4);       // of w; rows row0 + 16 i + e
+        const int live = (int)(g.w.rows - row0 < 16 * C::TM ? g.w.rows - row0 : 16 * C::TM);        // rows from row0 on that this wavefront has
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) {
-        const int col = wn * C::TN * 16 + j * 16 + (lane & 15);
-        const int64_t n = ni * C::BN + col;
-        const int64_t t = n < g.N ? g.target[n] - g.v0 : -1;
-        float m = -__builtin_inff();
+        for (int j = 0; j < C::TN; ++j) {
+            const int col = wn * C::TN * 16 + j * 16 + (lane & 15);
+            const int64_t n = n_at * C::BN + col;
+            const int64_t t64 = n < g.N ? g.target[n] - g.v0 - row0 : -1;
+            const int t = t64 < 0 || t64 >= live ? -1 : (int)t64;
+            float m = -__builtin_inff(), zt = 0.0f;
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+            for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t v = row0 + 16 * i + e;
-                if (v >= g.w.rows) acc[i][j][e] = -__builtin_inff();
-                else if (v == t) g.zt[n] = acc[i][j][e];
-                m = fmaxf(m, acc[i][j][e]);
+                for (int e = 0; e < 4; ++e) {
+                    if (16 * i + e >= live) acc[i][j][e] = -__builtin_inff();
+                    if (16 * i + e == t) zt = acc[i][j][e];
+                    m = fmaxf(m, acc[i][j][e]);
+                }
+            if (t >= 0 && (t & 15) < 4) g.zt[n] = zt;        // a lane holds rows 0..3 of every 16
+            const float ms = m == -__builtin_inff() ? 0.0f : m;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - ms) * LOG2E);
+#pragma unroll
+            for (int off = 16; off < 64; off <<= 1) {
+                const float mo = __shfl_xor(m, off, 64), so = __shfl_xor(s, off, 64);
+                const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
+                s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
+                m = mn;
             }
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - ms) * LOG2E);
-#pragma unroll
-        for (int off = 16; off < 64; off <<= 1) {
-            const float mo = __shfl_xor(m, off, 64), so = __shfl_xor(s, off, 64);
-            const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
-            s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
-            m = mn;
+            if (lane < 16) meet[wm][col] = make_float2(m, s);
         }
-        if (lane < 16) meet[wm * C::BN + col] = make_float2(m, s);
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < C::BN; c += C::THREADS) {
-        const int64_t n = ni * C::BN + c;
-        if (n >= g.N) break;
-        float m = meet[c].x, s = meet[c].y;
+        // LDS only: the loads of the next tile stay in flight
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int c = threadIdx.x; c < C::BN; c += C::THREADS) {
+            const int64_t n = n_at * C::BN + c;
+            if (n >= g.N) break;
+            float m = meet[0][c].x, s = meet[0][c].y;
 #pragma unroll
-        for (int w = 1; w < C::WGM; ++w) {
-            const float mo = meet[w * C::BN + c].x, so = meet[w * C::BN + c].y;
-            const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
-            s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
-            m = mn;
+            for (int w = 1; w < C::WGM; ++w) {
+                const float mo = meet[w][c].x, so = meet[w][c].y;
+                const float mn = fmaxf(m, mo), mz = mn == -__builtin_inff() ? 0.0f : mn;
+                s = s * __builtin_amdgcn_exp2f((m - mz) * LOG2E) + so * __builtin_amdgcn_exp2f((mo - mz) * LOG2E);
+                m = mn;
+            }
+            g.part[(g.part0 + m_at) * g.N + n] = make_float2(m, s);
         }
-        g.part[(g.part0 + mi) * g.N + n] = make_float2(m, s);
     }
 }
 
-// lse and loss of 16 tokens: 16 threads a token take the tiles in turn, then meet
+NK_D float2 join(float2 a, float2 b) {
+    const float mn = fmaxf(a.x, b.x), mz = mn == -__builtin_inff() ? 0.0f : mn;
+    return make_float2(mn, a.y * expf(a.x - mz) + b.y * expf(b.x - mz));
+}
+
+// lse and loss of TOK tokens a workgroup: 256 / TOK threads a token take the tiles in turn, then meet in one order
+template <int TOK>
 __global__ __launch_bounds__(256) void k_xent_join(const float2* __restrict__ part, int64_t tiles, int64_t N, int64_t V,
                                                    const int64_t* __restrict__ target, int64_t ignore, const float* __restrict__ zt,
                                                    float* __restrict__ lse, float* __restrict__ loss) {
-    __shared__ float2 meet[16][17];
-    const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const int64_t n = (int64_t)blockIdx.x * 16 + c;
-    float m = -__builtin_inff(), s = 0.0f;
+    __shared__ float2 meet[256];
+    constexpr int TH = 256 / TOK;
+    const int c = threadIdx.x % TOK, q = threadIdx.x / TOK;
+    const int64_t n = (int64_t)blockIdx.x * TOK + c;
+    float2 r = make_float2(-__builtin_inff(), 0.0f);
     if (n < N)
-        for (int64_t t = q; t < tiles; t += 16) {
-            const float2 p = part[t * N + n];
-            const float mn = fmaxf(m, p.x), mz = mn == -__builtin_inff() ? 0.0f : mn;
-            s = s * expf(m - mz) + p.y * expf(p.x - mz);
-            m = mn;
-        }
-    meet[q][c] = make_float2(m, s);
+        for (int64_t t = q; t < tiles; t += TH) r = join(r, part[t * N + n]);
+    meet[q * TOK + c] = r;
     __syncthreads();
+    for (int half = TH / 2; half > 0; half >>= 1) {
+        if (q < half) meet[q * TOK + c] = join(meet[q * TOK + c], meet[(q + half) * TOK + c]);
+        __syncthreads();
+    }
     if (q == 0 && n < N) {
-        for (int k = 1; k < 16; ++k) {
-            const float2 p = meet[k][c];
-            const float mn = fmaxf(m, p.x), mz = mn == -__builtin_inff() ? 0.0f : mn;
-            s = s * expf(m - mz) + p.y * expf(p.x - mz);
-            m = mn;
-        }
-        const float l = m + logf(s);
+        const float l = meet[c].x + logf(meet[c].y);
         const int64_t t = target[n];
         lse[n] = l;
         loss[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : l - zt[n];
@@ -362,41 +398,88 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_dz(const DzArgs g) {
     f32x4 acc[C::TM][C::TN];
     tile_product<T, C>(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
-    const int64_t row0 = mi * C::BM + wm * C::TM * 16 + 4 * (lane >> 4);
+    const int r0 = wm * C::TM * 16 + 4 * (lane >> 4), c0 = wn * C::TN * 16 + (lane & 15);      // this lane's first row and column of the tile
+    const int live = (int)(g.w.rows - mi * C::BM < C::BM ? g.w.rows - mi * C::BM : C::BM);
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
-        const int64_t n = ni * C::BN + wn * C::TN * 16 + j * 16 + (lane & 15);
+        const int64_t n = ni * C::BN + c0 + 16 * j;
         const bool in = n < g.N;
-        const int64_t t = in ? g.target[n] - g.v0 : -1;
+        const int64_t t64 = in ? g.target[n] - g.v0 - mi * C::BM : -1;
+        const int t = t64 < 0 || t64 >= C::BM ? -1 : (int)t64;
         const float lse = in ? g.lse[n] : 0.0f, c = in ? g.c[n] : 0.0f, cs = c * Op<T>::SCALE;
-        T* dz = (T*)g.dz + n * g.dz_ld;
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i) {
-            const int64_t v = row0 + 16 * i;
-            float d[4];
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+                const int r = r0 + 16 * i + e;
                 float p = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
-                if (v + e == t) p -= 1.0f;
-                d[e] = (c == 0.0f || v + e >= g.w.rows) ? 0.0f : p * cs;
+                if (r == t) p -= 1.0f;
+                acc[i][j][e] = (c == 0.0f || r >= live) ? 0.0f : p * cs;
             }
-            if constexpr (sizeof(T) == 2) {
-                typedef __attribute__((ext_vector_type(4))) T vec;
+    }
+    if constexpr (sizeof(T) == 2) {
+        // Both orders leave through LDS, as whole rows of the tile: straight from the registers a store would
+        // touch 16 rows with 32 bytes each.  Rows of 16-byte chunks, chunk ^ (row & mask) against bank conflicts.
+        typedef __attribute__((ext_vector_type(4))) T vec;
+        u32x2 pk[C::TM][C::TN];
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) {
                 vec w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (T)d[e];
-                const u32x2 p = __builtin_bit_cast(u32x2, w);
-                if (in && v < g.dz_ld) *(u32x2*)(dz + v) = p;
-                const u32x2 q = quad_transpose(p, lane);
-                const int64_t n4 = n - (lane & 3), vt = v + (lane & 3);
-                if (n4 < g.dzt_ld && vt < g.w.rows) *(u32x2*)((T*)g.dzt + vt * g.dzt_ld + n4) = q;
-            } else {
-                if (in && v < g.dz_ld) *(float4*)(dz + v) = make_float4(d[0], d[1], d[2], d[3]);
+                for (int e = 0; e < 4; ++e) w[e] = (T)acc[i][j][e];
+                pk[i][j] = __builtin_bit_cast(u32x2, w);
+            }
+        static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the operands' LDS");
+        {
+            constexpr int CH = C::BM / 8;           // [token][row]
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n < g.dzt_ld && v + e < g.w.rows) ((T*)g.dzt)[(v + e) * g.dzt_ld + n] = (T)d[e];
+            for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+                for (int i = 0; i < C::TM; ++i) {
+                    const int r = r0 + 16 * i, c = c0 + 16 * j;
+                    *(u32x2*)(lds + (c * CH + ((r >> 3) ^ (c & (CH - 1)))) * 16 + (r & 4) * 2) = pk[i][j];
+                }
+            __syncthreads();
+            T* dz = (T*)g.dz + mi * C::BM;
+#pragma unroll 4
+            for (int q = threadIdx.x; q < C::BN * CH; q += C::THREADS) {
+                const int c = q / CH, k = q % CH;
+                const int64_t n = ni * C::BN + c;
+                if (n < g.N && mi * C::BM + k * 8 < g.dz_ld) *(u32x4*)(dz + n * g.dz_ld + k * 8) = *(const u32x4*)(lds + (c * CH + (k ^ (c & (CH - 1)))) * 16);
+            }
+            __syncthreads();
+        }
+        {
+            constexpr int CH = C::BN / 8;           // [row][token]
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+                for (int i = 0; i < C::TM; ++i) {
+                    const int r = r0 + 16 * i + (lane & 3), c = c0 + 16 * j - (lane & 3);
+                    *(u32x2*)(lds + (r * CH + ((c >> 3) ^ (r & (CH - 1)))) * 16 + (c & 4) * 2) = quad_transpose(pk[i][j], lane);
+                }
+            __syncthreads();
+            T* dzt = (T*)g.dzt + ni * C::BN;
+#pragma unroll 4
+            for (int q = threadIdx.x; q < C::BM * CH; q += C::THREADS) {
+                const int r = q / CH, k = q % CH;
+                const int64_t v = mi * C::BM + r;
+                if (v < g.w.rows && ni * C::BN + k * 8 < g.dzt_ld) *(u32x4*)(dzt + v * g.dzt_ld + k * 8) = *(const u32x4*)(lds + (r * CH + (k ^ (r & (CH - 1)))) * 16);
             }
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i) {
+                const int64_t v = mi * C::BM + r0 + 16 * i, n = ni * C::BN + c0 + 16 * j;
+                if (n < g.N && v < g.dz_ld) *(f32x4*)((float*)g.dz + n * g.dz_ld + v) = acc[i][j];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n < g.dzt_ld && v + e < g.w.rows) ((float*)g.dzt)[(v + e) * g.dzt_ld + n] = acc[i][j][e];
+            }
     }
 }
 
@@ -458,15 +541,22 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g
     }
 }
 
-// d_hidden from its fp32 sums; tokens that do not count have none
-template <typename T>
+// d_hidden from its fp32 sums, the slices in one order; tokens that do not count have none.  VEC elements a thread.
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ sums, int slices, int64_t N, int64_t D, const float* __restrict__ c,
                                                      const float* __restrict__ rest, float scale, T* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
     if (i >= N * D) return;
-    float s = 0.0f;
-    for (int k = 0; k < slices; ++k) s += sums[(int64_t)k * N * D + i];
-    out[i] = (T)(c[i / D] == 0.0f ? 0.0f : s * (*rest * scale));
+    typedef __attribute__((ext_vector_type(VEC))) float fvec;
+    typedef __attribute__((ext_vector_type(VEC))) T tvec;
+    fvec s = *(const fvec*)(sums + i);
+    for (int k = 1; k < slices; ++k) s += *(const fvec*)(sums + (int64_t)k * N * D + i);
+    const float f = *rest * scale;
+    const bool on = c[i / D] != 0.0f;
+    tvec w;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[e] = (T)(on ? s[e] * f : 0.0f);
+    *(tvec*)(out + i) = w;
 }
 
 // dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take
@@ -480,32 +570,49 @@ __global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int
 
 // dst[c][0 .. dst_ld) = src[0 .. rows)[c], zeros behind; rows with factor c = 0 are left out as zeros (their
 // values may be anything)
-template <typename T>
+template <typename T, bool VEC>       // VEC: source rows start on 16 bytes
 __global__ __launch_bounds__(256) void k_xent_transpose(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
                                                         const float* __restrict__ factor, T* __restrict__ dst, int64_t dst_ld) {
-    __shared__ T tile[64][64 + 4 / sizeof(T)];
+    constexpr int E = 16 / sizeof(T), CH = 64 / E, LD = 64 + 4 / sizeof(T);     // elements per 16 bytes, such pieces per row
+    typedef __attribute__((ext_vector_type(E))) T vec;
+    __shared__ T tile[64 * LD];
     const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int k = y; k < 64; k += 4) {
+#pragma unroll
+    for (int q = threadIdx.x; q < 64 * CH; q += 256) {
+        const int k = q / CH, x = (q % CH) * E;
         const int64_t r = r0 + k, c = c0 + x;
-        T v = (T)0.0f;
-        if (r < rows && c < cols && !(factor && factor[r] == 0.0f)) v = src[r * ld + c];
-        tile[k][x] = v;
+        vec v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = (T)0.0f;
+        if (r < rows && !(factor && factor[r] == 0.0f)) {
+            if (VEC && c + E <= cols) v = *(const vec*)(src + r * ld + c);
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) if (c + e < cols) v[e] = src[r * ld + c + e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) tile[k * LD + x + e] = v[e];
     }
     __syncthreads();
-    for (int k = y; k < 64; k += 4) {
-        const int64_t c = c0 + k, r = r0 + x;
-        if (c < cols && r < dst_ld) dst[c * dst_ld + r] = tile[x][k];
+#pragma unroll
+    for (int q = threadIdx.x; q < 64 * CH; q += 256) {
+        const int x = q / CH, k = (q % CH) * E;         // column of the source, first row of the piece
+        const int64_t c = c0 + x, r = r0 + k;
+        if (c < cols && r < dst_ld) {                   // dst_ld is a multiple of E
+            vec v;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = tile[(k + e) * LD + x];
+            *(vec*)(dst + c * dst_ld + r) = v;
+        }
     }
 }
 
 // ---- host -------------------------------------------------------------------------------------
-#ifndef LARGE_WAVES
-#define LARGE_WAVES 8
-#endif
-typedef Cfg<256, 256, 2, LARGE_WAVES / 2, 2> Large;
+typedef Cfg<256, 256, 2, 4, 2> Large;
 typedef Cfg<128, 128, 2, 2, 2> Middle;
-typedef Cfg<128, 32, 4, 1, 4> Few;
+typedef Cfg<64, 64, 2, 2, 4> Small;
+typedef Cfg<128, 32, 4, 1, 3> Few;
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
@@ -519,12 +626,14 @@ int start(const ARGS& args, int64_t blocks, int slices, int threads, hipStream_t
     return NK_OK;
 }
 
-// Which tile: 0 large, 1 middle, 2 few columns.
-int tile_kind(int64_t M, int64_t N) {
-    if (N <= 32) return 2;
-    return cdiv(M, 256) * cdiv(N, 256) >= 224 ? 0 : 1;
+// Which tile for an M x N product cut into `slices` stretches of k: the largest that still fills the 256 CUs.
+enum { LARGE = 0, MIDDLE = 1, FEW = 2, SMALL = 3 };
+int tile_kind(int64_t M, int64_t N, int64_t slices = 1) {
+    if (N <= 32) return FEW;
+    if (cdiv(M, 256) * cdiv(N, 256) * slices >= 224) return LARGE;
+    return cdiv(M, 128) * cdiv(N, 128) * slices >= 200 ? MIDDLE : SMALL;
 }
-int kind_bm(int kind) { return kind == 0 ? 256 : 128; }
+int kind_bm(int kind) { return kind == LARGE ? 256 : kind == SMALL ? 64 : 128; }
 
 struct Plan {
     int64_t Dp, Np, piece;                  // padded k of the logits' product; tokens padded to a step; vocabulary rows per piece
@@ -574,35 +683,43 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
         p->ht = take(o->D * p->Np * es);
         p->dz = take(o->N * piece * es);
         p->dzt = take(piece * p->Np * es);
-        // d_hidden has few tiles: cut its k (the piece) until they fill the chip
-        const int64_t tiles = cdiv(o->D, 128) * cdiv(o->N, o->N <= 32 ? 32 : 128), most = piece / (8 * step);
-        int64_t s = tiles >= 256 || tiles < 1 ? 1 : cdiv(512, tiles);
-        if (s > most) s = most;
-        if (s > 16) s = 16;
-        p->slices = (int)(s < 1 ? 1 : s);
+        // d_hidden has few tiles: cut its k (the piece) until they fill the chip, in large tiles if the stretches stay long
+        const int64_t large = cdiv(o->D, 256) * cdiv(o->N, 256), tiles = cdiv(o->D, 64) * cdiv(o->N, o->N <= 32 ? 32 : 64);
+        int64_t cut = 1;
+        if (o->N > 32 && large > 0 && large < 224 && piece / cdiv(256, large) >= 2048) cut = cdiv(256, large);
+        else if (large < 224 && tiles > 0 && tiles < 256) cut = cdiv(512, tiles);
+        const int64_t most = piece / (8 * step);
+        if (cut > most) cut = most;
+        if (cut > 16) cut = 16;
+        p->slices = (int)(cut < 1 ? 1 : cut);
         p->sums = take((int64_t)p->slices * o->N * o->D * 4);
     }
     p->total = off;
     return NK_OK;
 }
 
+template <typename T, class C> int lse_start(const LseArgs& g, hipStream_t st) {
+    const int64_t tiles = cdiv(g.w.rows, C::BM) * cdiv(g.N, C::BN), fit = 256 * (163840 / (C::LDS + C::WGM * C::BN * 8));     // resident workgroups
+    return start<k_xent_lse<T, C>>(g, tiles < fit ? tiles : fit, 1, C::THREADS, st, "k_xent_lse");
+}
+template <typename T, class C> int dz_start(const DzArgs& g, hipStream_t st) {
+    return start<k_xent_dz<T, C>>(g, cdiv(g.w.rows, C::BM) * cdiv(g.dzt_ld, C::BN), 1, C::THREADS, st, "k_xent_dz");
+}
+template <typename T, class C, bool SUMS> int product_start(const ProductArgs& g, int slices, hipStream_t st) {
+    return start<k_xent_product<T, C, SUMS>>(g, cdiv(g.M, C::BM) * cdiv(g.N, C::BN), slices, C::THREADS, st, "k_xent_product");
+}
 template <typename T> int lse_launch(int kind, const LseArgs& g, hipStream_t st) {
-    const int64_t M = g.w.rows, N = g.N;
-    if (kind == 0) return start<k_xent_lse<T, Large>>(g, cdiv(M, 256) * cdiv(N, 256), 1, Large::THREADS, st, "k_xent_lse");
-    if (kind == 1) return start<k_xent_lse<T, Middle>>(g, cdiv(M, 128) * cdiv(N, 128), 1, Middle::THREADS, st, "k_xent_lse");
-    return start<k_xent_lse<T, Few>>(g, cdiv(M, 128) * cdiv(N, 32), 1, Few::THREADS, st, "k_xent_lse");
+    return kind == LARGE ? lse_start<T, Large>(g, st) : kind == MIDDLE ? lse_start<T, Middle>(g, st) : kind == FEW ? lse_start<T, Few>(g, st)
+                                                                                                        : lse_start<T, Small>(g, st);
 }
 template <typename T> int dz_launch(int kind, const DzArgs& g, hipStream_t st) {
-    const int64_t M = g.w.rows;
-    if (kind == 0) return start<k_xent_dz<T, Large>>(g, cdiv(M, 256) * cdiv(g.dzt_ld, 256), 1, Large::THREADS, st, "k_xent_dz");
-    if (kind == 1) return start<k_xent_dz<T, Middle>>(g, cdiv(M, 128) * cdiv(g.dzt_ld, 128), 1, Middle::THREADS, st, "k_xent_dz");
-    return start<k_xent_dz<T, Few>>(g, cdiv(M, 128) * cdiv(g.dzt_ld, 32), 1, Few::THREADS, st, "k_xent_dz");
+    return kind == LARGE ? dz_start<T, Large>(g, st) : kind == MIDDLE ? dz_start<T, Middle>(g, st) : kind == FEW ? dz_start<T, Few>(g, st)
+                                                                                                      : dz_start<T, Small>(g, st);
 }
 template <typename T, bool SUMS> int product_launch(const ProductArgs& g, int slices, hipStream_t st) {
-    const int kind = g.N <= 32 ? 2 : cdiv(g.M, 256) * cdiv(g.N, 256) * slices >= 224 ? 0 : 1;
-    if (kind == 0) return start<k_xent_product<T, Large, SUMS>>(g, cdiv(g.M, 256) * cdiv(g.N, 256), slices, Large::THREADS, st, "k_xent_product");
-    if (kind == 1) return start<k_xent_product<T, Middle, SUMS>>(g, cdiv(g.M, 128) * cdiv(g.N, 128), slices, Middle::THREADS, st, "k_xent_product");
-    return start<k_xent_product<T, Few, SUMS>>(g, cdiv(g.M, 128) * cdiv(g.N, 32), slices, Few::THREADS, st, "k_xent_product");
+    const int kind = tile_kind(g.M, g.N, slices);
+    return kind == LARGE ? product_start<T, Large, SUMS>(g, slices, st) : kind == MIDDLE ? product_start<T, Middle, SUMS>(g, slices, st)
+         : kind == FEW ? product_start<T, Few, SUMS>(g, slices, st) : product_start<T, Small, SUMS>(g, slices, st);
 }
 
 template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t dst_ld, hipStream_t st) {
@@ -613,8 +730,11 @@ template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t
     return NK_OK;
 }
 template <typename T> int transpose(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* factor, void* dst, int64_t dst_ld, hipStream_t st) {
-    hipLaunchKernelGGL(k_xent_transpose<T>, dim3((unsigned)cdiv(dst_ld, 64), (unsigned)cdiv(cols, 64)), dim3(256), 0, st, (const T*)src, ld, rows, cols,
-                       factor, (T*)dst, dst_ld);
+    const dim3 grid((unsigned)cdiv(dst_ld, 64), (unsigned)cdiv(cols, 64));
+    if (((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0)
+        hipLaunchKernelGGL((k_xent_transpose<T, true>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
+    else
+        hipLaunchKernelGGL((k_xent_transpose<T, false>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
     NK_CHECK_LAUNCH("k_xent_transpose");
     return NK_OK;
 }
@@ -642,8 +762,13 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
         if ((rc = lse_launch<T>(p.kind, g, st)) < 0) return rc;
         tiles += cdiv(rows, kind_bm(p.kind));
     }
-    hipLaunchKernelGGL(k_xent_join, dim3((unsigned)cdiv(o->N, 16)), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V, target,
-                       o->ignore_index, (const float*)(ws + p.zt), lse, loss);
+    // few tokens: all threads of a workgroup on one of them
+    if (o->N <= 1024)
+        hipLaunchKernelGGL(k_xent_join<1>, dim3((unsigned)o->N), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V, target,
+                           o->ignore_index, (const float*)(ws + p.zt), lse, loss);
+    else
+        hipLaunchKernelGGL(k_xent_join<16>, dim3((unsigned)cdiv(o->N, 16)), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V,
+                           target, o->ignore_index, (const float*)(ws + p.zt), lse, loss);
     NK_CHECK_LAUNCH("k_xent_join");
     if (o->reduction != NK_REDUCE_NONE) {
         hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, loss, target, o->N, o->ignore_index, o->reduction == NK_REDUCE_MEAN, reduced);
@@ -697,10 +822,13 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
         }
     }
     if (d_hidden) {
-        const int64_t n = o->N * o->D;
-        if (cdiv(n, 256) > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_linear_xent_bwd: too large");
-        hipLaunchKernelGGL(k_xent_finish<T>, dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c, rest,
-                           unscale, (T*)d_hidden);
+        const bool four = o->D % 4 == 0 && ((uintptr_t)d_hidden & (4 * es - 1)) == 0;
+        const int64_t blocks = cdiv(o->N * o->D, four ? 1024 : 256);
+        if (blocks > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_linear_xent_bwd: too large");
+        if (four) hipLaunchKernelGGL((k_xent_finish<T, 4>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c,
+                                     rest, unscale, (T*)d_hidden);
+        else hipLaunchKernelGGL((k_xent_finish<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c,
+                                rest, unscale, (T*)d_hidden);
         NK_CHECK_LAUNCH("k_xent_finish");
     }
     return NK_OK;
