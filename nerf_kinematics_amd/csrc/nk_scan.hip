@@ -21,7 +21,8 @@
 
 namespace {
 
-enum { SC_THREADS = 256, SC_U = 8, SC_KEEP = 32 };
+enum { SC_THREADS = 256, SC_U = 8, SC_KEEP = 32,
+       SC_NONE = -(1 << 30) };      // a limit below every step: nothing is loaded, not even from in front of the first step
 #ifndef NK_SCAN_LC
 #define NK_SCAN_LC 4
 #endif
@@ -237,15 +238,33 @@ NK_D void compose_both(const float* Ain, const float* Hin, const float* Ein, con
 }
 
 // state at the start of stretch y of this launch: the (A, H) of the stretches walked before it composed
-// onto the given one (ascending in the forward pass, descending in the backward pass)
-template <int VC, bool BWD> NK_D void stretch_start(const ScanArgs& A, const Place& p, float* carry) {
+// onto the given one (ascending in the forward pass, descending in the backward pass).  The runs of a column
+// share them, each a contiguous part, and meet as the runs of a tile do.
+template <int VC, bool BWD> NK_D void stretch_start(const ScanArgs& A, const Place& p, float* carry, Buf<VC>& buf) {
     const int n = BWD ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
-#pragma unroll 4
-    for (int q = 0; q < n; ++q) {
-        const int y = BWD ? gridDim.y - 1 - q : q;
-        const float* w = A.sums + (int64_t)y * 2 * A.cols * VC + p.col * VC;
+    if (n == 0) return;             // workgroup-uniform
+    const int runs = SC_THREADS >> A.LC, per = (n + runs - 1) / runs;
+    // q: in the order of the walk; the backward composition takes the runs from the last to the first
+    const int mine = BWD ? runs - 1 - p.run : p.run, q0 = mine * per, q1 = min(n, q0 + per);
+    float Ar[VC], Hr[VC], s[VC];
 #pragma unroll
-        for (int v = 0; v < VC; ++v) carry[v] = apply(w[v], w[A.cols * VC + v], carry[v]);
+    for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = 0.0f; }
+    if (p.on) {
+#pragma unroll 4
+        for (int q = q0; q < q1; ++q) {
+            const int y = BWD ? gridDim.y - 1 - q : q;
+            const float* w = A.sums + (int64_t)y * 2 * A.cols * VC + p.col * VC;
+#pragma unroll
+            for (int v = 0; v < VC; ++v) { Hr[v] = apply(w[v], w[A.cols * VC + v], Hr[v]); Ar[v] *= w[v]; }
+        }
+    }
+    if (BWD) {
+        float zero[VC], h[VC];
+#pragma unroll
+        for (int v = 0; v < VC; ++v) zero[v] = 0.0f;
+        compose_both<VC>(Ar, zero, Hr, zero, carry, h, s, A.LC, buf);
+    } else {
+        compose_up<VC>(Ar, Hr, carry, s, A.LC, buf);
     }
 }
 
@@ -272,7 +291,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_sum(const ScanArgs A) {
         Pack<GT, GV> ra[SC_U];
         Pack<T, VC> rx[SC_U];
         fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, hi, 1.0f);
-        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, A.x ? hi : 0, 0.0f);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, A.x ? hi : SC_NONE, 0.0f);
 #pragma unroll
         for (int w = 0; w < SC_U; ++w) {
             const int u = BWD ? SC_U - 1 - w : w;
@@ -313,10 +332,8 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
     float carry[VC], s[VC];
 #pragma unroll
     for (int v = 0; v < VC; ++v) carry[v] = 0.0f;
-    if (p.on) {
-        if (A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
-        stretch_start<VC, false>(A, p, carry);
-    }
+    if (p.on && A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
+    stretch_start<VC, false>(A, p, carry, buf[1]);
     const int64_t as = A.reverse ? -A.a_st : A.a_st, xs = A.reverse ? -A.x_st : A.x_st, os = A.reverse ? -A.C : A.C;
     const GT* ab = (const GT*)A.a + p.b * A.a_sb + p.gate;
     const T* xb = (const T*)A.x + p.b * A.x_sb + p.c;
@@ -424,10 +441,8 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
     float carry[VC];
 #pragma unroll
     for (int v = 0; v < VC; ++v) carry[v] = 0.0f;
-    if (p.on) {
-        if (A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
-        stretch_start<VC, true>(A, p, carry);
-    }
+    if (p.on && A.first) for (int v = 0; v < VC; ++v) carry[v] = A.first[p.b * A.C + p.c + v];
+    stretch_start<VC, true>(A, p, carry, buf[1]);
     const bool gates = A.d_a != nullptr;
     const int64_t as = A.reverse ? -A.a_st : A.a_st, xs = A.reverse ? -A.x_st : A.x_st, gs = A.reverse ? -A.g_st : A.g_st;
     const GT* ab = (const GT*)A.a + p.b * A.a_sb + p.gate;
@@ -458,22 +473,32 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
             }
         }
     }
+    Pack<GT, GV> ra[SC_U];
+    Pack<T, VC> rx[SC_U], rg[SC_U];
+    float hs[VC];
+    // the steps of tile q, and the state in front of it
+    auto load = [&](int q, Pack<GT, GV> (&qa)[SC_U], Pack<T, VC> (&qx)[SC_U], Pack<T, VC> (&qg)[SC_U], float (&qh)[VC]) {
+        const int at = begin + q * tile, s0 = at + p.run * SC_U, most = q >= 0 ? lim : SC_NONE;
+        const int64_t t0 = time_of(s0, p.len, A.reverse);
+        fetch<GT, GV>(qa, ab + t0 * A.a_st, as, s0, most, 1.0f);
+        fetch<T, VC>(qg, gb + t0 * A.g_st, gs, s0, A.g ? most : SC_NONE, 0.0f);
+        fetch<T, VC>(qx, xb + t0 * A.x_st, xs, s0, gates ? most : SC_NONE, 0.0f);
+#pragma unroll
+        for (int v = 0; v < VC; ++v) qh[v] = 0.0f;
+        if (gates && at < most) {
+            const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
+                                        : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
+            if (from) for (int v = 0; v < VC; ++v) qh[v] = from[v];
+        }
+    };
+    load(tiles - 1, ra, rx, rg, hs);
     for (int q = tiles - 1; q >= 0; --q, flip ^= 1) {
         const int at = begin + q * tile, s0 = at + p.run * SC_U;
         const int64_t t0 = time_of(s0, p.len, A.reverse);
-        Pack<GT, GV> ra[SC_U];
-        Pack<T, VC> rx[SC_U], rg[SC_U];
-        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
-        fetch<T, VC>(rg, gb + t0 * A.g_st, gs, s0, A.g ? lim : 0, 0.0f);
-        float hs[VC], h[VC], e[VC];
-#pragma unroll
-        for (int v = 0; v < VC; ++v) hs[v] = 0.0f;
-        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, gates ? lim : 0, 0.0f);
-        if (gates) {
-            const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
-                                        : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
-            if (p.on && from && at < lim) for (int v = 0; v < VC; ++v) hs[v] = from[v];
-        }
+        Pack<GT, GV> na[SC_U];
+        Pack<T, VC> nx[SC_U], ng[SC_U];
+        float nh[VC], h[VC], e[VC];
+        load(q - 1, na, nx, ng, nh);        // in flight while this tile is composed and written
         float Ar[VC], Hr[VC], Er[VC];
 #pragma unroll
         for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = Er[v] = 0.0f; }
@@ -535,6 +560,10 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
                     }
             }
         }
+#pragma unroll
+        for (int u = 0; u < SC_U; ++u) { ra[u] = na[u]; rx[u] = nx[u]; rg[u] = ng[u]; }
+#pragma unroll
+        for (int v = 0; v < VC; ++v) hs[v] = nh[v];
     }
     if (p.on && p.run == 0 && A.last && begin == A.begin)
         for (int v = 0; v < VC; ++v) A.last[p.b * A.C + p.c + v] = carry[v];
