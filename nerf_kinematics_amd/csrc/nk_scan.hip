@@ -32,13 +32,10 @@ enum { SC_THREADS = 256, SC_U = 8, SC_KEEP = 32,
 #ifndef NK_SCAN_FILL
 #define NK_SCAN_FILL 1024
 #endif
-#ifndef NK_SCAN_CACHE
-#define NK_SCAN_CACHE 96
-#endif
 
 struct ScanArgs {
     const void* a; const void* x; const void* g;    // g: dL/dh (backward)
-    const float* h0; const float* first;            // first: state the walk starts from (h0, d_last, or what the block before left)
+    const float* h0; const float* first;            // first: state the walk starts from (h0 or d_last)
     void* o; void* d_a;                             // o: h or dL/dx
     float* last;                                    // state behind the walk (h_last, dL/dh0)
     float* states;                                  // [B][ceil(T / 32)][C]: state in front of step 32 k
@@ -47,7 +44,7 @@ struct ScanArgs {
     const int32_t* lengths;
     int64_t C, a_sb, a_st, x_sb, x_st, g_sb, g_st;
     int64_t cols, B, J;
-    int32_t T, begin, end, stretch;                 // steps [begin, end) of this launch, steps per stretch
+    int32_t T, stretch;                             // steps, steps per stretch
     int32_t G, LG, per_b, LC, reverse;              // channels per gate, columns per gate, columns per sequence
 };
 
@@ -276,8 +273,8 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_sum(const ScanArgs A) {
     const Place p = place<VC, SHARED>(A);
     constexpr int GV = SHARED ? 1 : VC;
     const int y = blockIdx.y + (BWD ? 1 : 0);        // the stretch walked last needs no sum
-    const int per = A.stretch / (SC_THREADS >> A.LC), lo = A.begin + y * A.stretch + p.run * per;
-    const int hi = min(min(lo + per, A.end), p.len);
+    const int per = A.stretch / (SC_THREADS >> A.LC), lo = y * A.stretch + p.run * per;
+    const int hi = min(lo + per, p.len);
     float Ar[VC], Hr[VC];
 #pragma unroll
     for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = 0.0f; }
@@ -327,7 +324,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
     constexpr int GV = SHARED ? 1 : VC;
     const Place p = place<VC, SHARED>(A);
     const int tile = (SC_THREADS >> A.LC) * SC_U;
-    const int begin = A.begin + blockIdx.y * A.stretch, end = min(A.end, begin + A.stretch);
+    const int begin = blockIdx.y * A.stretch, end = min(A.T, begin + A.stretch);
     const int stop = min(end, longest(p, A));           // behind it every column is dead
     float carry[VC], s[VC];
 #pragma unroll
@@ -392,7 +389,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
 #pragma unroll
     for (int v = 0; v < VC; ++v) z[v] = 0.0f;
     if (p.on) for (int t = at + p.run; t < end; t += SC_THREADS >> A.LC) st<T, VC>(ob + (int64_t)t * A.C, z);
-    if (p.on && p.run == 0 && A.last && end == A.end)
+    if (p.on && p.run == 0 && A.last && end == A.T)
         for (int v = 0; v < VC; ++v) A.last[p.b * A.C + p.c + v] = carry[v];
 }
 
@@ -436,7 +433,7 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
     constexpr int GV = SHARED ? 1 : VC;
     const Place p = place<VC, SHARED>(A);
     const int tile = (SC_THREADS >> A.LC) * SC_U;
-    const int begin = A.begin + blockIdx.y * A.stretch, end = min(A.end, begin + A.stretch);
+    const int begin = blockIdx.y * A.stretch, end = min(A.T, begin + A.stretch);
     const int stop = min(end, longest(p, A));
     float carry[VC];
 #pragma unroll
@@ -473,32 +470,22 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
             }
         }
     }
-    Pack<GT, GV> ra[SC_U];
-    Pack<T, VC> rx[SC_U], rg[SC_U];
-    float hs[VC];
-    // the steps of tile q, and the state in front of it
-    auto load = [&](int q, Pack<GT, GV> (&qa)[SC_U], Pack<T, VC> (&qx)[SC_U], Pack<T, VC> (&qg)[SC_U], float (&qh)[VC]) {
-        const int at = begin + q * tile, s0 = at + p.run * SC_U, most = q >= 0 ? lim : SC_NONE;
-        const int64_t t0 = time_of(s0, p.len, A.reverse);
-        fetch<GT, GV>(qa, ab + t0 * A.a_st, as, s0, most, 1.0f);
-        fetch<T, VC>(qg, gb + t0 * A.g_st, gs, s0, A.g ? most : SC_NONE, 0.0f);
-        fetch<T, VC>(qx, xb + t0 * A.x_st, xs, s0, gates ? most : SC_NONE, 0.0f);
-#pragma unroll
-        for (int v = 0; v < VC; ++v) qh[v] = 0.0f;
-        if (gates && at < most) {
-            const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
-                                        : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
-            if (from) for (int v = 0; v < VC; ++v) qh[v] = from[v];
-        }
-    };
-    load(tiles - 1, ra, rx, rg, hs);
     for (int q = tiles - 1; q >= 0; --q, flip ^= 1) {
         const int at = begin + q * tile, s0 = at + p.run * SC_U;
         const int64_t t0 = time_of(s0, p.len, A.reverse);
-        Pack<GT, GV> na[SC_U];
-        Pack<T, VC> nx[SC_U], ng[SC_U];
-        float nh[VC], h[VC], e[VC];
-        load(q - 1, na, nx, ng, nh);        // in flight while this tile is composed and written
+        Pack<GT, GV> ra[SC_U];
+        Pack<T, VC> rx[SC_U], rg[SC_U];
+        float hs[VC], h[VC], e[VC];
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
+        fetch<T, VC>(rg, gb + t0 * A.g_st, gs, s0, A.g ? lim : SC_NONE, 0.0f);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, gates ? lim : SC_NONE, 0.0f);
+#pragma unroll
+        for (int v = 0; v < VC; ++v) hs[v] = 0.0f;
+        if (gates && at < lim) {            // the state in front of the tile
+            const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
+                                        : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
+            if (from) for (int v = 0; v < VC; ++v) hs[v] = from[v];
+        }
         float Ar[VC], Hr[VC], Er[VC];
 #pragma unroll
         for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = Er[v] = 0.0f; }
@@ -560,12 +547,8 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
                     }
             }
         }
-#pragma unroll
-        for (int u = 0; u < SC_U; ++u) { ra[u] = na[u]; rx[u] = nx[u]; rg[u] = ng[u]; }
-#pragma unroll
-        for (int v = 0; v < VC; ++v) hs[v] = nh[v];
     }
-    if (p.on && p.run == 0 && A.last && begin == A.begin)
+    if (p.on && p.run == 0 && A.last && begin == 0)
         for (int v = 0; v < VC; ++v) A.last[p.b * A.C + p.c + v] = carry[v];
 }
 
@@ -580,12 +563,12 @@ __global__ __launch_bounds__(256) void k_gate_sum(const float* __restrict__ part
 }
 
 struct Shape {
-    int VC, LC, S, parts, blocks;           // blocks: launches along the sequence
+    int VC, LC, S, parts;
     int64_t cols;
-    int32_t stretch, block;
+    int32_t stretch;
     int32_t G, LG, per_b;
     bool shared;
-    int64_t carry_bytes, sums_bytes, part_bytes;
+    int64_t sums_bytes, part_bytes;
 };
 
 inline int ceil_log2(int64_t x) { int k = 0; while (((int64_t)1 << k) < x) ++k; return k; }
@@ -621,24 +604,9 @@ void shape_of(const nk_scan_opts* o, bool vec, int bwd, Shape* s) {
     const int64_t groups = (s->cols + lcol - 1) / lcol, tile = (int64_t)(SC_THREADS >> LC) * SC_U;
     const int64_t tiles = (o->T + tile - 1) / tile;
     int64_t S = 1;
-    s->block = (int32_t)(tiles * tile);
-    if (groups < NK_SCAN_FEW && tiles > 1) {
-        // the second launch of a split block finds what the first one read in the 256 MB cache behind the L2s
-        const int64_t row = o->B * (o->C * elem(o->dtype) + o->gates * elem(o->gate_dtype));
-        int64_t fit = ((int64_t)NK_SCAN_CACHE << 20) / (row * tile);
-        if (fit < 1) fit = 1;
-        const int64_t blocks = (tiles + fit - 1) / fit;
-        const int64_t per = (tiles + blocks - 1) / blocks;
-        s->block = (int32_t)(per * tile);
-        S = (NK_SCAN_FILL + groups - 1) / groups;
-        if (S > per) S = per;
-        s->stretch = (int32_t)((per + S - 1) / S * tile);
-    } else {
-        s->stretch = s->block;
-    }
-    s->S = (s->block + s->stretch - 1) / s->stretch;
-    s->blocks = (int)((o->T + s->block - 1) / s->block);
-    s->carry_bytes = s->blocks > 1 ? up256(o->B * o->C * 4) : 0;
+    if (groups < NK_SCAN_FEW) { S = (NK_SCAN_FILL + groups - 1) / groups; if (S > tiles) S = tiles; }
+    s->stretch = (int32_t)((tiles + S - 1) / S * tile);
+    s->S = (int)((o->T + s->stretch - 1) / s->stretch);
     s->sums_bytes = s->S > 1 ? up256((int64_t)s->S * 2 * s->cols * s->VC * 4) : 0;
     s->part_bytes = bwd && s->parts > 1 ? (int64_t)s->parts * o->B * o->T * o->gates * 4 : 0;
 }
@@ -658,39 +626,27 @@ int check(const nk_scan_opts* o, const char* who) {
 }
 
 template <typename T, typename GT, int VC, bool SHARED, bool BWD>
-void launch(ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
+void launch(const ScanArgs& A, const Shape& s, hipStream_t st) {
     const unsigned groups = (unsigned)((s.cols + (1 << s.LC) - 1) >> s.LC);
-    float* last = A.last;
-    const int64_t n = s.carry_bytes / 4;        // two buffers in turn: a block's first stretches read what its last one replaces
-    for (int q = 0; q < s.blocks; ++q) {
-        const int k = BWD ? s.blocks - 1 - q : q;
-        A.begin = k * s.block;
-        A.end = (int)((int64_t)A.begin + s.block < A.T ? A.begin + s.block : A.T);
-        A.stretch = s.stretch;
-        const int S = (A.end - A.begin + s.stretch - 1) / s.stretch;
-        A.last = q + 1 < s.blocks ? carry + (q & 1) * n : last;
-        if (S > 1) {
-            ScanArgs B = A;
-            if (BWD) { B.x = A.g; B.x_sb = A.g_sb; B.x_st = A.g_st; }
-            hipLaunchKernelGGL((k_scan_sum<T, GT, VC, SHARED, BWD>), dim3(groups, S - 1), dim3(SC_THREADS), 0, st, B);
-        }
-        if constexpr (BWD) hipLaunchKernelGGL((k_scan_bwd<T, GT, VC, SHARED>), dim3(groups, S), dim3(SC_THREADS), 0, st, A);
-        else hipLaunchKernelGGL((k_scan_fwd<T, GT, VC, SHARED>), dim3(groups, S), dim3(SC_THREADS), 0, st, A);
-        A.first = carry + (q & 1) * n;
+    if (s.S > 1) {
+        ScanArgs B = A;
+        if (BWD) { B.x = A.g; B.x_sb = A.g_sb; B.x_st = A.g_st; }
+        hipLaunchKernelGGL((k_scan_sum<T, GT, VC, SHARED, BWD>), dim3(groups, s.S - 1), dim3(SC_THREADS), 0, st, B);
     }
+    if constexpr (BWD) hipLaunchKernelGGL((k_scan_bwd<T, GT, VC, SHARED>), dim3(groups, s.S), dim3(SC_THREADS), 0, st, A);
+    else hipLaunchKernelGGL((k_scan_fwd<T, GT, VC, SHARED>), dim3(groups, s.S), dim3(SC_THREADS), 0, st, A);
 }
-
 template <typename T, typename GT, bool BWD>
-void launch_vc(ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
-    if (s.VC == 4) { if (s.shared) launch<T, GT, 4, true, BWD>(A, s, carry, st); else launch<T, GT, 4, false, BWD>(A, s, carry, st); }
-    else { if (s.shared) launch<T, GT, 1, true, BWD>(A, s, carry, st); else launch<T, GT, 1, false, BWD>(A, s, carry, st); }
+void launch_vc(const ScanArgs& A, const Shape& s, hipStream_t st) {
+    if (s.VC == 4) { if (s.shared) launch<T, GT, 4, true, BWD>(A, s, st); else launch<T, GT, 4, false, BWD>(A, s, st); }
+    else { if (s.shared) launch<T, GT, 1, true, BWD>(A, s, st); else launch<T, GT, 1, false, BWD>(A, s, st); }
 }
 template <bool BWD>
-int launch_types(const nk_scan_opts* o, ScanArgs& A, const Shape& s, float* carry, hipStream_t st) {
+int launch_types(const nk_scan_opts* o, const ScanArgs& A, const Shape& s, hipStream_t st) {
     const bool g32 = o->gate_dtype == NK_F32;
-    if (o->dtype == NK_F32) launch_vc<float, float, BWD>(A, s, carry, st);
-    else if (o->dtype == NK_BF16) { if (g32) launch_vc<__bf16, float, BWD>(A, s, carry, st); else launch_vc<__bf16, __bf16, BWD>(A, s, carry, st); }
-    else { if (g32) launch_vc<_Float16, float, BWD>(A, s, carry, st); else launch_vc<_Float16, _Float16, BWD>(A, s, carry, st); }
+    if (o->dtype == NK_F32) launch_vc<float, float, BWD>(A, s, st);
+    else if (o->dtype == NK_BF16) { if (g32) launch_vc<__bf16, float, BWD>(A, s, st); else launch_vc<__bf16, __bf16, BWD>(A, s, st); }
+    else { if (g32) launch_vc<_Float16, float, BWD>(A, s, st); else launch_vc<_Float16, _Float16, BWD>(A, s, st); }
     NK_CHECK_LAUNCH("k_scan");
     if (BWD && s.parts > 1 && A.d_a) {
         const int64_t n = o->B * o->T * o->gates;
@@ -712,19 +668,17 @@ bool can_vec(const nk_scan_opts* o, const void* a, const void* x, const void* g,
     return ((uintptr_t)a % ge) == 0 && ((uintptr_t)d_a % ge) == 0 && o->a_stride_b % 4 == 0 && o->a_stride_t % 4 == 0;
 }
 
-ScanArgs args_of(const nk_scan_opts* o, const Shape& s, void* ws, float** carry) {
+ScanArgs args_of(const nk_scan_opts* o, const Shape& s, void* ws) {
     ScanArgs A = {};
     A.lengths = o->lengths; A.T = (int32_t)o->T; A.C = o->C; A.B = o->B; A.J = o->gates;
     A.a_sb = o->a_stride_b; A.a_st = o->a_stride_t; A.x_sb = o->x_stride_b; A.x_st = o->x_stride_t;
     A.g_sb = o->g_stride_b; A.g_st = o->g_stride_t;
-    A.cols = s.cols; A.G = s.G; A.LG = s.LG; A.per_b = s.per_b; A.LC = s.LC; A.reverse = o->reverse != 0;
-    *carry = (float*)ws;
-    A.sums = (float*)((char*)ws + 2 * s.carry_bytes);
-    A.gate_part = (float*)((char*)ws + 2 * s.carry_bytes + s.sums_bytes);
+    A.stretch = s.stretch; A.cols = s.cols; A.G = s.G; A.LG = s.LG; A.per_b = s.per_b; A.LC = s.LC; A.reverse = o->reverse != 0;
+    A.sums = (float*)ws; A.gate_part = (float*)((char*)ws + s.sums_bytes);
     return A;
 }
 
-int64_t bytes_of(const Shape& s) { return 2 * s.carry_bytes + s.sums_bytes + s.part_bytes; }
+int64_t bytes_of(const Shape& s) { return s.sums_bytes + s.part_bytes; }
 
 }  // namespace
 
@@ -758,10 +712,9 @@ extern "C" int nk_gated_scan_fwd(const nk_scan_opts* o, const void* a, const voi
     shape_of(o, can_vec(o, a, x, nullptr, h, nullptr, states), 0, &s);
     if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
         NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_fwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
-    float* carry;
-    ScanArgs A = args_of(o, s, workspace, &carry);
+    ScanArgs A = args_of(o, s, workspace);
     A.a = a; A.x = x; A.first = h0; A.o = h; A.last = h_last; A.states = states;
-    return launch_types<false>(o, A, s, carry, nk_stream(stream));
+    return launch_types<false>(o, A, s, nk_stream(stream));
 }
 
 extern "C" int nk_gated_scan_bwd(const nk_scan_opts* o, const void* a, const void* x, const float* states, const float* h0,
@@ -776,8 +729,7 @@ extern "C" int nk_gated_scan_bwd(const nk_scan_opts* o, const void* a, const voi
     shape_of(o, can_vec(o, a, d_a ? x : nullptr, d_h, d_x, d_a, states), 1, &s);
     if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
         NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_bwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
-    float* carry;
-    ScanArgs A = args_of(o, s, workspace, &carry);
+    ScanArgs A = args_of(o, s, workspace);
     A.a = a; A.x = x; A.g = d_h; A.h0 = h0; A.states = (float*)states; A.first = d_h_last; A.o = d_x; A.d_a = d_a; A.last = d_h0;
-    return launch_types<true>(o, A, s, carry, nk_stream(stream));
+    return launch_types<true>(o, A, s, nk_stream(stream));
 }
