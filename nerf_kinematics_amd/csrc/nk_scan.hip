@@ -17,22 +17,24 @@
 //
 // Where there are too few columns to fill the chip the sequence itself is cut into stretches (grid.y): a
 // first launch reduces every stretch to its (A, H), the second composes those in front of its own and walks.
+//
+// What bounds it, and the measurements behind the constants (MI355X; a copy reaches 4.8 TB/s here).  The walk is
+// a chain of load, compose, store per tile, so what counts is wavefronts in flight, not work per thread:
+//   two channels a thread (90-115 registers, 4-5 wavefronts a SIMD) against four (140-190, 2-3): 123 against
+//   215 us forward + backward for 4096 ragged sequences x 192 x 64 in bf16 with one fp32 gate a step, 312 against
+//   389 us for 2 x 32768 x 1024; one channel a thread: 146 and 403 us.
+//   8 steps a run against 4: 123 / 146 us and 312 / 375 us.
+//   Loading the next tile ahead in the backward pass costs registers and loses (280 against 164 us); in the
+//   forward pass it gains.
+// 2 x 32768 x 1024 in bf16 then takes 124 us forward (53 of them the first launch, 5.1 TB/s; the walk
+// moves 5.6 TB/s with the first launch's reads partly cached) and 186 us backward, against 169 us that the bytes of
+// one pass over every tensor cost; reading a and x (a and g) twice is what is left.
 #include "nk_common.h"
 
 namespace {
 
-enum { SC_THREADS = 256, SC_U = 8, SC_KEEP = 32,
+enum { SC_THREADS = 256, SC_VC = 2, SC_U = 8, SC_KEEP = 32,
        SC_NONE = -(1 << 30) };      // a limit below every step: nothing is loaded, not even from in front of the first step
-#ifndef NK_SCAN_LC
-#define NK_SCAN_LC 4
-#endif
-#ifndef NK_SCAN_FEW
-#define NK_SCAN_FEW 512
-#endif
-#ifndef NK_SCAN_FILL
-#define NK_SCAN_FILL 1024
-#endif
-
 struct ScanArgs {
     const void* a; const void* x; const void* g;    // g: dL/dh (backward)
     const float* h0; const float* first;            // first: state the walk starts from (h0 or d_last)
@@ -579,20 +581,23 @@ inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
 void shape_of(const nk_scan_opts* o, bool vec, int bwd, Shape* s) {
     s->G = (int32_t)(o->C / o->gates);
     s->shared = s->G > 1;
-    s->VC = vec && (s->shared ? s->G : o->C) % 4 == 0 ? 4 : 1;
+    s->VC = vec && (s->shared ? s->G : o->C) % SC_VC == 0 ? SC_VC : 1;
     const int64_t unit = s->shared ? (s->G + s->VC - 1) / s->VC : (o->C + s->VC - 1) / s->VC;
-    const int64_t all = (s->shared ? o->gates : 1) * o->B * unit;
-    // 16 columns x 16 runs (a row of a tile is 128 bytes of bf16 at four channels a column), 64 x 4 at one
-    int LC = s->VC == 4 ? NK_SCAN_LC : 6;
-    while (LC > 2 && ((int64_t)1 << LC) > all) --LC;
+    const int64_t row = unit * (s->shared ? o->gates : 1);
+    // As many columns as a row has, up to a wavefront of them: neighbouring lanes then read neighbouring
+    // channels, and narrow rows neighbouring steps (3038 x 3648 x 2: 123 us with 4 columns x 64 runs, 393 us
+    // with 64 x 4; 64 channels: 32 x 8 and 64 x 4 the same).
+    int LC = ceil_log2(row);
+    LC = LC > 6 ? 6 : LC < 2 ? 2 : LC;
     const int runs_wanted = ceil_log2((o->T + SC_U - 1) / SC_U);
     if (runs_wanted < 8 - LC) LC = 8 - runs_wanted;
     if (LC == 7) LC = 6;
     s->LC = LC;
     const int lcol = 1 << LC;
     if (s->shared) {
+        // the backward pass adds over a gate's columns with lane shuffles: a power of two of them, or whole wavefronts
         const int64_t p2 = (int64_t)1 << ceil_log2(unit);
-        s->LG = (int32_t)(p2 <= lcol ? p2 : (unit + lcol - 1) / lcol * lcol);
+        s->LG = (int32_t)(!bwd ? unit : p2 <= lcol ? p2 : (unit + lcol - 1) / lcol * lcol);
         s->per_b = (int32_t)(s->LG * o->gates);
     } else {
         s->LG = 1;
@@ -600,11 +605,13 @@ void shape_of(const nk_scan_opts* o, bool vec, int bwd, Shape* s) {
     }
     s->cols = o->B * s->per_b;
     const int wide = lcol < 64 ? lcol : 64;
-    s->parts = s->shared && s->LG > wide ? s->LG / wide : 1;
+    s->parts = bwd && s->shared && s->LG > wide ? s->LG / wide : 1;
     const int64_t groups = (s->cols + lcol - 1) / lcol, tile = (int64_t)(SC_THREADS >> LC) * SC_U;
     const int64_t tiles = (o->T + tile - 1) / tile;
+    // 128 groups: 70 us split, 147 whole; 256: 68 and 81; 384: 61 and 59 (forward + backward, 16 M elements).  To 1024
+    // workgroups, four a CU: 512 are 10 to 25 % slower, 2048 up to 20 %.
     int64_t S = 1;
-    if (groups < NK_SCAN_FEW) { S = (NK_SCAN_FILL + groups - 1) / groups; if (S > tiles) S = tiles; }
+    if (groups < 384) { S = (1024 + groups - 1) / groups; if (S > tiles) S = tiles; }
     s->stretch = (int32_t)((tiles + S - 1) / S * tile);
     s->S = (int)((o->T + s->stretch - 1) / s->stretch);
     s->sums_bytes = s->S > 1 ? up256((int64_t)s->S * 2 * s->cols * s->VC * 4) : 0;
@@ -638,7 +645,7 @@ void launch(const ScanArgs& A, const Shape& s, hipStream_t st) {
 }
 template <typename T, typename GT, bool BWD>
 void launch_vc(const ScanArgs& A, const Shape& s, hipStream_t st) {
-    if (s.VC == 4) { if (s.shared) launch<T, GT, 4, true, BWD>(A, s, st); else launch<T, GT, 4, false, BWD>(A, s, st); }
+    if (s.VC > 1) { if (s.shared) launch<T, GT, SC_VC, true, BWD>(A, s, st); else launch<T, GT, SC_VC, false, BWD>(A, s, st); }
     else { if (s.shared) launch<T, GT, 1, true, BWD>(A, s, st); else launch<T, GT, 1, false, BWD>(A, s, st); }
 }
 template <bool BWD>
@@ -659,13 +666,14 @@ int launch_types(const nk_scan_opts* o, const ScanArgs& A, const Shape& s, hipSt
     return NK_OK;
 }
 
-// four channels per load: every row of every tensor starts on a multiple of four elements
+// SC_VC channels per load: every row of every tensor starts on a multiple of as many elements
 bool can_vec(const nk_scan_opts* o, const void* a, const void* x, const void* g, const void* out, const void* d_a, const void* states) {
-    const int64_t e = elem(o->dtype) * 4, ge = elem(o->gate_dtype) * 4;
-    if (((uintptr_t)x % e) || ((uintptr_t)g % e) || ((uintptr_t)out % e) || ((uintptr_t)states % 16) || o->C % 4) return false;
-    if ((x && (o->x_stride_b % 4 || o->x_stride_t % 4)) || (g && (o->g_stride_b % 4 || o->g_stride_t % 4))) return false;
+    constexpr int V = SC_VC;
+    const uintptr_t e = elem(o->dtype) * V, ge = elem(o->gate_dtype) * V;
+    if (((uintptr_t)x % e) || ((uintptr_t)g % e) || ((uintptr_t)out % e) || ((uintptr_t)states % (4 * V)) || o->C % V) return false;
+    if ((x && (o->x_stride_b % V || o->x_stride_t % V)) || (g && (o->g_stride_b % V || o->g_stride_t % V))) return false;
     if (o->gates != o->C) return true;
-    return ((uintptr_t)a % ge) == 0 && ((uintptr_t)d_a % ge) == 0 && o->a_stride_b % 4 == 0 && o->a_stride_t % 4 == 0;
+    return ((uintptr_t)a % ge) == 0 && ((uintptr_t)d_a % ge) == 0 && o->a_stride_b % V == 0 && o->a_stride_t % V == 0;
 }
 
 ScanArgs args_of(const nk_scan_opts* o, const Shape& s, void* ws) {
