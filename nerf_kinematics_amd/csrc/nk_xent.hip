@@ -311,21 +311,46 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2* __restrict__ pa
     }
 }
 
-// sum (and mean over the tokens that count) in one order: one workgroup
-__global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ loss, const int64_t* __restrict__ target, int64_t N,
-                                                      int64_t ignore, int mean, float* __restrict__ out) {
+// Sum or mean over the tokens that count, in one order, by one workgroup of 1024 threads.
+NK_D void reduce_losses(double s, int k, int mean, float* out) {
     __shared__ double sums[16];
-    __shared__ int64_t counts[16];
-    double s = 0.0;
-    int64_t k = 0;
-    for (int64_t n = threadIdx.x; n < N; n += 1024) { s += (double)loss[n]; k += target[n] != ignore; }
-    for (int off = 32; off > 0; off >>= 1) { s += __shfl_xor(s, off, 64); k += __shfl_xor((int)k, off, 64); }
+    __shared__ int counts[16];
+    for (int off = 32; off > 0; off >>= 1) { s += __shfl_xor(s, off, 64); k += __shfl_xor(k, off, 64); }
     if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = s; counts[threadIdx.x >> 6] = k; }
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) { s += sums[w]; k += counts[w]; }
         out[0] = (float)(mean ? s / (double)(k > 0 ? k : 1) : s);
     }
+}
+
+// k_xent_join and k_xent_reduce in one launch where a thread per token is enough (N <= 1024, few tiles)
+__global__ __launch_bounds__(1024) void k_xent_join_reduce(const float2* __restrict__ part, int tiles, int N, int64_t V, const int64_t* __restrict__ target,
+                                                           int64_t ignore, const float* __restrict__ zt, int mean, float* __restrict__ lse,
+                                                           float* __restrict__ loss, float* __restrict__ out) {
+    const int n = threadIdx.x;
+    float l = 0.0f;
+    int k = 0;
+    if (n < N) {
+        float2 r = part[n];
+#pragma unroll 4
+        for (int t = 1; t < tiles; ++t) r = join(r, part[(int64_t)t * N + n]);
+        const float e = r.x + logf(r.y);
+        const int64_t t = target[n];
+        l = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : e - zt[n];
+        k = t != ignore;
+        lse[n] = e;
+        loss[n] = l;
+    }
+    reduce_losses((double)l, k, mean, out);
+}
+
+__global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ loss, const int64_t* __restrict__ target, int64_t N,
+                                                      int64_t ignore, int mean, float* __restrict__ out) {
+    double s = 0.0;
+    int k = 0;                  // N is at most 2^24
+    for (int64_t n = threadIdx.x; n < N; n += 1024) { s += (double)loss[n]; k += target[n] != ignore; }
+    reduce_losses(s, k, mean, out);
 }
 
 // ---- backward ---------------------------------------------------------------------------------
@@ -490,6 +515,7 @@ struct ProductArgs {
     void* out; int64_t ld;                  // [n][m]
     float* sums; int add;                   // fp32 sums [slice][n][m] instead; add: onto what is there
     const float* rest; float scale;
+    const float* row_on;                    // out: rows n with row_on[n] = 0 are zero
 };
 
 // C[m][n] -> out[n][m]: a lane holds four consecutive m of one n
@@ -510,6 +536,7 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g
     for (int j = 0; j < C::TN; ++j) {
         const int64_t n = ni * C::BN + wn * C::TN * 16 + j * 16 + (lane & 15);
         if (n >= g.N) continue;
+        const bool off = !SUMS && g.row_on && g.row_on[n] == 0.0f;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i) {
             const int64_t m = mi * C::BM + wm * C::TM * 16 + i * 16 + 4 * (lane >> 4);
@@ -526,6 +553,7 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g
                 }
             } else {
                 T* o = (T*)g.out + n * g.ld + m;
+                if (off) acc[i][j] = f32x4{0, 0, 0, 0};
                 if (vec && m + 4 <= g.M) {
                     typedef __attribute__((ext_vector_type(4))) T vt;
                     vt w;
@@ -692,7 +720,7 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
         if (cut > most) cut = most;
         if (cut > 16) cut = 16;
         p->slices = (int)(cut < 1 ? 1 : cut);
-        p->sums = take((int64_t)p->slices * o->N * o->D * 4);
+        p->sums = take(p->slices == 1 && piece >= o->V ? 0 : (int64_t)p->slices * o->N * o->D * 4);
     }
     p->total = off;
     return NK_OK;
@@ -762,6 +790,12 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
         if ((rc = lse_launch<T>(p.kind, g, st)) < 0) return rc;
         tiles += cdiv(rows, kind_bm(p.kind));
     }
+    if (o->reduction != NK_REDUCE_NONE && o->N <= 1024 && tiles <= 32) {
+        hipLaunchKernelGGL(k_xent_join_reduce, dim3(1), dim3(1024), 0, st, (const float2*)(ws + p.parts), (int)tiles, (int)o->N, o->V, target,
+                           o->ignore_index, (const float*)(ws + p.zt), (int)(o->reduction == NK_REDUCE_MEAN), lse, loss, reduced);
+        NK_CHECK_LAUNCH("k_xent_join_reduce");
+        return NK_OK;
+    }
     // few tokens: all threads of a workgroup on one of them
     if (o->N <= 1024)
         hipLaunchKernelGGL(k_xent_join<1>, dim3((unsigned)o->N), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V, target,
@@ -794,6 +828,7 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
     }
     if (d_weight && (rc = transpose<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.ht, p.Np, st)) < 0) return rc;
     const int64_t slice = up(cdiv(p.piece, p.slices), 128 / es) * es;
+    const bool direct = p.slices == 1 && p.piece >= o->V;      // d_hidden in one product: no sums to keep
     for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
         const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
         const char* src = (const char*)weight + v0 * o->weight_stride * es;
@@ -817,11 +852,16 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
             ProductArgs q = {};
             q.a = Mat{ws + p.wt, o->D, kv * es}; q.b = Mat{ws + p.dz, o->N, kv * es};
             q.kbytes = kv * es; q.kslice = slice; q.M = o->D; q.N = o->N;
-            q.sums = (float*)(ws + p.sums); q.add = v0 > 0;
-            if ((rc = product_launch<T, true>(q, p.slices, st)) < 0) return rc;
+            if (direct) {
+                q.out = d_hidden; q.ld = o->D; q.rest = rest; q.scale = unscale; q.row_on = c;
+                if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+            } else {
+                q.sums = (float*)(ws + p.sums); q.add = v0 > 0;
+                if ((rc = product_launch<T, true>(q, p.slices, st)) < 0) return rc;
+            }
         }
     }
-    if (d_hidden) {
+    if (d_hidden && !direct) {
         const bool four = o->D % 4 == 0 && ((uintptr_t)d_hidden & (4 * es - 1)) == 0;
         const int64_t blocks = cdiv(o->N * o->D, four ? 1024 : 256);
         if (blocks > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_linear_xent_bwd: too large");
