@@ -223,7 +223,7 @@ enum { NK_F32 = 0, NK_BF16 = 1, NK_F16 = 2 };
  *   lengths   NULL, or B device ints: sequence b has clamp(lengths[b], 0, T) steps.  Rows behind it are not read;
  *             the outputs there (h, d_a, d_x) are zero, and a reversed sequence starts at its own last step.
  * a, x and d_h may be strided over B and T, with unit channel stride; strides
- * in elements, zero allowed.  h, d_a and d_x are contiguous.                                         */
+ * in elements, zero allowed.  h, d_a and d_x are contiguous; outputs overlap no input.                */
 typedef struct nk_scan_opts {
     int64_t B, T, C, gates;
     int32_t dtype;                /* of x, h, d_h, d_x: NK_F32 | NK_BF16 | NK_F16              */
@@ -264,7 +264,8 @@ typedef struct nk_xent_opts {
     int32_t dtype;                /* NK_F32 | NK_BF16 | NK_F16                                */
     int32_t reduction;            /* NK_REDUCE_*                                              */
     int64_t piece;                /* rows of the vocabulary per piece of the backward call, rounded up to 256;
-                                     0: as many as keep a piece's gradients (2 N piece elements) near 256 MB */
+                                     0: as many as keep a piece's gradients (2 N piece elements) near
+                                     256 MB, 2048 at least                                 */
 } nk_xent_opts;
 /* Scratch of a call on these operands (256-byte aligned; it holds nothing between calls). */
 int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int backward);

@@ -18,9 +18,7 @@ namespace {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-#ifndef NK_XENT_PIECE_MB
-#define NK_XENT_PIECE_MB 256
-#endif
+enum { XENT_PIECE_MB = 256 };      // both orders of a piece's dz together, unless the caller names a piece
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -686,12 +684,13 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
     auto aligned = [&](const void* q, int64_t stride) { return ((uintptr_t)q & 15) == 0 && (stride * es) % 16 == 0 && (o->D * es) % 16 == 0; };
     p->pad_h = !aligned(hidden, o->hidden_stride); p->pad_w = !aligned(weight, o->weight_stride);
     p->Np = up(o->N, step);
+    const int64_t asked = o->piece < o->V ? up(o->piece, 256) : up(o->V, 256);       // 0: not asked for
     int64_t piece;
     if (backward) {
-        piece = o->piece ? up(o->piece, 256) : up((int64_t)(NK_XENT_PIECE_MB / 2 << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
-        if (piece < 2048 && !o->piece) piece = 2048;
+        piece = asked ? asked : up((int64_t)(XENT_PIECE_MB / 2 << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
+        if (piece < 2048 && !asked) piece = 2048;
     } else {
-        piece = p->pad_w ? (o->piece ? up(o->piece, 256) : 16384) : up(o->V, 256);
+        piece = p->pad_w ? (asked ? asked : 16384) : up(o->V, 256);
     }
     if (piece > up(o->V, 256)) piece = up(o->V, 256);
     p->piece = piece;

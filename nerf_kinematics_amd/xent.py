@@ -13,8 +13,10 @@ from .scan import _ptr
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
     N, D = hidden.shape
-    return _lib.NkXentOpts(N, D, weight.shape[0], hidden.stride(0), weight.stride(0), ignore_index, _lib.DTYPES[hidden.dtype],
-                           reduction, piece)
+    V = weight.shape[0]
+    # a dimension of one row has any stride
+    return _lib.NkXentOpts(N, D, V, hidden.stride(0) if N > 1 else D, weight.stride(0) if V > 1 else D, ignore_index,
+                           _lib.DTYPES[hidden.dtype], reduction, piece)
 
 
 def _workspace(L, o, hidden, weight, backward):
@@ -75,7 +77,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     tokens that are not ignored; 0 without any), "sum" or "none" ([N] losses).
 
     Differentiable in ``hidden`` and ``weight`` (first order).  The backward pass walks the vocabulary in pieces
-    of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB) and rounds the logit
+    of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB, 2048 at least) and rounds the logit
     gradients once to the operands' dtype between its products; sums are float32.
     """
     if reduction not in _lib.REDUCTIONS:

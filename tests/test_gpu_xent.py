@@ -185,6 +185,17 @@ def test_layouts(which):
 
 
 @gpu
+def test_single_rows_of_any_stride():
+    """One token and one label: torch gives a dimension of size one any stride, zero among them."""
+    h, w, t, g = make(1, 24, 1, BF16, 12, ignored=0.0)
+    one = h[0].as_strided((1, 24), (0, 1))
+    check(one, w, t, "none", g)
+    check(h, w[0].as_strided((1, 24), (3, 1)), t, "mean", g)
+    h, w, t, g = make(1, 24, 700, BF16, 13, ignored=0.0)
+    check(h[0].as_strided((1, 24), (0, 1)), w, t, "sum", g, piece=2 ** 62)
+
+
+@gpu
 def test_only_one_gradient():
     import nerf_kinematics_amd as nk
     h, w, t, g = make(100, 64, 500, BF16, 9)
