@@ -16,7 +16,8 @@
 
 namespace {
 
-enum { AW_MAX_TENSORS = 56, AW_THREADS = 256, AW_BLOCK = 256, AW_CHUNK = 4 * AW_THREADS };
+enum { AW_MAX_TENSORS = 56, AW_THREADS = 256, AW_BLOCK = 256, AW_CHUNK = 4 * AW_THREADS,
+       AW_MOST = (1 << 24) - 1 };       // workgroups of a launch: fewer than 2^32 threads
 
 // The tensors travel as kernel arguments (no device table to allocate, upload or keep in step with the
 // caller's buffers): 56 x 64 bytes + 56 x 4 + scalars stays below the 4 096 bytes of an argument block.
@@ -211,7 +212,7 @@ extern "C" int nk_adamw_step(const nk_adamw_tensor* tensors, int32_t count, cons
         if (t.n == 0) continue;
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (eight && (!t.scale_m || !t.scale_v)))
             NK_FAIL(NK_ERR_ARG, "nk_adamw_step: null pointer in tensor %d", k);
-        if (t.n > (int64_t)AW_CHUNK * 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_adamw_step: tensor %d is too large", k);
+        if (t.n > (int64_t)AW_CHUNK * AW_MOST) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_adamw_step: tensor %d is too large", k);
     }
     AwArgs a;
     a.omb1 = (float)(1.0 - o->beta1); a.b2 = (float)o->beta2; a.omb2 = (float)(1.0 - o->beta2); a.eps = (float)o->eps;
@@ -229,7 +230,7 @@ extern "C" int nk_adamw_step(const nk_adamw_tensor* tensors, int32_t count, cons
         for (; k < count && held < AW_MAX_TENSORS; ++k) {
             if (tensors[k].n == 0) continue;
             const uint64_t more = (uint64_t)((tensors[k].n + AW_CHUNK - 1) / AW_CHUNK);
-            if (held > 0 && blocks + more > 0x7FFFFFFFu) break;
+            if (held > 0 && blocks + more > AW_MOST) break;
             a.t[held] = tensors[k]; a.first[held] = (uint32_t)blocks;
             blocks += more; ++held;
         }

@@ -14,12 +14,14 @@ import ctypes as C
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import lib as _lib
 
 BLOCK = 256                       # elements that share a scale in an 8-bit moment
 MOMENT_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
 _TENSOR_WORDS = C.sizeof(_lib.NkAdamwTensor) // 8
+_address = torch.Tensor.data_ptr
 
 
 def _check_list(name: str, tensors: Sequence[torch.Tensor], numels: Sequence[int], dtype: torch.dtype, device, spans: list) -> List[int]:
@@ -37,6 +39,8 @@ def _check_list(name: str, tensors: Sequence[torch.Tensor], numels: Sequence[int
         at = t.data_ptr()
         out.append(at)
         if numels[i]:
+            if at == 0:
+                raise ValueError(f"{name}[{i}]: has no storage")
             spans.append((at, at + numels[i] * size))
     return out
 
@@ -93,7 +97,8 @@ class AdamW:
     ``params``: contiguous GPU tensors of one dtype (fp32, bf16 or fp16) on one device.  ``masters``: fp32
     copies that the step updates instead, the parameters then receive them rounded; low-precision
     parameters without masters lose updates below half their last place.  ``state_bits``: 32 or 8.
-    ``state``: moments to continue from, as ``adamw_state`` lays them out (their dtype decides the format)."""
+    ``state``: moments to continue from, as ``adamw_state`` lays them out (their dtype decides the format); they
+    stay the optimiser's, load into them with ``copy_``.  Parameters and masters may move (``p.data = ...``)."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, masters: Optional[Sequence[torch.Tensor]] = None,
@@ -109,60 +114,72 @@ class AdamW:
             raise ValueError("AdamW: expected GPU tensors (there is no CPU implementation)")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
             raise ValueError(f"AdamW: betas={tuple(betas)} in [0, 1), eps={eps} >= 0 wanted")
-        numels, spans, n = [p.numel() for p in params], [], len(params)
-        none = [0] * n
-        at_p = _check_list("params", params, numels, dt, dev, spans)
-        at_w = none if masters is None else _check_list("masters", masters, numels, torch.float32, dev, spans)
         if state is None:
             state = adamw_state(params, state_bits)
         m, v, scales = state
         if not m or m[0].dtype not in (torch.float32, torch.float8_e4m3fn):
             raise ValueError("AdamW: moments are float32 or float8_e4m3fn / float8_e5m2")
         state_bits = 32 if m[0].dtype == torch.float32 else 8
-        at_m = _check_list("exp_avgs", m, numels, MOMENT_DTYPES[state_bits][0], dev, spans)
-        at_v = _check_list("exp_avg_sqs", v, numels, MOMENT_DTYPES[state_bits][1], dev, spans)
-        at_sm = at_sv = none
-        if state_bits == 8:
-            if scales is None:
-                raise ValueError("AdamW: 8-bit moments need one (scale_m, scale_v) pair per parameter")
-            blocks = [-(-k // BLOCK) for k in numels]
-            at_sm = _check_list("scale_m", [s[0] for s in scales], blocks, torch.float32, dev, spans)
-            at_sv = _check_list("scale_v", [s[1] for s in scales], blocks, torch.float32, dev, spans)
-        elif scales is not None:
+        if state_bits == 8 and scales is None:
+            raise ValueError("AdamW: 8-bit moments need one (scale_m, scale_v) pair per parameter")
+        if state_bits == 32 and scales is not None:
             raise ValueError("AdamW: scales belong to 8-bit moments")
-        _check_disjoint(spans)
-        self.params, self.masters, self.exp_avgs, self.exp_avg_sqs, self.scales = params, masters, m, v, scales
+        self.params, self.masters = tuple(params), None if masters is None else tuple(masters)
+        self.exp_avgs, self.exp_avg_sqs, self.scales = tuple(m), tuple(v), None if scales is None else tuple(tuple(s) for s in scales)
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
         self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
-        self.device = dev
-        # nk_adamw_tensor, word by word: param, grad (filled in by step), exp_avg, exp_avg_sq, master, scales, n
-        self._words = (C.c_int64 * (_TENSOR_WORDS * n))(*[w for row in zip(at_p, none, at_m, at_v, at_w, at_sm, at_sv, numels) for w in row])
-        self._table = C.cast(self._words, C.POINTER(_lib.NkAdamwTensor))
-        self._numels = numels
+        self.device, self._dtype = dev, dt
+        self._numels = [p.numel() for p in params]
+        self._owned = self.params + (self.masters or ())
+        self._held = [t.detach() for t in (*m, *v, *(s for pair in scales or () for s in pair))]       # the table's moments, whatever becomes of `state`
+        self._bind()
         self._opts = _lib.NkAdamwOpts()
         self._opts.param_dtype, self._opts.state_bits = _lib.DTYPES[dt], state_bits
         self._opts.beta1, self._opts.beta2, self._opts.eps = self.betas[0], self.betas[1], self.eps
 
+    def _bind(self) -> None:
+        """Checks every tensor and lays down the launch table."""
+        numels, dev, spans, n = self._numels, self.device, [], len(self.params)
+        none = [0] * n
+        at_p = _check_list("params", self.params, numels, self._dtype, dev, spans)
+        at_w = none if self.masters is None else _check_list("masters", self.masters, numels, torch.float32, dev, spans)
+        dm, dv = MOMENT_DTYPES[self.state_bits]
+        at_m = _check_list("exp_avgs", self._held[:len(self.exp_avgs)], numels, dm, dev, spans)
+        at_v = _check_list("exp_avg_sqs", self._held[len(self.exp_avgs):len(self.exp_avgs) + len(self.exp_avg_sqs)], numels, dv, dev, spans)
+        at_sm = at_sv = none
+        if self.state_bits == 8:
+            blocks = [-(-k // BLOCK) for k in numels]
+            scales = self._held[len(self.exp_avgs) + len(self.exp_avg_sqs):]
+            at_sm = _check_list("scale_m", scales[0::2], blocks, torch.float32, dev, spans)
+            at_sv = _check_list("scale_v", scales[1::2], blocks, torch.float32, dev, spans)
+        _check_disjoint(spans)
+        self._at = at_p + (at_w if self.masters is not None else [])
+        # nk_adamw_tensor, word by word: param, grad (filled in by step), exp_avg, exp_avg_sq, master, scales, n
+        self._words = (C.c_int64 * (_TENSOR_WORDS * n))(*[w for row in zip(at_p, none, at_m, at_v, at_w, at_sm, at_sv, numels) for w in row])
+        self._table = C.cast(self._words, C.POINTER(_lib.NkAdamwTensor))
+
     def step(self, grads: Optional[Sequence[torch.Tensor]] = None, *, lr: Optional[float] = None, step: Optional[int] = None,
              grad_scale: float = 1.0, seed: Optional[int] = None, step_state: Optional[int] = None) -> None:
         """One update.  ``grads``: one contiguous tensor per parameter, all fp32 or all of the parameters' dtype
-        (default: the parameters' ``.grad``, which must exist).  ``step`` (from 1; default: one more than the
+        (default: the parameters' ``.grad``, which must exist); they share no memory with what the step writes.  ``step`` (from 1; default: one more than the
         last) sets the bias corrections, ``seed`` the stochastic rounding of 8-bit moments (default: the
         optimiser's, moved on by the step).  ``step_state``: device address of an ``nk_step_state`` to read the
         step-dependent scalars from when the kernel runs (graph replay)."""
         n = len(self.params)
+        if list(map(_address, self._owned)) != self._at:        # a parameter moved
+            self._bind()
         if grads is None:
             grads = [p.grad for p in self.params]
             if any(g is None for g in grads):
                 raise ValueError("AdamW.step: a parameter has no .grad")
-        if len(grads) != n:
-            raise ValueError(f"grads: {len(grads)} tensors for {n} parameters")
+        if len(grads) != n or not isinstance(grads[0], torch.Tensor):
+            raise ValueError(f"grads: {len(grads)} entries for {n} parameters, one tensor each wanted")
         gd, dev, words, numels = grads[0].dtype, self.device, self._words, self._numels
         if gd != torch.float32 and gd != self.params[0].dtype:
             raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self.params[0].dtype})")
         at = 1
         for g, k in zip(grads, numels):
-            if g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
+            if g is None or g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
                 raise ValueError(f"grads[{at // _TENSOR_WORDS}]: expected {k} contiguous {gd} values on {dev}")
             words[at] = g.data_ptr()
             at += _TENSOR_WORDS
@@ -176,6 +193,7 @@ class AdamW:
         o.state = step_state
         _lib.launch(dev, self._L.nk_adamw_step, self._table, n, o)
         self.steps = step
+        _increment_version(self.params)         # autograd refuses to use what it saved of them before
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],

@@ -253,6 +253,47 @@ def test_default_gradients_streams_and_graph_replay():
         assert all(torch.allclose(a.detach(), b, rtol=2 ** -21, atol=1e-7) for a, b in zip(leaves, copy))
 
 
+@gpu
+def test_parameters_that_move():
+    """A parameter or master whose storage is replaced is updated where it is now; the old storage is left alone."""
+    import nerf_kinematics_amd as nk
+    dev = torch.device("cuda:0")
+    p = [torch.randn(n, device=dev) for n in (300, 5)]
+    low = [t.bfloat16() for t in p]
+    g = [torch.randn_like(t) for t in p]
+    still, stay, moved = [t.clone() for t in p], [t.clone() for t in low], [t.clone() for t in p]
+    a, b = nk.AdamW(stay, 1e-2, masters=still), nk.AdamW(low, 1e-2, masters=moved)
+    a.step(g); b.step(g)
+    old = low[0].data, moved[1].data
+    kept = [t.clone() for t in old]
+    low[0].data, moved[1].data = low[0].data.clone(), moved[1].data.clone()
+    a.step(g); b.step(g)
+    assert all(torch.equal(x, y) for x, y in zip(stay + still, low + moved))
+    assert all(torch.equal(x, y) for x, y in zip(old, kept)) and not torch.equal(old[0], low[0])
+    low[1].data = torch.zeros(6, device=dev, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="elements"):
+        b.step(g)
+    low[1].data = low[0].data[:5]
+    with pytest.raises(ValueError, match="overlap"):
+        b.step(g)
+
+
+@gpu
+def test_autograd_notices_the_step():
+    import nerf_kinematics_amd as nk
+    p = torch.randn(40, device="cuda:0", requires_grad=True)
+    opt = nk.AdamW([p])
+    loss = (p * p).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(ValueError, match="grads"):
+        opt.step([None])
+    with pytest.raises(ValueError, match="grads"):
+        opt.step([p.detach()[::2]])
+
+
 def test_moment_codec_round_trip():
     from nerf_kinematics_amd.optim import decode_moment, encode_moment
     gen = torch.Generator().manual_seed(0)
@@ -296,6 +337,8 @@ def test_refusals_on_the_host():
         bad = nklib.NkAdamwOpts.from_buffer_copy(o)
         setattr(bad, field, value)
         assert L.nk_adamw_step(t, 1, bad, None) == rc, field
+    far = (nklib.NkAdamwTensor * 1)(nklib.NkAdamwTensor(8, 8, 8, 8, 0, 0, 0, 1 << 34))
+    assert L.nk_adamw_step(far, 1, o, None) == -2 and b"too large" in L.nk_last_error()
     t[0].n = -1
     assert L.nk_adamw_step(t, 1, o, None) == -1
     t[0].n = 0
