@@ -688,6 +688,14 @@ ScanArgs args_of(const nk_scan_opts* o, const Shape& s, void* ws) {
 
 int64_t bytes_of(const Shape& s) { return s.sums_bytes + s.part_bytes; }
 
+int check_launch(const nk_scan_opts* o, const Shape& s, const void* workspace, int64_t workspace_bytes, const char* who) {
+    if (((s.cols + (1 << s.LC) - 1) >> s.LC) >= (1 << 24) || (s.parts > 1 && o->B * o->gates > ((int64_t)1 << 31) / o->T))
+        NK_FAIL(NK_ERR_UNSUPPORTED, "%s: more columns than the 2^32 threads of a launch", who);
+    if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
+        NK_FAIL(NK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who, (long long)workspace_bytes, (long long)bytes_of(s));
+    return NK_OK;
+}
+
 }  // namespace
 
 extern "C" int64_t nk_gated_scan_workspace_bytes(const nk_scan_opts* o, int backward) {
@@ -718,8 +726,7 @@ extern "C" int nk_gated_scan_fwd(const nk_scan_opts* o, const void* a, const voi
     if (!a || !x || !h) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_fwd: null pointer");
     Shape s;
     shape_of(o, can_vec(o, a, x, nullptr, h, nullptr, states), 0, &s);
-    if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
-        NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_fwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
+    if ((rc = check_launch(o, s, workspace, workspace_bytes, "nk_gated_scan_fwd")) < 0) return rc;
     ScanArgs A = args_of(o, s, workspace);
     A.a = a; A.x = x; A.first = h0; A.o = h; A.last = h_last; A.states = states;
     return launch_types<false>(o, A, s, nk_stream(stream));
@@ -735,8 +742,7 @@ extern "C" int nk_gated_scan_bwd(const nk_scan_opts* o, const void* a, const voi
     if (!a || (d_a && (!x || !states)) || (!d_a && !d_x && !d_h0)) NK_FAIL(NK_ERR_ARG, "nk_gated_scan_bwd: null pointer");
     Shape s;
     shape_of(o, can_vec(o, a, d_a ? x : nullptr, d_h, d_x, d_a, states), 1, &s);
-    if (bytes_of(s) > workspace_bytes || (bytes_of(s) && (!workspace || ((uintptr_t)workspace & 255))))
-        NK_FAIL(NK_ERR_WORKSPACE, "nk_gated_scan_bwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)workspace_bytes, (long long)bytes_of(s));
+    if ((rc = check_launch(o, s, workspace, workspace_bytes, "nk_gated_scan_bwd")) < 0) return rc;
     ScanArgs A = args_of(o, s, workspace);
     A.a = a; A.x = x; A.g = d_h; A.h0 = h0; A.states = (float*)states; A.first = d_h_last; A.o = d_x; A.d_a = d_a; A.last = d_h0;
     return launch_types<true>(o, A, s, nk_stream(stream));

@@ -300,6 +300,7 @@ def test_refusals_on_the_host():
                     (dict(x_stride_t=-4), -1), (dict(C=1 << 30, gates=1), -2)):
         assert L.nk_gated_scan_workspace_bytes(opts(**bad), 1) == rc, bad
         assert L.nk_gated_scan_fwd(opts(**bad), 8, 8, None, 8, None, None, None, 0, None) == rc, bad
+    assert L.nk_gated_scan_fwd(opts(B=1 << 29, T=1, C=16, gates=16), 8, 8, None, 8, None, None, None, 0, None) == -2     # a launch has 2^32 threads
     long = opts(B=1, T=100000)
     need = L.nk_gated_scan_workspace_bytes(long, 0)
     assert need > 0
