@@ -283,11 +283,12 @@ NK_D float2 join(float2 a, float2 b) {
     return make_float2(mn, a.y * expf(a.x - mz) + b.y * expf(b.x - mz));
 }
 
-// lse and loss of TOK tokens a workgroup: 256 / TOK threads a token take the tiles in turn, then meet in one order
+// lse and loss of TOK tokens a workgroup: 256 / TOK threads a token take the tiles in turn, then meet in one order.
+// sums: NULL, or per workgroup the sum of its losses and how many of its tokens count.
 template <int TOK>
 __global__ __launch_bounds__(256) void k_xent_join(const float2* __restrict__ part, int64_t tiles, int64_t N, int64_t V,
                                                    const int64_t* __restrict__ target, int64_t ignore, const float* __restrict__ zt,
-                                                   float* __restrict__ lse, float* __restrict__ loss) {
+                                                   float* __restrict__ lse, float* __restrict__ loss, double2* __restrict__ sums) {
     __shared__ float2 meet[256];
     constexpr int TH = 256 / TOK;
     const int c = threadIdx.x % TOK, q = threadIdx.x / TOK;
@@ -301,24 +302,29 @@ __global__ __launch_bounds__(256) void k_xent_join(const float2* __restrict__ pa
         if (q < half) meet[q * TOK + c] = join(meet[q * TOK + c], meet[(q + half) * TOK + c]);
         __syncthreads();
     }
+    double total = 0.0, count = 0.0;
     if (q == 0 && n < N) {
         const float l = meet[c].x + logf(meet[c].y);
         const int64_t t = target[n];
+        const float mine = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : l - zt[n];
         lse[n] = l;
-        loss[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : l - zt[n];
+        loss[n] = mine;
+        total = (double)mine; count = t != ignore ? 1.0 : 0.0;
     }
+    if (!sums) return;
+    for (int off = TOK / 2; off > 0; off >>= 1) { total += __shfl_xor(total, off, 64); count += __shfl_xor(count, off, 64); }
+    if (threadIdx.x == 0) sums[blockIdx.x] = make_double2(total, count);
 }
 
 // Sum or mean over the tokens that count, in one order, by one workgroup of 1024 threads.
-NK_D void reduce_losses(double s, int k, int mean, float* out) {
-    __shared__ double sums[16];
-    __shared__ int counts[16];
+NK_D void reduce_losses(double s, double k, int mean, float* out) {
+    __shared__ double sums[16], counts[16];
     for (int off = 32; off > 0; off >>= 1) { s += __shfl_xor(s, off, 64); k += __shfl_xor(k, off, 64); }
     if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = s; counts[threadIdx.x >> 6] = k; }
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) { s += sums[w]; k += counts[w]; }
-        out[0] = (float)(mean ? s / (double)(k > 0 ? k : 1) : s);
+        out[0] = (float)(mean ? s / (k > 0.0 ? k : 1.0) : s);
     }
 }
 
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(1024) void k_xent_join_reduce(const float2* __restr
                                                            float* __restrict__ loss, float* __restrict__ out) {
     const int n = threadIdx.x;
     float l = 0.0f;
-    int k = 0;
+    double k = 0.0;
     if (n < N) {
         float2 r = part[n];
 #pragma unroll 4
@@ -336,18 +342,17 @@ __global__ __launch_bounds__(1024) void k_xent_join_reduce(const float2* __restr
         const float e = r.x + logf(r.y);
         const int64_t t = target[n];
         l = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : e - zt[n];
-        k = t != ignore;
+        k = t != ignore ? 1.0 : 0.0;
         lse[n] = e;
         loss[n] = l;
     }
     reduce_losses((double)l, k, mean, out);
 }
 
-__global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ loss, const int64_t* __restrict__ target, int64_t N,
-                                                      int64_t ignore, int mean, float* __restrict__ out) {
-    double s = 0.0;
-    int k = 0;                  // N is at most 2^24
-    for (int64_t n = threadIdx.x; n < N; n += 1024) { s += (double)loss[n]; k += target[n] != ignore; }
+__global__ __launch_bounds__(1024) void k_xent_reduce(const double2* __restrict__ sums, int64_t n, int mean, float* __restrict__ out) {
+    double s = 0.0, k = 0.0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += 1024) { s += sums[i].x; k += sums[i].y; }
     reduce_losses(s, k, mean, out);
 }
 
@@ -355,34 +360,64 @@ __global__ __launch_bounds__(1024) void k_xent_reduce(const float* __restrict__ 
 // Row factors of dz and the factor that is left for the end: the products see dz with |c| <= 1.
 //   mean / sum: c = 1 for tokens that count, rest = d_loss / count or d_loss
 //   none:       c = d_loss_n / rest with rest the power of two above the largest |d_loss|
-__global__ __launch_bounds__(1024) void k_xent_factors(const int64_t* __restrict__ target, int64_t N, int64_t V, int64_t ignore, int reduction,
-                                                       const float* __restrict__ d_loss, float* __restrict__ c, float* __restrict__ rest) {
-    __shared__ int64_t counts[16];
-    __shared__ uint32_t peaks[16];
-    __shared__ float unit;
-    int64_t k = 0;
-    uint32_t peak = 0;
-    for (int64_t n = threadIdx.x; n < N; n += 1024) {
-        const bool on = target[n] != ignore;
-        k += on;
-        if (reduction == NK_REDUCE_NONE && on) peak = max(peak, __float_as_uint(d_loss[n]) & 0x7FFFFFFFu);
-    }
-    for (int off = 32; off > 0; off >>= 1) { k += __shfl_xor((int)k, off, 64); peak = max(peak, (uint32_t)__shfl_xor((int)peak, off, 64)); }
-    if ((threadIdx.x & 63) == 0) { counts[threadIdx.x >> 6] = k; peaks[threadIdx.x >> 6] = peak; }
+struct Tally { int count; uint32_t peak; };     // tokens that count, bits of the largest |d_loss| among them
+enum { TALLY_TOKENS = 4096 };
+
+NK_D Tally tally(const int64_t* target, int64_t n0, int64_t n1, int64_t ignore, int reduction, const float* d_loss) {
+    Tally r = {0, 0};
+#pragma unroll 4
+    for (int64_t n = n0 + threadIdx.x; n < n1; n += 1024)
+        if (target[n] != ignore) {
+            ++r.count;
+            if (reduction == NK_REDUCE_NONE) r.peak = max(r.peak, __float_as_uint(d_loss[n]) & 0x7FFFFFFFu);
+        }
+    return r;
+}
+// over the workgroup of 1024 threads; the result is in thread 0
+NK_D Tally meet_tally(Tally r) {
+    __shared__ Tally meet[16];
+    for (int off = 32; off > 0; off >>= 1) { r.count += __shfl_xor(r.count, off, 64); r.peak = max(r.peak, (uint32_t)__shfl_xor((int)r.peak, off, 64)); }
+    if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = r;
     __syncthreads();
+    if (threadIdx.x == 0) for (int w = 1; w < 16; ++w) { r.count += meet[w].count; r.peak = max(r.peak, meet[w].peak); }
+    return r;
+}
+
+// Where one workgroup would take long over the tokens, TALLY_TOKENS of them a workgroup first; k_xent_factors then
+// adds these up in every workgroup, each of which writes the factors of as many tokens.  196 608 tokens: 10 us instead of 66.
+__global__ __launch_bounds__(1024) void k_xent_tally(const int64_t* __restrict__ target, int64_t N, int64_t ignore, int reduction,
+                                                     const float* __restrict__ d_loss, Tally* __restrict__ out) {
+    const int64_t n0 = (int64_t)blockIdx.x * TALLY_TOKENS, n1 = n0 + TALLY_TOKENS < N ? n0 + TALLY_TOKENS : N;
+    const Tally r = meet_tally(tally(target, n0, n1, ignore, reduction, d_loss));
+    if (threadIdx.x == 0) out[blockIdx.x] = r;
+}
+
+__global__ __launch_bounds__(1024) void k_xent_factors(const int64_t* __restrict__ target, int64_t N, int64_t V, int64_t ignore, int reduction,
+                                                       const float* __restrict__ d_loss, const Tally* __restrict__ parts, int n_parts,
+                                                       float* __restrict__ c, float* __restrict__ rest) {
+    __shared__ float unit;
+    Tally r = {0, 0};
+    if (parts) {
+        for (int i = threadIdx.x; i < n_parts; i += 1024) { r.count += parts[i].count; r.peak = max(r.peak, parts[i].peak); }
+    } else {
+        r = tally(target, 0, N, ignore, reduction, d_loss);
+    }
+    r = meet_tally(r);
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) { k += counts[w]; peak = max(peak, peaks[w]); }
+        float left;
         if (reduction == NK_REDUCE_NONE) {
-            const int e = min(max((int)(peak >> 23) + 1, 27), 227);          // 2^-100 .. 2^100; infinities and NaN stay in c
+            const int e = min(max((int)(r.peak >> 23) + 1, 27), 227);          // 2^-100 .. 2^100; infinities and NaN stay in c
             unit = __uint_as_float((uint32_t)(254 - e) << 23);
-            *rest = __uint_as_float((uint32_t)e << 23);
+            left = __uint_as_float((uint32_t)e << 23);
         } else {
             unit = 1.0f;
-            *rest = reduction == NK_REDUCE_MEAN ? d_loss[0] / (float)(k > 0 ? k : 1) : d_loss[0];
+            left = reduction == NK_REDUCE_MEAN ? d_loss[0] / (float)(r.count > 0 ? r.count : 1) : d_loss[0];
         }
+        if (blockIdx.x == 0) *rest = left;
     }
     __syncthreads();
-    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+#pragma unroll 4
+    for (int64_t n = (int64_t)blockIdx.x * 1024 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 1024) {
         const int64_t t = target[n];
         c[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : reduction == NK_REDUCE_NONE ? d_loss[n] * unit : 1.0f;
     }
@@ -567,18 +602,27 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g
     }
 }
 
-// d_hidden from its fp32 sums, the slices in one order; tokens that do not count have none.  VEC elements a thread.
+// A grid over many elements: the launch holds fewer than 2^32 threads along x.
+inline dim3 flat_grid(int64_t blocks) {
+    const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+NK_D int64_t flat_block() { return blockIdx.x + (int64_t)blockIdx.y * gridDim.x; }
+
+// out [N][D] from its fp32 sums, the slices in one order.  c: NULL, or rows with c = 0 (tokens that do not count) are
+// zero.  VEC elements a thread.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ sums, int slices, int64_t N, int64_t D, const float* __restrict__ c,
                                                      const float* __restrict__ rest, float scale, T* __restrict__ out) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+    const int64_t i = (flat_block() * 256 + threadIdx.x) * VEC;
     if (i >= N * D) return;
     typedef __attribute__((ext_vector_type(VEC))) float fvec;
     typedef __attribute__((ext_vector_type(VEC))) T tvec;
     fvec s = *(const fvec*)(sums + i);
+#pragma unroll 8
     for (int k = 1; k < slices; ++k) s += *(const fvec*)(sums + (int64_t)k * N * D + i);
     const float f = *rest * scale;
-    const bool on = c[i / D] != 0.0f;
+    const bool on = !c || c[i / D] != 0.0f;
     tvec w;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) w[e] = (T)(on ? s[e] * f : 0.0f);
@@ -588,7 +632,7 @@ __global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ s
 // dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, T* __restrict__ dst, int64_t dst_ld) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = flat_block() * 256 + threadIdx.x;
     if (i >= rows * dst_ld) return;
     const int64_t r = i / dst_ld, c = i - r * dst_ld;
     dst[i] = c < cols ? src[r * ld + c] : (T)0.0f;
@@ -646,7 +690,7 @@ inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
 
 template <auto K, typename ARGS>
 int start(const ARGS& args, int64_t blocks, int slices, int threads, hipStream_t st, const char* name) {
-    if (blocks > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+    if (blocks * threads > 0xFFFFFFFFll) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: too many tiles", name);
     hipLaunchKernelGGL(K, dim3((unsigned)blocks, (unsigned)slices), dim3(threads), 0, st, args);
     NK_CHECK_LAUNCH(name);
     return NK_OK;
@@ -661,11 +705,26 @@ int tile_kind(int64_t M, int64_t N, int64_t slices = 1) {
 }
 int kind_bm(int kind) { return kind == LARGE ? 256 : kind == SMALL ? 64 : 128; }
 
+// Into how many stretches the k of an M x N product is cut where it has too few tiles to fill the chip: large tiles if
+// the stretches stay long, otherwise small ones of eight steps at least.  64 at most: their fp32 sums are read
+// once more.  d_weight of 196 608 tokens x 64 with 16 labels in bf16: 667 us whole, 21 us cut into 64; 65 536 x 256
+// with 150 labels in fp32: 1 165 and 83 us.
+int64_t cut_of(int64_t M, int64_t N, int64_t k, int64_t step) {
+    const int64_t large = cdiv(M, 256) * cdiv(N, 256), tiles = cdiv(M, N <= 32 ? 128 : 64) * cdiv(N, N <= 32 ? 32 : 64);
+    int64_t cut = 1;
+    if (N > 32 && large < 224 && k / cdiv(256, large) >= 2048) cut = cdiv(256, large);
+    else if (large < 224 && tiles < 256) cut = cdiv(512, tiles);
+    const int64_t most = k / (8 * step);
+    if (cut > most) cut = most;
+    if (cut > 64) cut = 64;
+    return cut < 1 ? 1 : cut;
+}
+
 struct Plan {
     int64_t Dp, Np, piece;                  // padded k of the logits' product; tokens padded to a step; vocabulary rows per piece
     bool pad_h, pad_w;
     int kind, slices;
-    int64_t parts, zt, h, w, c, rest, wt, ht, dz, dzt, sums, total;
+    int64_t parts, zt, losses, h, w, c, rest, tally, wt, ht, dz, dzt, sums, wsums, total;
 };
 
 int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int backward, Plan* p, const char* who) {
@@ -692,7 +751,7 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
     } else {
         piece = p->pad_w ? (asked ? asked : 16384) : up(o->V, 256);
     }
-    if (piece > up(o->V, 256)) piece = up(o->V, 256);
+    if (piece > o->V) piece = up(o->V, step);           // the only one
     p->piece = piece;
     int64_t off = 0;
     auto take = [&](int64_t bytes) { const int64_t at = off; off = up(off + bytes, 1024); return at; };
@@ -701,25 +760,26 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
     p->kind = tile_kind(piece < o->V ? piece : o->V, o->N);
     p->slices = 1;
     if (!backward) {
-        p->parts = take(cdiv(o->V, piece) * (piece / kind_bm(p->kind)) * o->N * 8);
+        p->parts = take(cdiv(o->V, piece) * cdiv(piece, kind_bm(p->kind)) * o->N * 8);
         p->zt = take(o->N * 4);
+        p->losses = take(cdiv(o->N, o->N <= 1024 ? 1 : 16) * sizeof(double2));
     } else {
         p->c = take(o->N * 4);
         p->rest = take(4);
+        p->tally = take(cdiv(o->N, TALLY_TOKENS) * sizeof(Tally));
         p->wt = take(o->D * piece * es);
         p->ht = take(o->D * p->Np * es);
         p->dz = take(o->N * piece * es);
         p->dzt = take(piece * p->Np * es);
-        // d_hidden has few tiles: cut its k (the piece) until they fill the chip, in large tiles if the stretches stay long
-        const int64_t large = cdiv(o->D, 256) * cdiv(o->N, 256), tiles = cdiv(o->D, 64) * cdiv(o->N, o->N <= 32 ? 32 : 64);
-        int64_t cut = 1;
-        if (o->N > 32 && large > 0 && large < 224 && piece / cdiv(256, large) >= 2048) cut = cdiv(256, large);
-        else if (large < 224 && tiles > 0 && tiles < 256) cut = cdiv(512, tiles);
-        const int64_t most = piece / (8 * step);
-        if (cut > most) cut = most;
-        if (cut > 16) cut = 16;
-        p->slices = (int)(cut < 1 ? 1 : cut);
+        p->slices = o->N > 0 ? (int)cut_of(o->D, o->N, piece, step) : 1;
         p->sums = take(p->slices == 1 && piece >= o->V ? 0 : (int64_t)p->slices * o->N * o->D * 4);
+        // d_weight of a whole piece, and of the last one
+        int64_t most = 0;
+        for (const int64_t rows : {piece < o->V ? piece : o->V, (o->V - 1) % piece + 1}) {
+            const int64_t cut = cut_of(o->D, rows, p->Np, step);
+            if (cut > 1 && cut * rows > most) most = cut * rows;
+        }
+        p->wsums = take(most * o->D * 4);
     }
     p->total = off;
     return NK_OK;
@@ -751,8 +811,7 @@ template <typename T, bool SUMS> int product_launch(const ProductArgs& g, int sl
 
 template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t dst_ld, hipStream_t st) {
     const int64_t n = rows * dst_ld;
-    if (cdiv(n, 256) > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "k_xent_pad: too large");
-    hipLaunchKernelGGL(k_xent_pad<T>, dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, (const T*)src, ld, rows, cols, (T*)dst, dst_ld);
+    hipLaunchKernelGGL(k_xent_pad<T>, flat_grid(cdiv(n, 256)), dim3(256), 0, st, (const T*)src, ld, rows, cols, (T*)dst, dst_ld);
     NK_CHECK_LAUNCH("k_xent_pad");
     return NK_OK;
 }
@@ -763,6 +822,16 @@ template <typename T> int transpose(const void* src, int64_t ld, int64_t rows, i
     else
         hipLaunchKernelGGL((k_xent_transpose<T, false>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
     NK_CHECK_LAUNCH("k_xent_transpose");
+    return NK_OK;
+}
+
+template <typename T>
+int finish(const float* sums, int slices, int64_t rows, int64_t D, const float* c, const float* rest, float scale, void* out, hipStream_t st) {
+    if (D % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0)
+        hipLaunchKernelGGL((k_xent_finish<T, 4>), flat_grid(cdiv(rows * D, 1024)), dim3(256), 0, st, sums, slices, rows, D, c, rest, scale, (T*)out);
+    else
+        hipLaunchKernelGGL((k_xent_finish<T, 1>), flat_grid(cdiv(rows * D, 256)), dim3(256), 0, st, sums, slices, rows, D, c, rest, scale, (T*)out);
+    NK_CHECK_LAUNCH("k_xent_finish");
     return NK_OK;
 }
 
@@ -795,16 +864,17 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
         NK_CHECK_LAUNCH("k_xent_join_reduce");
         return NK_OK;
     }
+    double2* losses = o->reduction != NK_REDUCE_NONE ? (double2*)(ws + p.losses) : nullptr;
     // few tokens: all threads of a workgroup on one of them
     if (o->N <= 1024)
         hipLaunchKernelGGL(k_xent_join<1>, dim3((unsigned)o->N), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V, target,
-                           o->ignore_index, (const float*)(ws + p.zt), lse, loss);
+                           o->ignore_index, (const float*)(ws + p.zt), lse, loss, losses);
     else
         hipLaunchKernelGGL(k_xent_join<16>, dim3((unsigned)cdiv(o->N, 16)), dim3(256), 0, st, (const float2*)(ws + p.parts), tiles, o->N, o->V,
-                           target, o->ignore_index, (const float*)(ws + p.zt), lse, loss);
+                           target, o->ignore_index, (const float*)(ws + p.zt), lse, loss, losses);
     NK_CHECK_LAUNCH("k_xent_join");
     if (o->reduction != NK_REDUCE_NONE) {
-        hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, loss, target, o->N, o->ignore_index, o->reduction == NK_REDUCE_MEAN, reduced);
+        hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, losses, cdiv(o->N, o->N <= 1024 ? 1 : 16), o->reduction == NK_REDUCE_MEAN, reduced);
         NK_CHECK_LAUNCH("k_xent_reduce");
     }
     return NK_OK;
@@ -818,7 +888,14 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
     float* c = (float*)(ws + p.c);
     float* rest = (float*)(ws + p.rest);
     int rc;
-    hipLaunchKernelGGL(k_xent_factors, dim3(1), dim3(1024), 0, st, target, o->N, o->V, o->ignore_index, o->reduction, d_loss, c, rest);
+    const int groups = (int)cdiv(o->N, TALLY_TOKENS);
+    Tally* parts = groups > 2 ? (Tally*)(ws + p.tally) : nullptr;       // up to two: less than another launch
+    if (parts) {
+        hipLaunchKernelGGL(k_xent_tally, dim3(groups), dim3(1024), 0, st, target, o->N, o->ignore_index, o->reduction, d_loss, parts);
+        NK_CHECK_LAUNCH("k_xent_tally");
+    }
+    hipLaunchKernelGGL(k_xent_factors, dim3(parts ? groups : 1), dim3(1024), 0, st, target, o->N, o->V, o->ignore_index, o->reduction, d_loss, parts,
+                       groups, c, rest);
     NK_CHECK_LAUNCH("k_xent_factors");
     Mat h = {(const char*)hidden, o->N, o->hidden_stride * es};
     if (p.pad_h) {
@@ -843,8 +920,16 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
             ProductArgs q = {};
             q.a = Mat{ws + p.ht, o->D, p.Np * es}; q.b = Mat{ws + p.dzt, rows, p.Np * es};
             q.kbytes = q.kslice = p.Np * es; q.M = o->D; q.N = rows;
-            q.out = (char*)d_weight + v0 * o->D * es; q.ld = o->D; q.rest = rest; q.scale = unscale;
-            if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+            char* out = (char*)d_weight + v0 * o->D * es;
+            const int cut = (int)cut_of(o->D, rows, p.Np, 128 / es);
+            if (cut == 1) {
+                q.out = out; q.ld = o->D; q.rest = rest; q.scale = unscale;
+                if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+            } else {
+                q.kslice = up(cdiv(p.Np, cut), 128 / es) * es; q.sums = (float*)(ws + p.wsums);
+                if ((rc = product_launch<T, true>(q, cut, st)) < 0) return rc;
+                if ((rc = finish<T>(q.sums, cut, rows, o->D, nullptr, rest, unscale, out, st)) < 0) return rc;
+            }
         }
         if (d_hidden) {
             if ((rc = transpose<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.wt, kv, st)) < 0) return rc;
@@ -860,16 +945,7 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
             }
         }
     }
-    if (d_hidden && !direct) {
-        const bool four = o->D % 4 == 0 && ((uintptr_t)d_hidden & (4 * es - 1)) == 0;
-        const int64_t blocks = cdiv(o->N * o->D, four ? 1024 : 256);
-        if (blocks > 0x7FFFFFFF) NK_FAIL(NK_ERR_UNSUPPORTED, "nk_linear_xent_bwd: too large");
-        if (four) hipLaunchKernelGGL((k_xent_finish<T, 4>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c,
-                                     rest, unscale, (T*)d_hidden);
-        else hipLaunchKernelGGL((k_xent_finish<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)(ws + p.sums), p.slices, o->N, o->D, c,
-                                rest, unscale, (T*)d_hidden);
-        NK_CHECK_LAUNCH("k_xent_finish");
-    }
+    if (d_hidden && !direct && (rc = finish<T>((const float*)(ws + p.sums), p.slices, o->N, o->D, c, rest, unscale, d_hidden, st)) < 0) return rc;
     return NK_OK;
 }
 
@@ -898,7 +974,7 @@ extern "C" int nk_linear_xent_fwd(const nk_xent_opts* o, const void* hidden, con
     const hipStream_t st = nk_stream(stream);
     if (o->N == 0) {
         if (o->reduction != NK_REDUCE_NONE) {
-            hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, loss, target, (int64_t)0, o->ignore_index, 0, reduced);
+            hipLaunchKernelGGL(k_xent_reduce, dim3(1), dim3(1024), 0, st, (const double2*)nullptr, (int64_t)0, 0, reduced);
             NK_CHECK_LAUNCH("k_xent_reduce");
         }
         return NK_OK;

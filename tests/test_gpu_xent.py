@@ -95,6 +95,16 @@ def test_large_tiles(shape):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", [(20000, 64, 16), (9001, 50, 150), (16385, 24, 2), (8193, 33, 65)], ids=lambda s: "x".join(map(str, s)))
+def test_many_tokens_few_labels(shape, dt):
+    """d_weight's long sum is cut into stretches, and the tokens are counted by many workgroups."""
+    h, w, t, g = make(*shape, dt, 14)
+    check(h, w, t, "none" if shape[1] == 64 else "mean", g)
+    check(h, w, t, "sum", g, piece=256)
+
+
+@gpu
 @pytest.mark.parametrize("piece", [1, 256, 300, 512, 5000])
 @pytest.mark.parametrize("D", [64, 50])
 def test_pieces(piece, D):
