@@ -57,16 +57,6 @@ template <typename T> NK_D void store(T* p, const float* o, bool whole, int live
     for (int k = 0; k < 4; ++k) if (k < live) p[k] = (T)o[k];
 }
 
-// Largest of a non-negative integer over the wavefront, as a scalar: rows of 16 by row shifts, then the rows
-// onto each other (lanes without a source take 0).
-NK_D uint32_t wave_max(uint32_t v) {
-#define NK_MAX_STEP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false))
-    NK_MAX_STEP(0x111); NK_MAX_STEP(0x112); NK_MAX_STEP(0x114); NK_MAX_STEP(0x118);     // row_shr 1, 2, 4, 8
-    NK_MAX_STEP(0x142); NK_MAX_STEP(0x143);                                             // row_bcast 15, 31
-#undef NK_MAX_STEP
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
 // Square root to one unit in the last place (v_sqrt_f32), values whose low bits it would drop scaled up first.  The
 // step with 8-bit moments is bound by the vector unit, not by memory: this and the factor 1 / sqrt(1 - b2^t)
 // in place of a division take about a fifth of its instructions away.
@@ -165,7 +155,7 @@ __global__ __launch_bounds__(AW_THREADS) void k_adamw(const AwArgs A) {
             bm = max(bm, __float_as_uint(m[k]) & 0x7FFFFFFFu);
             bv = max(bv, __float_as_uint(v[k]) & 0x7FFFFFFFu);
         }
-        bm = wave_max(bm); bv = wave_max(bv);
+        bm = nk_wave_max(bm); bv = nk_wave_max(bv);
         const int em = scale_exp(bm, 8), ev = scale_exp(bv, 15);
         const float im = __uint_as_float((uint32_t)(127 - em) << 23), iv = __uint_as_float((uint32_t)(127 - ev) << 23);
         uint32_t cm = 0, cv = 0;

@@ -27,6 +27,16 @@ void nk_set_error(const char* fmt, ...);
 #define NK_CHECK_LAUNCH(name) do { hipError_t e_ = hipGetLastError(); if (e_ != hipSuccess) { \
     nk_set_error("launch of %s failed: %s", name, hipGetErrorString(e_)); return NK_ERR_HIP; } } while (0)
 
+// Largest of a non-negative integer over the wavefront, as a scalar: rows of 16 by row shifts, then the rows
+// onto each other (lanes without a source take 0).
+NK_D uint32_t nk_wave_max(uint32_t v) {
+#define NK_MAX_STEP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false))
+    NK_MAX_STEP(0x111); NK_MAX_STEP(0x112); NK_MAX_STEP(0x114); NK_MAX_STEP(0x118);     // row_shr 1, 2, 4, 8
+    NK_MAX_STEP(0x142); NK_MAX_STEP(0x143);                                             // row_bcast 15, 31
+#undef NK_MAX_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // ---- counter-based RNG: 32 bits for element idx of a stream under a seed --------------------
 enum { NK_STREAM_STRATIFIED = 0, NK_STREAM_PDF = 1, NK_STREAM_NOISE_COARSE = 2,
        NK_STREAM_NOISE_FINE = 3, NK_STREAM_PIXELS = 4, NK_STREAM_OPTIMISER = 5 };

@@ -24,10 +24,13 @@
 //   215 us forward + backward for 4096 ragged sequences x 192 x 64 in bf16 with one fp32 gate a step, 312 against
 //   389 us for 2 x 32768 x 1024; one channel a thread: 146 and 403 us.
 //   8 steps a run against 4: 123 / 146 us and 312 / 375 us.
+//   Short sequences pay for what happens once a workgroup: the longest length by lane shifts and not by an LDS
+//   atomic, and rows walked by pointer (multiples of five strides no longer fill the scalar registers), took
+//   4096 x 192 x 64 from 123 to 98 us (31 forward, 67 backward; its bytes cost 75).
 //   Loading the next tile ahead in the backward pass costs registers and loses (280 against 164 us); in the
 //   forward pass it gains.
 // 2 x 32768 x 1024 in bf16 then takes 124 us forward (53 of them the first launch, 5.1 TB/s; the walk
-// moves 5.6 TB/s with the first launch's reads partly cached) and 186 us backward, against 169 us that the bytes of
+// moves 5.6 TB/s with the first launch's reads partly cached) and 184 us backward, against 169 us that the bytes of
 // one pass over every tensor cost; reading a and x (a and g) twice is what is left.
 #include "nk_common.h"
 
@@ -105,18 +108,19 @@ template <int VC, bool SHARED> NK_D Place place(const ScanArgs& A) {
     return p;
 }
 
-// Steps s0 .. s0 + SC_U - 1 of a column; `fill` where s reaches `lim`.  base: the row of step s0.
+// Steps s0 .. s0 + SC_U - 1 of a column; `fill` where s reaches `lim`.  base: the row of step s0.  whole: no lane
+// of the wavefront reaches it.
 template <typename T, int VC>
-NK_D void fetch(Pack<T, VC> (&r)[SC_U], const T* base, int64_t step, int s0, int lim, float fill) {
-    if (__all(s0 + SC_U <= lim)) {
+NK_D void fetch(Pack<T, VC> (&r)[SC_U], const T* base, int64_t step, int s0, int lim, float fill, bool whole) {
+    if (whole) {
 #pragma unroll
-        for (int u = 0; u < SC_U; ++u) r[u] = ld<T, VC>(base + u * step);
+        for (int u = 0; u < SC_U; ++u, base += step) r[u] = ld<T, VC>(base);
     } else {
 #pragma unroll
-        for (int u = 0; u < SC_U; ++u) {
+        for (int u = 0; u < SC_U; ++u, base += step) {
 #pragma unroll
             for (int v = 0; v < VC; ++v) r[u].v[v] = (T)fill;
-            if (s0 + u < lim) r[u] = ld<T, VC>(base + u * step);
+            if (s0 + u < lim) r[u] = ld<T, VC>(base);
         }
     }
 }
@@ -126,12 +130,14 @@ NK_D int64_t time_of(int s, int len, int reverse) { return reverse ? len - 1 - s
 // Largest live length of the workgroup's columns.
 NK_D int longest(const Place& p, const ScanArgs& A) {
     if (!A.lengths) return A.T;
-    __shared__ int most;
-    if (threadIdx.x == 0) most = 0;
+    __shared__ int most[SC_THREADS / 64];
+    const int mine = (int)nk_wave_max((uint32_t)p.len);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = mine;
     __syncthreads();
-    if (p.len > 0) atomicMax(&most, p.len);
-    __syncthreads();
-    return most;
+    int m = most[0];
+#pragma unroll
+    for (int w = 1; w < SC_THREADS / 64; ++w) m = max(m, most[w]);
+    return m;
 }
 
 template <int VC> struct Buf { float v[4][3 * VC][64]; };
@@ -289,8 +295,9 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_sum(const ScanArgs A) {
         const int64_t t0 = time_of(s0, p.len, A.reverse);
         Pack<GT, GV> ra[SC_U];
         Pack<T, VC> rx[SC_U];
-        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, hi, 1.0f);
-        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, A.x ? hi : SC_NONE, 0.0f);
+        const bool whole = __all(s0 + SC_U <= hi);
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, hi, 1.0f, whole);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, A.x ? hi : SC_NONE, 0.0f, whole && A.x);
 #pragma unroll
         for (int w = 0; w < SC_U; ++w) {
             const int u = BWD ? SC_U - 1 - w : w;
@@ -342,20 +349,22 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
     Pack<GT, GV> ra[SC_U];
     Pack<T, VC> rx[SC_U];
     int s0 = begin + p.run * SC_U;
+    bool whole = __all(s0 + SC_U <= lim);
     {
         const int64_t t0 = time_of(s0, p.len, A.reverse);
-        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
-        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, lim, 0.0f);
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f, whole);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, lim, 0.0f, whole);
     }
     int flip = 0, at = begin;
     for (; at < stop; at += tile, s0 += tile, flip ^= 1) {
         Pack<GT, GV> na[SC_U];
         Pack<T, VC> nx[SC_U];
+        const bool next = __all(s0 + tile + SC_U <= lim);
         {       // the next tile's loads are in flight while this one is composed and written
             const int s1 = s0 + tile;
             const int64_t t1 = time_of(s1, p.len, A.reverse);
-            fetch<GT, GV>(na, ab + t1 * A.a_st, as, s1, lim, 1.0f);
-            fetch<T, VC>(nx, xb + t1 * A.x_st, xs, s1, lim, 0.0f);
+            fetch<GT, GV>(na, ab + t1 * A.a_st, as, s1, lim, 1.0f, next);
+            fetch<T, VC>(nx, xb + t1 * A.x_st, xs, s1, lim, 0.0f, next);
         }
         float Ar[VC], Hr[VC];
 #pragma unroll
@@ -371,19 +380,25 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_fwd(const ScanArgs A) {
         compose_up<VC>(Ar, Hr, carry, s, A.LC, buf[flip]);
         if (A.states && (s0 & (SC_KEEP - 1)) == 0 && s0 < lim) st<float, VC>(A.states + ((int64_t)p.b * kept + s0 / SC_KEEP) * A.C + p.c, s);
         T* o = ob + time_of(s0, p.len, A.reverse) * A.C;
-        const bool whole = __all(s0 + SC_U <= lim);
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < SC_U; ++u) {
+            for (int u = 0; u < SC_U; ++u, o += os) {
 #pragma unroll
-            for (int v = 0; v < VC; ++v) s[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], s[v], (float)rx[u].v[v]);
-            if (whole || s0 + u < lim) st<T, VC>(o + u * os, s);
-            else if (p.on && s0 + u < end) {
-                float z[VC];
+                for (int v = 0; v < VC; ++v) s[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], s[v], (float)rx[u].v[v]);
+                st<T, VC>(o, s);
+            }
+        } else {
+            T* behind = ob + (int64_t)s0 * A.C;         // rows behind the sequence: zeros, in place
 #pragma unroll
-                for (int v = 0; v < VC; ++v) z[v] = 0.0f;
-                st<T, VC>(ob + (int64_t)(s0 + u) * A.C, z);
+            for (int u = 0; u < SC_U; ++u, o += os, behind += A.C) {
+                float w[VC];
+                const bool live = s0 + u < lim;
+#pragma unroll
+                for (int v = 0; v < VC; ++v) { s[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], s[v], (float)rx[u].v[v]); w[v] = live ? s[v] : 0.0f; }
+                if (live || (p.on && s0 + u < end)) st<T, VC>(live ? o : behind, w);
             }
         }
+        whole = next;
 #pragma unroll
         for (int u = 0; u < SC_U; ++u) { ra[u] = na[u]; rx[u] = nx[u]; }
     }
@@ -430,7 +445,7 @@ NK_D void gate_sums(float (&v)[SC_U], int wide, int k, int* u0, int* n, bool* mi
 }
 
 template <typename T, typename GT, int VC, bool SHARED>
-__global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
+__global__ __launch_bounds__(SC_THREADS, 4) void k_scan_bwd(const ScanArgs A) {
     __shared__ Buf<VC> buf[2];
     constexpr int GV = SHARED ? 1 : VC;
     const Place p = place<VC, SHARED>(A);
@@ -478,19 +493,18 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
         Pack<GT, GV> ra[SC_U];
         Pack<T, VC> rx[SC_U], rg[SC_U];
         float hs[VC], h[VC], e[VC];
-        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f);
-        fetch<T, VC>(rg, gb + t0 * A.g_st, gs, s0, A.g ? lim : SC_NONE, 0.0f);
-        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, gates ? lim : SC_NONE, 0.0f);
+        const bool whole = __all(s0 + SC_U <= lim);
+        float Ar[VC], Hr[VC], Er[VC];
 #pragma unroll
-        for (int v = 0; v < VC; ++v) hs[v] = 0.0f;
+        for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = Er[v] = hs[v] = 0.0f; }
+        fetch<GT, GV>(ra, ab + t0 * A.a_st, as, s0, lim, 1.0f, whole);
+        fetch<T, VC>(rg, gb + t0 * A.g_st, gs, s0, A.g ? lim : SC_NONE, 0.0f, whole && A.g);
+        fetch<T, VC>(rx, xb + t0 * A.x_st, xs, s0, gates ? lim : SC_NONE, 0.0f, whole && gates);
         if (gates && at < lim) {            // the state in front of the tile
             const float* from = at == 0 ? (A.h0 ? A.h0 + p.b * A.C + p.c : nullptr)
                                         : A.states + ((int64_t)p.b * kept + at / SC_KEEP) * A.C + p.c;
             if (from) for (int v = 0; v < VC; ++v) hs[v] = from[v];
         }
-        float Ar[VC], Hr[VC], Er[VC];
-#pragma unroll
-        for (int v = 0; v < VC; ++v) { Ar[v] = 1.0f; Hr[v] = Er[v] = 0.0f; }
 #pragma unroll
         for (int u = 0; u < SC_U; ++u)
 #pragma unroll
@@ -504,33 +518,49 @@ __global__ __launch_bounds__(SC_THREADS) void k_scan_bwd(const ScanArgs A) {
 #pragma unroll
             for (int v = 0; v < VC; ++v) Er[v] = (float)ra[u].v[SHARED ? 0 : v] * ((float)rg[u].v[v] + Er[v]);
         compose_both<VC>(Ar, Hr, Er, hs, carry, h, e, A.LC, buf[flip]);
-        float prev[SC_U][VC], sum[SC_U];
+        float prev[SC_U][VC], d[SC_U][VC], sum[SC_U];
 #pragma unroll
         for (int u = 0; u < SC_U; ++u)
 #pragma unroll
             for (int v = 0; v < VC; ++v) { prev[u][v] = h[v]; h[v] = fmaf((float)ra[u].v[SHARED ? 0 : v], h[v], (float)rx[u].v[v]); }
-        const bool whole = __all(s0 + SC_U <= lim);
-        T* o = ob + t0 * A.C;
-        const int64_t os = A.reverse ? -A.C : A.C, ds = A.reverse ? -drow : drow;
 #pragma unroll
         for (int u = SC_U - 1; u >= 0; --u) {
-            float d[VC], dg[VC];
-            const bool live = whole || s0 + u < lim;
             sum[u] = 0.0f;
 #pragma unroll
             for (int v = 0; v < VC; ++v) {
-                d[v] = (float)rg[u].v[v] + e[v];
-                e[v] = (float)ra[u].v[SHARED ? 0 : v] * d[v];
-                if (!live) d[v] = 0.0f;
-                dg[v] = live ? d[v] * prev[u][v] : 0.0f;
-                sum[u] += dg[v];
+                d[u][v] = (float)rg[u].v[v] + e[v];
+                e[v] = (float)ra[u].v[SHARED ? 0 : v] * d[u][v];
+                prev[u][v] *= d[u][v];              // dL/da of the channel
+                sum[u] += prev[u][v];
             }
-            if (live) {
-                if (A.o) st<T, VC>(o + u * os, d);
-                if (!SHARED && gates) st<GT, VC>(db + t0 * drow + u * ds, dg);
-            } else if (p.on && s0 + u < end) {      // behind the sequence: zeros, in place
-                if (A.o) st<T, VC>(ob + (int64_t)(s0 + u) * A.C, d);
-                if (!SHARED && gates) st<GT, VC>(db + (int64_t)(s0 + u) * drow, dg);
+        }
+        const int64_t os = A.reverse ? -A.C : A.C, ds = A.reverse ? -drow : drow;
+        if (whole) {
+            if (A.o) {
+                T* o = ob + t0 * A.C;
+#pragma unroll
+                for (int u = 0; u < SC_U; ++u, o += os) st<T, VC>(o, d[u]);
+            }
+            if (!SHARED && gates) {
+                GT* o = db + t0 * drow;
+#pragma unroll
+                for (int u = 0; u < SC_U; ++u, o += ds) st<GT, VC>(o, prev[u]);
+            }
+        } else {
+            int64_t row = t0;
+#pragma unroll
+            for (int u = 0; u < SC_U; ++u, row += A.reverse ? -1 : 1) {
+                const bool live = s0 + u < lim;
+                if (!live) {
+                    sum[u] = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < VC; ++v) d[u][v] = prev[u][v] = 0.0f;
+                }
+                if (live || (p.on && s0 + u < end)) {
+                    const int64_t at_row = live ? row : s0 + u;         // behind the sequence: zeros, in place
+                    if (A.o) st<T, VC>(ob + at_row * A.C, d[u]);
+                    if (!SHARED && gates) st<GT, VC>(db + at_row * drow, prev[u]);
+                }
             }
         }
         if (SHARED && gates) {
