@@ -11,6 +11,7 @@ is ``code * scale`` with an OCP e4m3 code (first moment) or e5m2 code (second mo
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -21,7 +22,8 @@ from . import lib as _lib
 BLOCK = 256                       # elements that share a scale in an 8-bit moment
 MOMENT_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
 _TENSOR_WORDS = C.sizeof(_lib.NkAdamwTensor) // 8
-_address = torch.Tensor.data_ptr
+_address, _numel, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+_dtype = operator.attrgetter("dtype")
 
 
 def _check_list(name: str, tensors: Sequence[torch.Tensor], numels: Sequence[int], dtype: torch.dtype, device, spans: list) -> List[int]:
@@ -129,7 +131,7 @@ class AdamW:
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
         self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
         self.device, self._dtype = dev, dt
-        self._numels = [p.numel() for p in params]
+        self._numels, self._indices = [p.numel() for p in params], [dev.index] * len(params)
         self._owned = self.params + (self.masters or ())
         self._held = [t.detach() for t in (*m, *v, *(s for pair in scales or () for s in pair))]       # the table's moments, whatever becomes of `state`
         self._bind()
@@ -158,6 +160,21 @@ class AdamW:
         self._words = (C.c_int64 * (_TENSOR_WORDS * n))(*[w for row in zip(at_p, none, at_m, at_v, at_w, at_sm, at_sv, numels) for w in row])
         self._table = C.cast(self._words, C.POINTER(_lib.NkAdamwTensor))
 
+    def _check_grads(self, grads) -> List[int]:
+        """Addresses of the gradients, after their checks (whole lists at a time: a step is called with hundreds)."""
+        n, numels, dev = len(self.params), self._numels, self.device
+        if len(grads) != n or not all(isinstance(g, torch.Tensor) for g in grads):
+            raise ValueError(f"grads: {len(grads)} entries for {n} parameters, one tensor each wanted")
+        gd = grads[0].dtype
+        if gd != torch.float32 and gd != self._dtype:
+            raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self._dtype})")
+        if (list(map(_numel, grads)) != numels or list(map(_get_device, grads)) != self._indices or list(map(_dtype, grads)) != [gd] * n
+                or not all(map(_is_contiguous, grads))):
+            for i, (g, k) in enumerate(zip(grads, numels)):
+                if g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
+                    raise ValueError(f"grads[{i}]: expected {k} contiguous {gd} values on {dev}")
+        return list(map(_address, grads))
+
     def step(self, grads: Optional[Sequence[torch.Tensor]] = None, *, lr: Optional[float] = None, step: Optional[int] = None,
              grad_scale: float = 1.0, seed: Optional[int] = None, step_state: Optional[int] = None) -> None:
         """One update.  ``grads``: one contiguous tensor per parameter, all fp32 or all of the parameters' dtype
@@ -172,17 +189,8 @@ class AdamW:
             grads = [p.grad for p in self.params]
             if any(g is None for g in grads):
                 raise ValueError("AdamW.step: a parameter has no .grad")
-        if len(grads) != n or not isinstance(grads[0], torch.Tensor):
-            raise ValueError(f"grads: {len(grads)} entries for {n} parameters, one tensor each wanted")
-        gd, dev, words, numels = grads[0].dtype, self.device, self._words, self._numels
-        if gd != torch.float32 and gd != self.params[0].dtype:
-            raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self.params[0].dtype})")
-        at = 1
-        for g, k in zip(grads, numels):
-            if g is None or g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
-                raise ValueError(f"grads[{at // _TENSOR_WORDS}]: expected {k} contiguous {gd} values on {dev}")
-            words[at] = g.data_ptr()
-            at += _TENSOR_WORDS
+        self._words[1::_TENSOR_WORDS] = self._check_grads(grads)
+        gd = grads[0].dtype
         step = self.steps + 1 if step is None else int(step)
         if step < 1:
             raise ValueError(f"step={step}: from 1")
@@ -191,7 +199,7 @@ class AdamW:
         o.grad_scale = float(grad_scale)
         o.seed = (self.seed + 0x9E3779B1 * step if seed is None else int(seed)) & 0xFFFFFFFF
         o.state = step_state
-        _lib.launch(dev, self._L.nk_adamw_step, self._table, n, o)
+        _lib.launch(self.device, self._L.nk_adamw_step, self._table, n, o)
         self.steps = step
         _increment_version(self.params)         # autograd refuses to use what it saved of them before
 

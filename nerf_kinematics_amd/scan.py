@@ -112,7 +112,7 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     if not isinstance(x, torch.Tensor) or x.dtype not in _lib.DTYPES or x.dim() != 3:
         raise ValueError("x: expected a [B, T, C] tensor of float32, bfloat16 or float16")
     B, T, C = x.shape
-    if not isinstance(a, torch.Tensor) or a.dim() != 3 or tuple(a.shape[:2]) != (B, T) or a.dtype not in (x.dtype, torch.float32):
+    if not isinstance(a, torch.Tensor) or a.dim() != 3 or a.shape != (B, T, a.shape[2]) or a.dtype not in (x.dtype, torch.float32):
         raise ValueError(f"a: expected a [{B}, {T}, J] tensor of {x.dtype} or float32")
     J = a.shape[2]
     if C < 1 or J < 1 or C % J:
@@ -124,11 +124,11 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     if a.device != dev:
         raise ValueError(f"a: expected a tensor on {dev}")
     if h0 is not None:
-        if h0.dtype != torch.float32 or tuple(h0.shape) != (B, C) or h0.device != dev:
+        if h0.dtype != torch.float32 or h0.shape != (B, C) or h0.device != dev:
             raise ValueError(f"h0: expected a float32 tensor of shape {(B, C)} on {dev}")
         h0 = h0.contiguous()
     if lengths is not None:
-        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or lengths.device != dev:
+        if lengths.dtype != torch.int32 or lengths.shape != (B,) or lengths.device != dev:
             raise ValueError(f"lengths: expected an int32 tensor of shape {(B,)} on {dev}")
         lengths = lengths.contiguous()
     a, x = _rows(a), _rows(x)
