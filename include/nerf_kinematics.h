@@ -265,7 +265,7 @@ typedef struct nk_xent_opts {
     int32_t reduction;            /* NK_REDUCE_*                                              */
     int64_t piece;                /* rows of the vocabulary per piece of the backward call, rounded up to 256;
                                      0: as many as keep a piece's gradients (2 N piece elements) near
-                                     256 MB, 2048 at least                                 */
+                                     512 MB, 2048 at least                                 */
 } nk_xent_opts;
 /* Scratch of a call on these operands (256-byte aligned; it holds nothing between calls). */
 int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int backward);
