@@ -163,13 +163,16 @@ class AdamW:
     def _check_grads(self, grads) -> List[int]:
         """Addresses of the gradients, after their checks (whole lists at a time: a step is called with hundreds)."""
         n, numels, dev = len(self.params), self._numels, self.device
-        if len(grads) != n or not all(isinstance(g, torch.Tensor) for g in grads):
-            raise ValueError(f"grads: {len(grads)} entries for {n} parameters, one tensor each wanted")
+        try:
+            same = len(grads) == n and list(map(_numel, grads)) == numels and list(map(_get_device, grads)) == self._indices and all(map(_is_contiguous, grads))
+        except TypeError:           # not a tensor
+            raise ValueError(f"grads: {len(grads)} entries for {n} parameters, one tensor each wanted") from None
+        if len(grads) != n:
+            raise ValueError(f"grads: {len(grads)} tensors for {n} parameters")
         gd = grads[0].dtype
         if gd != torch.float32 and gd != self._dtype:
             raise ValueError(f"grads: dtype {gd} (float32 or the parameters' {self._dtype})")
-        if (list(map(_numel, grads)) != numels or list(map(_get_device, grads)) != self._indices or list(map(_dtype, grads)) != [gd] * n
-                or not all(map(_is_contiguous, grads))):
+        if not same or list(map(_dtype, grads)) != [gd] * n:
             for i, (g, k) in enumerate(zip(grads, numels)):
                 if g.dtype != gd or g.numel() != k or g.device != dev or not g.is_contiguous():
                     raise ValueError(f"grads[{i}]: expected {k} contiguous {gd} values on {dev}")

@@ -48,8 +48,8 @@ def _forward(a, x, h0, lengths, reverse, training):
     dev = x.device
     if B == 0 or T == 0:        # no step: the state passes through
         return x.new_empty(B, T, C), (h0.clone() if h0 is not None else torch.zeros(B, C, dtype=torch.float32, device=dev)), None
-    h = torch.empty((B, T, C), dtype=x.dtype, device=dev)
-    last = torch.empty((B, C), dtype=torch.float32, device=dev)
+    h = torch.empty_like(x) if x.is_contiguous() else torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    last = torch.empty_like(h0) if h0 is not None else torch.empty((B, C), dtype=torch.float32, device=dev)
     o = _opts(a, x, None, lengths, reverse)
     states = torch.empty(B * (-(-T // _KEEP)) * C, dtype=torch.float32, device=dev) if training else None
     ws, n = _workspace(L, o, 0, dev)
