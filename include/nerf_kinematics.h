@@ -254,8 +254,9 @@ int nk_gated_scan_bwd(const nk_scan_opts* opts /*host*/, const void* a, const vo
  * target: device int64, 0 .. V-1 or ignore_index (loss 0, no gradient; such a row of hidden may hold
  * anything).  Any other value makes the token's loss and the gradients NaN; nothing is read out of range.
  * NK_REDUCE_MEAN divides by the number of tokens that are not ignored (0 if there are none).
- * hidden and weight have unit stride along D and the given row strides (in elements); rows that do not start
- * on 16 bytes are copied into the workspace first, the weight piece by piece.                       */
+ * hidden and weight have unit stride along D and the given row strides (in elements, up to 2^22 bytes); rows
+ * that do not start on 16 bytes are copied into the workspace first, the weight piece by piece.  N up to 2^24 (the
+ * backward call in fp32: 2^20), V up to 2^26, D up to 2^20.                                           */
 enum { NK_REDUCE_NONE = 0, NK_REDUCE_MEAN = 1, NK_REDUCE_SUM = 2 };
 typedef struct nk_xent_opts {
     int64_t N, D, V;
@@ -264,8 +265,8 @@ typedef struct nk_xent_opts {
     int32_t dtype;                /* NK_F32 | NK_BF16 | NK_F16                                */
     int32_t reduction;            /* NK_REDUCE_*                                              */
     int64_t piece;                /* rows of the vocabulary per piece of the backward call, rounded up to 256;
-                                     0: as many as keep a piece's gradients (2 N piece elements) near
-                                     512 MB, 2048 at least                                 */
+                                     0: as many as keep a piece's gradients (N piece elements; fp32 keeps
+                                     them twice) near 256 MB, 2048 at least; 2^22 bytes of them at most */
 } nk_xent_opts;
 /* Scratch of a call on these operands (256-byte aligned; it holds nothing between calls). */
 int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int backward);

@@ -9,18 +9,19 @@
 // computed again, turned into dz (rounded once to the operands' type: the two products that follow take it as
 // a matrix operand) and multiplied into d_weight's rows of the piece and onto d_hidden's fp32 sums.
 //
-// All products have the form C[m][n] = sum_k A[m][k] B[n][k] with k contiguous in both operands; where the
-// mathematics wants the other order (weight^T, hidden^T) a piece is transposed once by a copy, and dz is
-// written in both orders by the tile that computes it.
+// All products have the form C[m][n] = sum_k A[m][k] B[n][k].  For 16-bit types an operand may have k along its rows
+// or along its columns, so weight and dz serve both products as they are; fp32 has k contiguous in both operands:
+// where the mathematics wants the other order (weight^T, hidden^T) a piece is transposed once by a copy, and dz
+// is written in both orders by the tile that computes it.
 #include "nk_common.h"
 
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-// Both orders of a piece's dz together, unless the caller names a piece.  Kernel time of a training pass of
-// 8192 x 2048 x 65536 / 4096 x 1024 x 32003: 128 MB 8.4 / 1.41 ms, 256 MB 7.75 / 1.25, 512 MB 7.64 / 1.20, 1 GB 7.61 / 1.25.
-enum { XENT_PIECE_MB = 512 };
+// A piece's dz, unless the caller names a piece.  Kernel time of a training pass of 8192 x 2048 x 65536 /
+// 4096 x 1024 x 32003: 64 MB 8.4 / 1.41 ms, 128 MB 7.75 / 1.25, 256 MB 7.64 / 1.20, 512 MB 7.61 / 1.25.
+enum { XENT_PIECE_MB = 256 };
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -58,7 +59,13 @@ template <> struct Op<float> {
 // chunk ^ (r & 7), so that the 16 rows a fragment read touches fall on different banks; the order is made by the
 // source address, the LDS side of such a load being fixed.  Rows behind the matrix and the end of k
 // are outside the buffer resource's range and arrive as zeros.
-struct Mat { const char* p; int64_t rows, stride; };      // stride in bytes, a multiple of 16, as is p
+//
+// An operand may also come with k along its rows ("k-major": A[k][m]), for 16-bit types: a step is then 64 rows of BM
+// (BN) elements, and the fragments are read with the transposing LDS read, which hands the 16 lanes of a group the
+// columns of four rows.  Chunk c of row k lies at c ^ f(k), f even and different for the rows that a wavefront reads at
+// once.  This takes the products of the backward pass straight from dz [token][row], weight and hidden: with
+// transposed copies of the three, 8192 x 2048 x 65536 took 7.64 ms of kernels and 4096 x 1024 x 32003 1.20 ms.
+struct Mat { const char* p; int64_t rows, stride, width; };      // bytes: stride, a multiple of 16, as is p; width of a row that may be read
 
 template <int BM_, int BN_, int WGM_, int WGN_, int STAGES_> struct Cfg {
     static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_;
@@ -85,24 +92,107 @@ NK_D u32x4 resource(const char* p, int64_t bytes) {
     return r;
 }
 
+// Place of chunk c of row k of a k-major operand of CH chunks a row.
+template <int CH> NK_D int k_major_chunk(int c, int k) { return c ^ ((2 * ((k & 3) | ((k >> 3) & 3) << 2)) & (CH - 2)); }
+
 // One tile's product in two parts: begin() starts the loads of the first steps, run() does the rest.  The
-// LDS of the operands has to be idle at begin().
-template <typename T, class C> struct TileProduct {
-    u32x4 ra, rb;
-    uint32_t va[C::PA], vb[C::PB];
+// LDS of the operands has to be idle at begin().  KA, KB: the operand is k-major.
+template <typename T, class C, bool KA = false, bool KB = false> struct TileProduct {
+    static_assert(sizeof(T) == 2 || !(KA || KB), "the transposing read takes 16-bit elements");
+    // What a wavefront loads of an operand: P instructions a step.
+    template <int P, bool K> struct Source {
+        u32x4 r;
+        uint32_t v[P];
+        uint64_t base;              // k-major: address of the next step's first row
+        int left;                   // and the rows that are left from there on
+        uint32_t stride, width;
+        template <int ROWS> NK_D void begin(const Mat& M, int64_t at, int64_t row_bytes, int wave, int lane) {
+            if constexpr (K) {
+                constexpr int CH = ROWS / 8;
+                const uint64_t a = (uint64_t)(M.p + at * sizeof(T));
+                base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) << 32;
+                left = __builtin_amdgcn_readfirstlane((int)M.rows);
+                stride = __builtin_amdgcn_readfirstlane((int)M.stride);
+                width = __builtin_amdgcn_readfirstlane((int)(M.width - at * (int64_t)sizeof(T)));
+                r[3] = 0x00027000;
+                asm volatile("s_nop 4" : "+s"(base), "+s"(left), "+s"(stride), "+s"(width));    // scalars written by the vector unit, read by loads issued from asm
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int l = (wave * P + i) * 64 + lane, k = l / CH;
+                    v[i] = (uint32_t)k * (uint32_t)M.stride + (uint32_t)k_major_chunk<CH>(l % CH, k) * 16;
+                }
+            } else {
+                r = resource(M.p + at * M.stride, (M.rows - at - 1) * M.stride + row_bytes);
+                asm volatile("s_nop 4" : "+s"(r));
+                // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
+                const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[i] = (uint32_t)((wave * P + i) * 8 + lrow) * (uint32_t)M.stride + lchunk * 16;
+            }
+        }
+        // The loads of step s, behind the end of k as well (out of range: no memory is touched), so that the loop has no
+        // branches and the number of loads in flight is always the same.
+        NK_D void issue(uint32_t at, int s, uint32_t out, int wave) {
+            if constexpr (K) {
+                const int rows = left < 64 ? left : 64;
+                r[0] = (uint32_t)base; r[1] = (uint32_t)(base >> 32) & 0xFFFF; r[2] = rows > 0 ? (uint32_t)(rows - 1) * stride + width : 0;
+                base += (uint64_t)stride * 64; left -= 64;
+#pragma unroll
+                for (int i = 0; i < P; ++i) lds_load(at + (wave * P + i) * 1024, r, v[i], 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i) lds_load(at + (wave * P + i) * 1024, r, v[i] | out, (uint32_t)s * 128);
+            }
+        }
+    };
+    // Where a lane finds its fragments of an operand of ROWS rows (columns, if k-major): TILES of 16 from `first` on.
+    template <int ROWS, int TILES, bool K> struct Fragments {
+        const char* p;
+        int x0, x1;
+        int c[K ? TILES : 1];
+        NK_D Fragments(const char* lds, int first, int lane) {
+            if constexpr (K) {
+                constexpr int CH = ROWS / 8;
+                const int q = lane >> 4, j = lane & 15, k = 8 * q + (j >> 2);
+                p = lds + k * CH * 16 + (j & 1) * 8;
+                x0 = 0; x1 = 32 * CH * 16;
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) c[i] = k_major_chunk<CH>(first / 8 + 2 * i + ((j >> 1) & 1), k) * 16;
+            } else {
+                const int frow = lane & 15, fchunk = lane >> 4;
+                p = lds + (first + frow) * 128;
+                x0 = (fchunk ^ (frow & 7)) * 16; x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
+                c[0] = 0;
+            }
+        }
+        NK_D void read(u32x4 (&f)[TILES], int at, int x) const {
+            const char* a = p + at + x;
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+                if constexpr (K) {
+                    constexpr int CH = ROWS / 8;
+                    typedef __attribute__((ext_vector_type(4))) short s16x4;
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NK_LDS s16x4*)(a + c[i])));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NK_LDS s16x4*)(a + c[i] + 4 * CH * 16)));
+                    f[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                } else {
+                    f[i] = *(const u32x4*)(a + i * 2048);
+                }
+            }
+        }
+    };
+
+    Source<C::PA, KA> sa;
+    Source<C::PB, KB> sb;
     uint32_t lds0;
     int steps, last, wave;
     char* lds;
 
-    // Loads of a step, behind the end of k as well (out of range: no memory is touched), so that the loop has
-    // no branches and the number of loads in flight is always the same.
     NK_D void issue(int s, int slot) {
         const uint32_t out = s < last ? 0u : 0x80000000u;
         const uint32_t at = lds0 + slot * C::STAGE_BYTES;
-#pragma unroll
-        for (int i = 0; i < C::PA; ++i) lds_load(at + (wave * C::PA + i) * 1024, ra, va[i] | out, (uint32_t)s * 128);
-#pragma unroll
-        for (int i = 0; i < C::PB; ++i) lds_load(at + C::BM * 128 + (wave * C::PB + i) * 1024, rb, vb[i] | out, (uint32_t)s * 128);
+        sa.issue(at, s, out, wave);
+        sb.issue(at + C::BM * 128, s, out, wave);
     }
 
     NK_D void begin(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds_) {
@@ -111,17 +201,11 @@ template <typename T, class C> struct TileProduct {
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         // the last byte that a row of this stretch of k may be read to; rows and steps behind it arrive as zeros
         const int64_t row_bytes = (kbytes + 15) & ~(int64_t)15;
-        ra = resource(A.p + m0 * A.stride, (A.rows - m0 - 1) * A.stride + row_bytes);
-        rb = resource(B.p + n0 * B.stride, (B.rows - n0 - 1) * B.stride + row_bytes);
-        asm volatile("s_nop 4" : "+s"(ra), "+s"(rb));       // scalars written by the vector unit, read by loads issued from asm
+        sa.template begin<C::BM>(A, m0, row_bytes, wave, lane);
+        sb.template begin<C::BN>(B, n0, row_bytes, wave, lane);
         lds0 = (uint32_t)(uintptr_t)(NK_LDS char*)lds;
-        // this lane's place in a load instruction: row (lane / 8) of eight, chunk of the row by the order above
-        const int lrow = lane >> 3, lchunk = (lane & 7) ^ (lrow & 7);
-#pragma unroll
-        for (int i = 0; i < C::PA; ++i) va[i] = (uint32_t)((wave * C::PA + i) * 8 + lrow) * (uint32_t)A.stride + lchunk * 16;
-#pragma unroll
-        for (int i = 0; i < C::PB; ++i) vb[i] = (uint32_t)((wave * C::PB + i) * 8 + lrow) * (uint32_t)B.stride + lchunk * 16;
         steps = (int)((kbytes + 127) / 128);
+        const int lchunk = (lane & 7) ^ ((lane >> 3) & 7);
         last = (int)((kbytes - lchunk * 16 + 127) / 128);       // steps in which this lane's chunk is inside k
 #pragma unroll
         for (int s = 0; s < C::STAGES; ++s) issue(s, s);
@@ -133,18 +217,12 @@ template <typename T, class C> struct TileProduct {
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-        const int frow = lane & 15, fchunk = lane >> 4;
-        const char* fa = lds + (wm * C::TM * 16 + frow) * 128;
-        const char* fb = lds + (C::BM + wn * C::TN * 16 + frow) * 128;
-        const int x0 = (fchunk ^ (frow & 7)) * 16, x1 = ((fchunk + 4) ^ (frow & 7)) * 16;
+        const Fragments<C::BM, C::TM, KA> fa(lds, wm * C::TM * 16, lane);
+        const Fragments<C::BN, C::TN, KB> fb(lds + C::BM * 128, wn * C::TN * 16, lane);
         u32x4 a0[C::TM], b0[C::TN], a1[C::TM], b1[C::TN];
-        auto read = [&](u32x4 (&a)[C::TM], u32x4 (&b)[C::TN], int slot, int x) {
-            const char* pa = fa + slot * C::STAGE_BYTES + x;
-            const char* pb = fb + slot * C::STAGE_BYTES + x;
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j) b[j] = *(const u32x4*)(pb + j * 2048);
-#pragma unroll
-            for (int i = 0; i < C::TM; ++i) a[i] = *(const u32x4*)(pa + i * 2048);
+        auto read = [&](u32x4 (&a)[C::TM], u32x4 (&b)[C::TN], int slot, bool second) {
+            fb.read(b, slot * C::STAGE_BYTES, second ? fb.x1 : fb.x0);
+            fa.read(a, slot * C::STAGE_BYTES, second ? fa.x1 : fa.x0);
         };
         auto multiply = [&](const u32x4 (&a)[C::TM], const u32x4 (&b)[C::TN]) {
 #pragma unroll
@@ -152,27 +230,28 @@ template <typename T, class C> struct TileProduct {
 #pragma unroll
                 for (int j = 0; j < C::TN; ++j) acc[i][j] = Op<T>::mma(a[i], b[j], acc[i][j]);
             // one LDS read between every few products (0x100: LDS read, 0x008: matrix product)
+            constexpr int READS = C::TM * (KA ? 2 : 1) + C::TN * (KB ? 2 : 1), EACH = C::TM * C::TN / READS;
 #pragma unroll
-            for (int q = 0; q < C::TM + C::TN; ++q) {
+            for (int q = 0; q < READS; ++q) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, C::TM * C::TN / (C::TM + C::TN), 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, EACH > 0 ? EACH : 1, 0);
             }
         };
         constexpr int S = C::STAGES;
         wait_loads_and_meet<(S - 1) * C::PIECES>();
-        read(a0, b0, 0, x0);
+        read(a0, b0, 0, false);
         int slot = 0;
         for (int s = 0; s < steps; ++s) {
             const int next = slot + 1 == S ? 0 : slot + 1;
             // the second half of the step's fragments arrives while the first is multiplied
-            read(a1, b1, slot, x1);
+            read(a1, b1, slot, true);
             multiply(a0, b0);
             __builtin_amdgcn_sched_barrier(0);
             // everyone has read this step; the next one has landed when at most the loads behind it are outstanding
             wait_loads_and_meet<(S - 2) * C::PIECES>();
             issue(s + S, slot);
             __builtin_amdgcn_sched_barrier(0);
-            read(a0, b0, next, x0);
+            read(a0, b0, next, false);
             multiply(a1, b1);
             __builtin_amdgcn_sched_barrier(0);
             slot = next;
@@ -181,9 +260,9 @@ template <typename T, class C> struct TileProduct {
     }
 };
 
-template <typename T, class C>
+template <typename T, class C, bool KA = false, bool KB = false>
 NK_D void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0, int64_t kbytes, char* lds, f32x4 (&acc)[C::TM][C::TN]) {
-    TileProduct<T, C> p;
+    TileProduct<T, C, KA, KB> p;
     p.begin(A, B, m0, n0, kbytes, lds);
     p.run(acc);
 }
@@ -430,31 +509,19 @@ struct DzArgs {
     int64_t kbytes, v0, N;
     const int64_t* target;
     const float* lse; const float* c;
-    void* dz; int64_t dz_ld;                // [token][row of the piece]
-    void* dzt; int64_t dzt_ld;              // [row of the piece][token], zero up to dzt_ld
+    void* dz; int64_t dz_ld;                // [token][row of the piece], zero up to dz_ld
+    void* dzt; int64_t dzt_ld;              // fp32 only: [row of the piece][token], zero up to dzt_ld
 };
 
-// 4 x 4 transpose of 16-bit values over the four lanes of a quad: in, p = elements 0..3 of this lane's column;
-// out, element (lane & 3) of the quad's four columns
-NK_D u32x2 quad_transpose(u32x2 p, int lane) {
-    const bool b0 = lane & 1, b1 = lane & 2;
-    const uint32_t x = b1 ? p[1] : p[0];
-    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)(b1 ? p[0] : p[1]), 0x4E, 0xF, 0xF, true);      // from lane ^ 2
-    // x: elements 2 b1, 2 b1 + 1 of this column; y: of column ^ 2
-    const uint32_t lo = (x & 0xFFFFu) | (y << 16), hi = (x >> 16) | (y & 0xFFFF0000u);
-    uint32_t keep = b0 ? hi : lo;                                                                              // columns own, own ^ 2
-    uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(b0 ? lo : hi), 0xB1, 0xF, 0xF, true);              // columns own ^ 1, own ^ 3
-    if (b1) { keep = (keep >> 16) | (keep << 16); got = (got >> 16) | (got << 16); }
-    const uint32_t even = b0 ? got : keep, odd = b0 ? keep : got;
-    return u32x2{(even & 0xFFFFu) | (odd << 16), (even >> 16) | (odd & 0xFFFF0000u)};
-}
+// dz leaves in the orders that the products take: one for 16-bit types, both for fp32
+template <typename T> constexpr bool BOTH_ORDERS = sizeof(T) == 4;
 
 template <typename T, class C>
 __global__ __launch_bounds__(C::THREADS) void k_xent_dz(const DzArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
     int64_t mi, ni;
     // up to the padded token count: those columns of dzt have to be zero
-    tile_of(blockIdx.x, (g.w.rows + C::BM - 1) / C::BM, (g.dzt_ld + C::BN - 1) / C::BN, &mi, &ni);
+    tile_of(blockIdx.x, (g.w.rows + C::BM - 1) / C::BM, ((BOTH_ORDERS<T> ? g.dzt_ld : g.N) + C::BN - 1) / C::BN, &mi, &ni);
     f32x4 acc[C::TM][C::TN];
     tile_product<T, C>(g.w, g.h, mi * C::BM, ni * C::BN, g.kbytes, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
@@ -477,57 +544,29 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_dz(const DzArgs g) {
                 acc[i][j][e] = (c == 0.0f || r >= live) ? 0.0f : p * cs;
             }
     }
-    if constexpr (sizeof(T) == 2) {
-        // Both orders leave through LDS, as whole rows of the tile: straight from the registers a store would
-        // touch 16 rows with 32 bytes each.  Rows of 16-byte chunks, chunk ^ (row & mask) against bank conflicts.
+    if constexpr (!BOTH_ORDERS<T>) {
+        // The tile leaves through LDS, as whole rows of it: straight from the registers a store would touch 16
+        // rows with 32 bytes each.  Rows of 16-byte chunks, chunk ^ (row & mask) against bank conflicts.
         typedef __attribute__((ext_vector_type(4))) T vec;
-        u32x2 pk[C::TM][C::TN];
+        static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the operands' LDS");
+        constexpr int CH = C::BM / 8;           // [token][row]
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+        for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-            for (int j = 0; j < C::TN; ++j) {
+            for (int i = 0; i < C::TM; ++i) {
+                const int r = r0 + 16 * i, c = c0 + 16 * j;
                 vec w;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = (T)acc[i][j][e];
-                pk[i][j] = __builtin_bit_cast(u32x2, w);
+                *(u32x2*)(lds + (c * CH + ((r >> 3) ^ (c & (CH - 1)))) * 16 + (r & 4) * 2) = __builtin_bit_cast(u32x2, w);
             }
-        static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the operands' LDS");
-        {
-            constexpr int CH = C::BM / 8;           // [token][row]
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-                for (int i = 0; i < C::TM; ++i) {
-                    const int r = r0 + 16 * i, c = c0 + 16 * j;
-                    *(u32x2*)(lds + (c * CH + ((r >> 3) ^ (c & (CH - 1)))) * 16 + (r & 4) * 2) = pk[i][j];
-                }
-            __syncthreads();
-            T* dz = (T*)g.dz + mi * C::BM;
+        __syncthreads();
+        T* dz = (T*)g.dz + mi * C::BM;
 #pragma unroll 4
-            for (int q = threadIdx.x; q < C::BN * CH; q += C::THREADS) {
-                const int c = q / CH, k = q % CH;
-                const int64_t n = ni * C::BN + c;
-                if (n < g.N && mi * C::BM + k * 8 < g.dz_ld) *(u32x4*)(dz + n * g.dz_ld + k * 8) = *(const u32x4*)(lds + (c * CH + (k ^ (c & (CH - 1)))) * 16);
-            }
-            __syncthreads();
-        }
-        {
-            constexpr int CH = C::BN / 8;           // [row][token]
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-                for (int i = 0; i < C::TM; ++i) {
-                    const int r = r0 + 16 * i + (lane & 3), c = c0 + 16 * j - (lane & 3);
-                    *(u32x2*)(lds + (r * CH + ((c >> 3) ^ (r & (CH - 1)))) * 16 + (c & 4) * 2) = quad_transpose(pk[i][j], lane);
-                }
-            __syncthreads();
-            T* dzt = (T*)g.dzt + ni * C::BN;
-#pragma unroll 4
-            for (int q = threadIdx.x; q < C::BM * CH; q += C::THREADS) {
-                const int r = q / CH, k = q % CH;
-                const int64_t v = mi * C::BM + r;
-                if (v < g.w.rows && ni * C::BN + k * 8 < g.dzt_ld) *(u32x4*)(dzt + v * g.dzt_ld + k * 8) = *(const u32x4*)(lds + (r * CH + (k ^ (r & (CH - 1)))) * 16);
-            }
+        for (int q = threadIdx.x; q < C::BN * CH; q += C::THREADS) {
+            const int c = q / CH, k = q % CH;
+            const int64_t n = ni * C::BN + c;
+            if (n < g.N && mi * C::BM + k * 8 < g.dz_ld) *(u32x4*)(dz + n * g.dz_ld + k * 8) = *(const u32x4*)(lds + (c * CH + (k ^ (c & (CH - 1)))) * 16);
         }
     } else {
 #pragma unroll
@@ -545,7 +584,7 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_dz(const DzArgs g) {
 
 struct ProductArgs {
     Mat a, b;
-    int64_t k0, kbytes, kslice;             // bytes of k: slice z takes k0 + z * kslice .. (kslice a multiple of 128)
+    int64_t kbytes, kslice;                 // bytes of k: slice z takes z * kslice .. (kslice a multiple of 128)
     int64_t M, N;
     void* out; int64_t ld;                  // [n][m]
     float* sums; int add;                   // fp32 sums [slice][n][m] instead; add: onto what is there
@@ -554,16 +593,18 @@ struct ProductArgs {
 };
 
 // C[m][n] -> out[n][m]: a lane holds four consecutive m of one n
-template <typename T, class C, bool SUMS>
+template <typename T, class C, bool SUMS, bool KA, bool KB>
 __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
     int64_t mi, ni;
     tile_of(blockIdx.x, (g.M + C::BM - 1) / C::BM, (g.N + C::BN - 1) / C::BN, &mi, &ni);
     const int64_t at = blockIdx.y * g.kslice, left = g.kbytes - at;
     Mat a = g.a, b = g.b;
-    a.p += at; b.p += at;
+    const int64_t row = at / (int64_t)sizeof(T);
+    if (KA) { a.p += row * a.stride; a.rows -= row; } else a.p += at;
+    if (KB) { b.p += row * b.stride; b.rows -= row; } else b.p += at;
     f32x4 acc[C::TM][C::TN];
-    tile_product<T, C>(a, b, mi * C::BM, ni * C::BN, left < 0 ? 0 : left < g.kslice ? left : g.kslice, lds, acc);
+    tile_product<T, C, KA, KB>(a, b, mi * C::BM, ni * C::BN, left < 0 ? 0 : left < g.kslice ? left : g.kslice, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / C::WGN, wn = wave % C::WGN;
     const float f = SUMS ? 1.0f : *g.rest * g.scale;
     const bool vec = SUMS ? (g.M & 3) == 0 : (g.ld & 3) == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0;
@@ -631,13 +672,27 @@ __global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ s
     *(tvec*)(out + i) = w;
 }
 
-// dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take
-template <typename T>
-__global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, T* __restrict__ dst, int64_t dst_ld) {
-    const int64_t i = flat_block() * 256 + threadIdx.x;
+// dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take, or
+// whose values may be anything where factor[r] = 0 (they become zeros).  16 bytes a thread; VEC: source rows start on 16 bytes.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, const float* __restrict__ factor,
+                                                  T* __restrict__ dst, int64_t dst_ld) {
+    constexpr int E = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(E))) T vec;
+    const int64_t i = (flat_block() * 256 + threadIdx.x) * E;
     if (i >= rows * dst_ld) return;
-    const int64_t r = i / dst_ld, c = i - r * dst_ld;
-    dst[i] = c < cols ? src[r * ld + c] : (T)0.0f;
+    const int64_t r = i / dst_ld, c = i - r * dst_ld;           // dst_ld is a multiple of E
+    vec v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (T)0.0f;
+    if (!(factor && factor[r] == 0.0f)) {
+        if (VEC && c + E <= cols) v = *(const vec*)(src + r * ld + c);
+        else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) if (c + e < cols) v[e] = src[r * ld + c + e];
+        }
+    }
+    *(vec*)(dst + i) = v;
 }
 
 // dst[c][0 .. dst_ld) = src[0 .. rows)[c], zeros behind; rows with factor c = 0 are left out as zeros (their
@@ -724,7 +779,7 @@ int64_t cut_of(int64_t M, int64_t N, int64_t k, int64_t step) {
 
 struct Plan {
     int64_t Dp, Np, piece;                  // padded k of the logits' product; tokens padded to a step; vocabulary rows per piece
-    bool pad_h, pad_w;
+    bool pad_h, pad_w, copy_h;
     int kind, slices;
     int64_t parts, zt, losses, h, w, c, rest, tally, wt, ht, dz, dzt, sums, wsums, total;
 };
@@ -748,16 +803,20 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
     const int64_t asked = o->piece < o->V ? up(o->piece, 256) : up(o->V, 256);       // 0: not asked for
     int64_t piece;
     if (backward) {
-        piece = asked ? asked : up((int64_t)(XENT_PIECE_MB / 2 << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
+        piece = asked ? asked : up(((int64_t)XENT_PIECE_MB << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
         if (piece < 2048 && !asked) piece = 2048;
     } else {
         piece = p->pad_w ? (asked ? asked : 16384) : up(o->V, 256);
     }
+    if (piece > (1 << 22) / es) piece = (1 << 22) / es;         // a row of dz: up to 2^22 bytes, as of the other operands
     if (piece > o->V) piece = up(o->V, step);           // the only one
+    const bool both = o->dtype == NK_F32;               // dz in both orders, transposed copies of weight and hidden
+    if (backward && both && o->N > (1 << 20)) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: fp32 gradients of up to 2^20 tokens a call", who);
     p->piece = piece;
     int64_t off = 0;
     auto take = [&](int64_t bytes) { const int64_t at = off; off = up(off + bytes, 1024); return at; };
-    p->h = take(p->pad_h ? o->N * p->Dp * es : 0);
+    p->copy_h = p->pad_h || (backward && !both);        // without the values of tokens that do not count
+    p->h = take(p->copy_h ? o->N * p->Dp * es : 0);
     p->w = take(p->pad_w ? piece * p->Dp * es : 0);
     p->kind = tile_kind(piece < o->V ? piece : o->V, o->N);
     p->slices = 1;
@@ -769,10 +828,10 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
         p->c = take(o->N * 4);
         p->rest = take(4);
         p->tally = take(cdiv(o->N, TALLY_TOKENS) * sizeof(Tally));
-        p->wt = take(o->D * piece * es);
-        p->ht = take(o->D * p->Np * es);
+        p->wt = take(both ? o->D * piece * es : 0);
+        p->ht = take(both ? o->D * p->Np * es : 0);
         p->dz = take(o->N * piece * es);
-        p->dzt = take(piece * p->Np * es);
+        p->dzt = take(both ? piece * p->Np * es : 0);
         p->slices = o->N > 0 ? (int)cut_of(o->D, o->N, piece, step) : 1;
         p->sums = take(p->slices == 1 && piece >= o->V ? 0 : (int64_t)p->slices * o->N * o->D * 4);
         // d_weight of a whole piece, and of the last one
@@ -792,10 +851,10 @@ template <typename T, class C> int lse_start(const LseArgs& g, hipStream_t st) {
     return start<k_xent_lse<T, C>>(g, tiles < fit ? tiles : fit, 1, C::THREADS, st, "k_xent_lse");
 }
 template <typename T, class C> int dz_start(const DzArgs& g, hipStream_t st) {
-    return start<k_xent_dz<T, C>>(g, cdiv(g.w.rows, C::BM) * cdiv(g.dzt_ld, C::BN), 1, C::THREADS, st, "k_xent_dz");
+    return start<k_xent_dz<T, C>>(g, cdiv(g.w.rows, C::BM) * cdiv(BOTH_ORDERS<T> ? g.dzt_ld : g.N, C::BN), 1, C::THREADS, st, "k_xent_dz");
 }
-template <typename T, class C, bool SUMS> int product_start(const ProductArgs& g, int slices, hipStream_t st) {
-    return start<k_xent_product<T, C, SUMS>>(g, cdiv(g.M, C::BM) * cdiv(g.N, C::BN), slices, C::THREADS, st, "k_xent_product");
+template <typename T, class C, bool SUMS, bool KA, bool KB> int product_start(const ProductArgs& g, int slices, hipStream_t st) {
+    return start<k_xent_product<T, C, SUMS, KA, KB>>(g, cdiv(g.M, C::BM) * cdiv(g.N, C::BN), slices, C::THREADS, st, "k_xent_product");
 }
 template <typename T> int lse_launch(int kind, const LseArgs& g, hipStream_t st) {
     return kind == LARGE ? lse_start<T, Large>(g, st) : kind == MIDDLE ? lse_start<T, Middle>(g, st) : kind == FEW ? lse_start<T, Few>(g, st)
@@ -805,15 +864,18 @@ template <typename T> int dz_launch(int kind, const DzArgs& g, hipStream_t st) {
     return kind == LARGE ? dz_start<T, Large>(g, st) : kind == MIDDLE ? dz_start<T, Middle>(g, st) : kind == FEW ? dz_start<T, Few>(g, st)
                                                                                                       : dz_start<T, Small>(g, st);
 }
-template <typename T, bool SUMS> int product_launch(const ProductArgs& g, int slices, hipStream_t st) {
+template <typename T, bool SUMS, bool KA, bool KB> int product_launch(const ProductArgs& g, int slices, hipStream_t st) {
     const int kind = tile_kind(g.M, g.N, slices);
-    return kind == LARGE ? product_start<T, Large, SUMS>(g, slices, st) : kind == MIDDLE ? product_start<T, Middle, SUMS>(g, slices, st)
-         : kind == FEW ? product_start<T, Few, SUMS>(g, slices, st) : product_start<T, Small, SUMS>(g, slices, st);
+    return kind == LARGE ? product_start<T, Large, SUMS, KA, KB>(g, slices, st) : kind == MIDDLE ? product_start<T, Middle, SUMS, KA, KB>(g, slices, st)
+         : kind == FEW ? product_start<T, Few, SUMS, KA, KB>(g, slices, st) : product_start<T, Small, SUMS, KA, KB>(g, slices, st);
 }
 
-template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t dst_ld, hipStream_t st) {
-    const int64_t n = rows * dst_ld;
-    hipLaunchKernelGGL(k_xent_pad<T>, flat_grid(cdiv(n, 256)), dim3(256), 0, st, (const T*)src, ld, rows, cols, (T*)dst, dst_ld);
+template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* factor, void* dst, int64_t dst_ld, hipStream_t st) {
+    const dim3 grid = flat_grid(cdiv(rows * dst_ld, 256 * (16 / (int64_t)sizeof(T))));
+    if (((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0)
+        hipLaunchKernelGGL((k_xent_pad<T, true>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
+    else
+        hipLaunchKernelGGL((k_xent_pad<T, false>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
     NK_CHECK_LAUNCH("k_xent_pad");
     return NK_OK;
 }
@@ -842,19 +904,19 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
             char* ws, hipStream_t st) {
     const int es = sizeof(T);
     int rc;
-    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es};
-    if (p.pad_h) {
-        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, ws + p.h, p.Dp, st)) < 0) return rc;
-        h = Mat{ws + p.h, o->N, p.Dp * es};
+    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es, o->D * es};
+    if (p.copy_h) {
+        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, nullptr, ws + p.h, p.Dp, st)) < 0) return rc;
+        h = Mat{ws + p.h, o->N, p.Dp * es, p.Dp * es};
     }
     int64_t tiles = 0;
     for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
         const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
         const char* src = (const char*)weight + v0 * o->weight_stride * es;
-        Mat w = {src, rows, o->weight_stride * es};
+        Mat w = {src, rows, o->weight_stride * es, o->D * es};
         if (p.pad_w) {
-            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, ws + p.w, p.Dp, st)) < 0) return rc;
-            w = Mat{ws + p.w, rows, p.Dp * es};
+            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.w, p.Dp, st)) < 0) return rc;
+            w = Mat{ws + p.w, rows, p.Dp * es, p.Dp * es};
         }
         const LseArgs g = {w, h, o->D * es, v0, o->V, o->N, target, (float2*)(ws + p.parts), tiles, (float*)(ws + p.zt)};
         if ((rc = lse_launch<T>(p.kind, g, st)) < 0) return rc;
@@ -899,51 +961,58 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
     hipLaunchKernelGGL(k_xent_factors, dim3(parts ? groups : 1), dim3(1024), 0, st, target, o->N, o->V, o->ignore_index, o->reduction, d_loss, parts,
                        groups, c, rest);
     NK_CHECK_LAUNCH("k_xent_factors");
-    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es};
-    if (p.pad_h) {
-        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, ws + p.h, p.Dp, st)) < 0) return rc;
-        h = Mat{ws + p.h, o->N, p.Dp * es};
+    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es, o->D * es};
+    constexpr bool BOTH = BOTH_ORDERS<T>;
+    if (p.copy_h && (p.pad_h || d_weight)) {
+        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.h, p.Dp, st)) < 0) return rc;
+        h = Mat{ws + p.h, o->N, p.Dp * es, p.Dp * es};
     }
-    if (d_weight && (rc = transpose<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.ht, p.Np, st)) < 0) return rc;
+    if (BOTH && d_weight && (rc = transpose<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.ht, p.Np, st)) < 0) return rc;
     const int64_t slice = up(cdiv(p.piece, p.slices), 128 / es) * es;
     const bool direct = p.slices == 1 && p.piece >= o->V;      // d_hidden in one product: no sums to keep
     for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
         const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
         const char* src = (const char*)weight + v0 * o->weight_stride * es;
-        Mat w = {src, rows, o->weight_stride * es};
+        Mat w = {src, rows, o->weight_stride * es, o->D * es};
         if (p.pad_w) {
-            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, ws + p.w, p.Dp, st)) < 0) return rc;
-            w = Mat{ws + p.w, rows, p.Dp * es};
+            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.w, p.Dp, st)) < 0) return rc;
+            w = Mat{ws + p.w, rows, p.Dp * es, p.Dp * es};
         }
         const int64_t kv = up(rows, 128 / es);          // columns of dz that the product takes: zeros behind `rows`
         const DzArgs g = {w, h, o->D * es, v0, o->N, target, lse, c, ws + p.dz, kv, ws + p.dzt, p.Np};
         if ((rc = dz_launch<T>(tile_kind(rows, o->N), g, st)) < 0) return rc;
         if (d_weight) {
             ProductArgs q = {};
-            q.a = Mat{ws + p.ht, o->D, p.Np * es}; q.b = Mat{ws + p.dzt, rows, p.Np * es};
+            if (BOTH) { q.a = Mat{ws + p.ht, o->D, p.Np * es, 0}; q.b = Mat{ws + p.dzt, rows, p.Np * es, 0}; }
+            else { q.a = h; q.b = Mat{ws + p.dz, o->N, kv * es, kv * es}; }
             q.kbytes = q.kslice = p.Np * es; q.M = o->D; q.N = rows;
             char* out = (char*)d_weight + v0 * o->D * es;
             const int cut = (int)cut_of(o->D, rows, p.Np, 128 / es);
             if (cut == 1) {
                 q.out = out; q.ld = o->D; q.rest = rest; q.scale = unscale;
-                if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+                if ((rc = product_launch<T, false, !BOTH, !BOTH>(q, 1, st)) < 0) return rc;
             } else {
                 q.kslice = up(cdiv(p.Np, cut), 128 / es) * es; q.sums = (float*)(ws + p.wsums);
-                if ((rc = product_launch<T, true>(q, cut, st)) < 0) return rc;
+                if ((rc = product_launch<T, true, !BOTH, !BOTH>(q, cut, st)) < 0) return rc;
                 if ((rc = finish<T>(q.sums, cut, rows, o->D, nullptr, rest, unscale, out, st)) < 0) return rc;
             }
         }
         if (d_hidden) {
-            if ((rc = transpose<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.wt, kv, st)) < 0) return rc;
             ProductArgs q = {};
-            q.a = Mat{ws + p.wt, o->D, kv * es}; q.b = Mat{ws + p.dz, o->N, kv * es};
+            if (BOTH) {
+                if ((rc = transpose<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.wt, kv, st)) < 0) return rc;
+                q.a = Mat{ws + p.wt, o->D, kv * es, 0};
+            } else {
+                q.a = w;
+            }
+            q.b = Mat{ws + p.dz, o->N, kv * es, kv * es};
             q.kbytes = kv * es; q.kslice = slice; q.M = o->D; q.N = o->N;
             if (direct) {
                 q.out = d_hidden; q.ld = o->D; q.rest = rest; q.scale = unscale; q.row_on = c;
-                if ((rc = product_launch<T, false>(q, 1, st)) < 0) return rc;
+                if ((rc = product_launch<T, false, !BOTH, false>(q, 1, st)) < 0) return rc;
             } else {
                 q.sums = (float*)(ws + p.sums); q.add = v0 > 0;
-                if ((rc = product_launch<T, true>(q, p.slices, st)) < 0) return rc;
+                if ((rc = product_launch<T, true, !BOTH, false>(q, p.slices, st)) < 0) return rc;
             }
         }
     }

@@ -77,7 +77,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     tokens that are not ignored; 0 without any), "sum" or "none" ([N] losses).
 
     Differentiable in ``hidden`` and ``weight`` (first order).  The backward pass walks the vocabulary in pieces
-    of ``piece`` rows (default: as many as keep a piece's logit gradients near 512 MB, 2048 at least) and rounds the logit
+    of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB, 2048 at least) and rounds the logit
     gradients once to the operands' dtype between its products; sums are float32.
     """
     if reduction not in _lib.REDUCTIONS:

@@ -195,6 +195,13 @@ def test_layouts(which):
 
 
 @gpu
+def test_millions_of_tokens():
+    """Row offsets of the logit gradients far beyond 2^22 bytes times a tile's rows."""
+    h, w, t, g = make(4200003, 16, 3, BF16, 15)
+    check(h, w, t, "mean", g)
+
+
+@gpu
 def test_single_rows_of_any_stride():
     """One token and one label: torch gives a dimension of size one any stride, zero among them."""
     h, w, t, g = make(1, 24, 1, BF16, 12, ignored=0.0)
@@ -284,6 +291,8 @@ def test_refusals_on_the_host():
                     (dict(weight_stride=7), -1), (dict(piece=-1), -1), (dict(V=1 << 27), -2), (dict(D=1 << 21, hidden_stride=1 << 21, weight_stride=1 << 21), -2)):
         assert L.nk_linear_xent_workspace_bytes(o(**bad), 1024, 1024, 1) == rc, bad
         assert L.nk_linear_xent_fwd(o(**bad), 1024, 1024, 1024, 1024, 1024, 1024, 1024, 1 << 40, None) == rc, bad
+    assert L.nk_linear_xent_bwd(o(N=(1 << 20) + 1, dtype=0), 1024, 1024, 1024, 1024, 1024, 1024, 1024, 1024, 1 << 40, None) == -2
+    assert L.nk_linear_xent_workspace_bytes(o(N=64, D=8, V=1 << 26, piece=1 << 26), 1024, 1024, 1) < 64 * (1 << 22) + (1 << 20)     # a row of dz: 2^22 bytes
     assert L.nk_linear_xent_fwd(o(), None, 1024, 1024, 1024, 1024, 1024, 1024, 1 << 40, None) == -1
     assert L.nk_linear_xent_fwd(o(), 1024, 1024, 1024, 1024, 1024, None, 1024, 1 << 40, None) == -1
     assert L.nk_linear_xent_fwd(o(), 1024, 1024, 1024, 1024, 1024, 1024, 1024, 0, None) == -4
