@@ -86,7 +86,7 @@ template <int MANT, int BIAS> NK_D uint32_t encode(float y, uint32_t r16) {
 // wavefront holds exactly one block of 256.  Memory bounds the 32-bit step, memory and the vector unit about
 // equally the 8-bit one.  Four elements a thread and many workgroups, not a loop over more: 200 M fp32
 // parameters take 1 009 us (5.5 TB/s; a copy reaches 4.8) against 1 067 us with 16 elements a thread, 200 M bf16 ones
-// with masters and 8-bit moments 589 us (5.5 TB/s) against 641, the 1.2 M of an 8x256 pair in 48 tensors 7.8 us
+// with masters and 8-bit moments 589 us (5.5 TB/s; to 614 us on a warmer card) against 641, the 1.2 M of an 8x256 pair in 48 tensors 7.8 us
 // against 11.5.
 template <typename PT, typename GT, bool EIGHT>
 __global__ __launch_bounds__(AW_THREADS) void k_adamw(const AwArgs A) {
