@@ -449,23 +449,23 @@ __global__ __launch_bounds__(1024) void k_xent_reduce(const double2* __restrict_
 struct Tally { int count; uint32_t peak; };     // tokens that count, bits of the largest |d_loss| among them
 enum { TALLY_TOKENS = 4096 };
 
-NK_D Tally tally(const int64_t* target, int64_t n0, int64_t n1, int64_t ignore, int reduction, const float* d_loss) {
+template <int THREADS> NK_D Tally tally(const int64_t* target, int64_t n0, int64_t n1, int64_t ignore, int reduction, const float* d_loss) {
     Tally r = {0, 0};
 #pragma unroll 4
-    for (int64_t n = n0 + threadIdx.x; n < n1; n += 1024)
+    for (int64_t n = n0 + threadIdx.x; n < n1; n += THREADS)
         if (target[n] != ignore) {
             ++r.count;
             if (reduction == NK_REDUCE_NONE) r.peak = max(r.peak, __float_as_uint(d_loss[n]) & 0x7FFFFFFFu);
         }
     return r;
 }
-// over the workgroup of 1024 threads; the result is in thread 0
-NK_D Tally meet_tally(Tally r) {
-    __shared__ Tally meet[16];
+// over the workgroup; the result is in thread 0
+template <int THREADS> NK_D Tally meet_tally(Tally r) {
+    __shared__ Tally meet[THREADS / 64];
     for (int off = 32; off > 0; off >>= 1) { r.count += __shfl_xor(r.count, off, 64); r.peak = max(r.peak, (uint32_t)__shfl_xor((int)r.peak, off, 64)); }
     if ((threadIdx.x & 63) == 0) meet[threadIdx.x >> 6] = r;
     __syncthreads();
-    if (threadIdx.x == 0) for (int w = 1; w < 16; ++w) { r.count += meet[w].count; r.peak = max(r.peak, meet[w].peak); }
+    if (threadIdx.x == 0) for (int w = 1; w < THREADS / 64; ++w) { r.count += meet[w].count; r.peak = max(r.peak, meet[w].peak); }
     return r;
 }
 
@@ -474,40 +474,46 @@ NK_D Tally meet_tally(Tally r) {
 __global__ __launch_bounds__(1024) void k_xent_tally(const int64_t* __restrict__ target, int64_t N, int64_t ignore, int reduction,
                                                      const float* __restrict__ d_loss, Tally* __restrict__ out) {
     const int64_t n0 = (int64_t)blockIdx.x * TALLY_TOKENS, n1 = n0 + TALLY_TOKENS < N ? n0 + TALLY_TOKENS : N;
-    const Tally r = meet_tally(tally(target, n0, n1, ignore, reduction, d_loss));
+    const Tally r = meet_tally<1024>(tally<1024>(target, n0, n1, ignore, reduction, d_loss));
     if (threadIdx.x == 0) out[blockIdx.x] = r;
 }
 
-__global__ __launch_bounds__(1024) void k_xent_factors(const int64_t* __restrict__ target, int64_t N, int64_t V, int64_t ignore, int reduction,
-                                                       const float* __restrict__ d_loss, const Tally* __restrict__ parts, int n_parts,
-                                                       float* __restrict__ c, float* __restrict__ rest) {
+struct FactorArgs {
+    const int64_t* target; int64_t N, V, ignore;
+    int reduction, n_parts;
+    const float* d_loss;
+    const Tally* parts;         // NULL: every workgroup counts all tokens itself
+    float* c; float* rest;
+};
+template <int THREADS> NK_D void factors(const FactorArgs& f, int64_t block, int64_t blocks) {
     __shared__ float unit;
     Tally r = {0, 0};
-    if (parts) {
-        for (int i = threadIdx.x; i < n_parts; i += 1024) { r.count += parts[i].count; r.peak = max(r.peak, parts[i].peak); }
+    if (f.parts) {
+        for (int i = threadIdx.x; i < f.n_parts; i += THREADS) { r.count += f.parts[i].count; r.peak = max(r.peak, f.parts[i].peak); }
     } else {
-        r = tally(target, 0, N, ignore, reduction, d_loss);
+        r = tally<THREADS>(f.target, 0, f.N, f.ignore, f.reduction, f.d_loss);
     }
-    r = meet_tally(r);
+    r = meet_tally<THREADS>(r);
     if (threadIdx.x == 0) {
         float left;
-        if (reduction == NK_REDUCE_NONE) {
+        if (f.reduction == NK_REDUCE_NONE) {
             const int e = min(max((int)(r.peak >> 23) + 1, 27), 227);          // 2^-100 .. 2^100; infinities and NaN stay in c
             unit = __uint_as_float((uint32_t)(254 - e) << 23);
             left = __uint_as_float((uint32_t)e << 23);
         } else {
             unit = 1.0f;
-            left = reduction == NK_REDUCE_MEAN ? d_loss[0] / (float)(r.count > 0 ? r.count : 1) : d_loss[0];
+            left = f.reduction == NK_REDUCE_MEAN ? f.d_loss[0] / (float)(r.count > 0 ? r.count : 1) : f.d_loss[0];
         }
-        if (blockIdx.x == 0) *rest = left;
+        if (block == 0) *f.rest = left;
     }
     __syncthreads();
 #pragma unroll 4
-    for (int64_t n = (int64_t)blockIdx.x * 1024 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 1024) {
-        const int64_t t = target[n];
-        c[n] = t == ignore ? 0.0f : (t < 0 || t >= V) ? __builtin_nanf("") : reduction == NK_REDUCE_NONE ? d_loss[n] * unit : 1.0f;
+    for (int64_t n = block * THREADS + threadIdx.x; n < f.N; n += blocks * THREADS) {
+        const int64_t t = f.target[n];
+        f.c[n] = t == f.ignore ? 0.0f : (t < 0 || t >= f.V) ? __builtin_nanf("") : f.reduction == NK_REDUCE_NONE ? f.d_loss[n] * unit : 1.0f;
     }
 }
+__global__ __launch_bounds__(1024) void k_xent_factors(const FactorArgs f) { factors<1024>(f, blockIdx.x, gridDim.x); }
 
 struct DzArgs {
     Mat w, h;
@@ -592,15 +598,14 @@ struct ProductArgs {
     int64_t kbytes, kslice;                 // bytes of k: slice z takes z * kslice .. (kslice a multiple of 128)
     int64_t M, N;
     void* out; int64_t ld;                  // [n][m]
+    int slices;
     float* sums; int add;                   // fp32 sums [slice][n][m] instead; add: onto what is there
     const float* rest; float scale;
     const float* row_on;                    // out: rows n with row_on[n] = 0 are zero
 };
 
 // C[m][n] -> out[n][m]: a lane holds four consecutive m of one n
-template <typename T, class C, bool SUMS, bool KA, bool KB>
-__global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g) {
-    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+template <typename T, class C, bool SUMS, bool KA, bool KB> NK_D void product(const ProductArgs& g, char* lds) {
     int64_t mi, ni;
     tile_of(blockIdx.x, (g.M + C::BM - 1) / C::BM, (g.N + C::BN - 1) / C::BN, &mi, &ni);
     const int64_t at = blockIdx.y * g.kslice, left = g.kbytes - at;
@@ -650,6 +655,24 @@ __global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g
     }
 }
 
+template <typename T, class C, bool SUMS, bool KA, bool KB>
+__global__ __launch_bounds__(C::THREADS) void k_xent_product(const ProductArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    product<T, C, SUMS, KA, KB>(g, lds);
+}
+// d_weight (z = 0) and d_hidden (z = 1) of a small call in one launch: each alone leaves most of the chip idle, and
+// the host's time for launches is what such a call costs.  With k_xent_prepare and the finish of both in one, the backward
+// pass of 1024 x 256 x 1000 in fp32 takes four launches instead of eight: 35 us instead of 47, 35 of host instead of 44.
+struct PairArgs { ProductArgs p[2]; };
+template <typename T, class C, bool SUMS>
+__global__ __launch_bounds__(C::THREADS) void k_xent_pair(const PairArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    const ProductArgs& p = g.p[blockIdx.z];
+    if (blockIdx.x >= ((p.M + C::BM - 1) / C::BM) * ((p.N + C::BN - 1) / C::BN) || blockIdx.y >= p.slices) return;
+    constexpr bool K = !BOTH_ORDERS<T>;
+    if (blockIdx.z == 0) product<T, C, SUMS, K, K>(p, lds); else product<T, C, SUMS, K, false>(p, lds);
+}
+
 // A grid over many elements: the launch holds fewer than 2^32 threads along x.
 inline dim3 flat_grid(int64_t blocks) {
     const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
@@ -659,68 +682,74 @@ NK_D int64_t flat_block() { return blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
 
 // out [N][D] from its fp32 sums, the slices in one order.  c: NULL, or rows with c = 0 (tokens that do not count) are
 // zero.  VEC elements a thread.
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ sums, int slices, int64_t N, int64_t D, const float* __restrict__ c,
-                                                     const float* __restrict__ rest, float scale, T* __restrict__ out) {
-    const int64_t i = (flat_block() * 256 + threadIdx.x) * VEC;
-    if (i >= N * D) return;
+struct FinishArgs { const float* sums; int slices, vec; int64_t N, D; const float* c; const float* rest; float scale; void* out; int64_t blocks; };
+template <typename T, int VEC> NK_D void finish_block(const FinishArgs& g, int64_t block) {
+    const int64_t i = (block * 256 + threadIdx.x) * VEC;
+    if (i >= g.N * g.D) return;
     typedef __attribute__((ext_vector_type(VEC))) float fvec;
     typedef __attribute__((ext_vector_type(VEC))) T tvec;
-    fvec s = *(const fvec*)(sums + i);
+    fvec s = *(const fvec*)(g.sums + i);
 #pragma unroll 8
-    for (int k = 1; k < slices; ++k) s += *(const fvec*)(sums + (int64_t)k * N * D + i);
-    const float f = *rest * scale;
-    const bool on = !c || c[i / D] != 0.0f;
+    for (int k = 1; k < g.slices; ++k) s += *(const fvec*)(g.sums + (int64_t)k * g.N * g.D + i);
+    const float f = *g.rest * g.scale;
+    const bool on = !g.c || g.c[i / g.D] != 0.0f;
     tvec w;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) w[e] = (T)(on ? s[e] * f : 0.0f);
-    *(tvec*)(out + i) = w;
+    *(tvec*)((T*)g.out + i) = w;
+}
+template <typename T> __global__ __launch_bounds__(256) void k_xent_finish(const FinishArgs a, const FinishArgs b) {      // b: what is behind a's workgroups
+    const int64_t block = flat_block();
+    const FinishArgs& g = block < a.blocks ? a : b;
+    const int64_t at = block < a.blocks ? block : block - a.blocks;
+    if (at >= g.blocks) return;
+    if (g.vec) finish_block<T, 4>(g, at); else finish_block<T, 1>(g, at);
 }
 
-// dst[r][0 .. dst_ld) = src[r][0 .. cols), zeros behind: rows whose start or length the wide loads cannot take, or
-// whose values may be anything where factor[r] = 0 (they become zeros).  16 bytes a thread; VEC: source rows start on 16 bytes.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_xent_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, const float* __restrict__ factor,
-                                                  T* __restrict__ dst, int64_t dst_ld) {
+// A copy [rows][cols] into rows of dst_ld (PAD: rows whose start or length the wide loads cannot take), or transposed into
+// [cols][dst_ld]; zeros behind.  target: NULL, or rows whose target is `ignore` become zeros (their values may be anything).
+struct CopyArgs { const void* src; int64_t ld, rows, cols; const int64_t* target; int64_t ignore; void* dst; int64_t dst_ld, blocks; int vec, across; };     // vec: source rows start on 16 bytes
+
+// 16 bytes a thread
+template <typename T> NK_D void pad_block(const CopyArgs& g, int64_t block) {
     constexpr int E = 16 / sizeof(T);
     typedef __attribute__((ext_vector_type(E))) T vec;
-    const int64_t i = (flat_block() * 256 + threadIdx.x) * E;
-    if (i >= rows * dst_ld) return;
-    const int64_t r = i / dst_ld, c = i - r * dst_ld;           // dst_ld is a multiple of E
+    const int64_t i = (block * 256 + threadIdx.x) * E;
+    if (i >= g.rows * g.dst_ld) return;
+    const int64_t r = i / g.dst_ld, c = i - r * g.dst_ld;           // dst_ld is a multiple of E
+    const T* src = (const T*)g.src + r * g.ld + c;
     vec v;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = (T)0.0f;
-    if (!(factor && factor[r] == 0.0f)) {
-        if (VEC && c + E <= cols) v = *(const vec*)(src + r * ld + c);
+    if (!(g.target && g.target[r] == g.ignore)) {
+        if (g.vec && c + E <= g.cols) v = *(const vec*)src;
         else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) if (c + e < cols) v[e] = src[r * ld + c + e];
+            for (int e = 0; e < E; ++e) if (c + e < g.cols) v[e] = src[e];
         }
     }
-    *(vec*)(dst + i) = v;
+    *(vec*)((T*)g.dst + i) = v;
 }
 
-// dst[c][0 .. dst_ld) = src[0 .. rows)[c], zeros behind; rows with factor c = 0 are left out as zeros (their
-// values may be anything)
-template <typename T, bool VEC>       // VEC: source rows start on 16 bytes
-__global__ __launch_bounds__(256) void k_xent_transpose(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
-                                                        const float* __restrict__ factor, T* __restrict__ dst, int64_t dst_ld) {
+// 64 x 64; `across` blocks cover dst_ld
+template <typename T> NK_D void transpose_block(const CopyArgs& g, int64_t block) {
     constexpr int E = 16 / sizeof(T), CH = 64 / E, LD = 64 + 4 / sizeof(T);     // elements per 16 bytes, such pieces per row
     typedef __attribute__((ext_vector_type(E))) T vec;
     __shared__ T tile[64 * LD];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+    const int64_t r0 = (block % g.across) * 64, c0 = (block / g.across) * 64;
 #pragma unroll
     for (int q = threadIdx.x; q < 64 * CH; q += 256) {
         const int k = q / CH, x = (q % CH) * E;
         const int64_t r = r0 + k, c = c0 + x;
+        const T* src = (const T*)g.src + r * g.ld + c;
         vec v;
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = (T)0.0f;
-        if (r < rows && !(factor && factor[r] == 0.0f)) {
-            if (VEC && c + E <= cols) v = *(const vec*)(src + r * ld + c);
+        if (r < g.rows && !(g.target && g.target[r] == g.ignore)) {
+            if (g.vec && c + E <= g.cols) v = *(const vec*)src;
             else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) if (c + e < cols) v[e] = src[r * ld + c + e];
+                for (int e = 0; e < E; ++e) if (c + e < g.cols) v[e] = src[e];
             }
         }
 #pragma unroll
@@ -731,13 +760,27 @@ __global__ __launch_bounds__(256) void k_xent_transpose(const T* __restrict__ sr
     for (int q = threadIdx.x; q < 64 * CH; q += 256) {
         const int x = q / CH, k = (q % CH) * E;         // column of the source, first row of the piece
         const int64_t c = c0 + x, r = r0 + k;
-        if (c < cols && r < dst_ld) {                   // dst_ld is a multiple of E
+        if (c < g.cols && r < g.dst_ld) {               // dst_ld is a multiple of E
             vec v;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = tile[(k + e) * LD + x];
-            *(vec*)(dst + c * dst_ld + r) = v;
+            *(vec*)((T*)g.dst + c * g.dst_ld + r) = v;
         }
     }
+}
+template <typename T> __global__ __launch_bounds__(256) void k_xent_pad(const CopyArgs g) { pad_block<T>(g, flat_block()); }
+template <typename T> __global__ __launch_bounds__(256) void k_xent_transpose(const CopyArgs g) {
+    const int64_t block = flat_block();
+    if (block < g.blocks) transpose_block<T>(g, block);
+}
+
+// What the backward pass of a few tokens starts with, in one launch: the factors (workgroup 0) and the copies that the type
+// needs (fp32: both transposed; 16 bits: hidden).
+template <typename T> __global__ __launch_bounds__(256) void k_xent_prepare(const FactorArgs f, const CopyArgs a, const CopyArgs b) {
+    const int64_t block = (int64_t)blockIdx.x - 1;
+    if (block < 0) factors<256>(f, 0, 1);
+    else if (block < a.blocks) { if (BOTH_ORDERS<T>) transpose_block<T>(a, block); else pad_block<T>(a, block); }
+    else if (BOTH_ORDERS<T>) transpose_block<T>(b, block - a.blocks);
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -750,12 +793,16 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
 
-template <auto K, typename ARGS>
-int start(const ARGS& args, int64_t blocks, int slices, int threads, hipStream_t st, const char* name) {
-    if (blocks * threads > 0xFFFFFFFFll) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: too many tiles", name);
-    hipLaunchKernelGGL(K, dim3((unsigned)blocks, (unsigned)slices), dim3(threads), 0, st, args);
+template <auto K, typename... ARGS>
+int start(dim3 grid, int threads, hipStream_t st, const char* name, const ARGS&... args) {
+    hipLaunchKernelGGL(K, grid, dim3(threads), 0, st, args...);
     NK_CHECK_LAUNCH(name);
     return NK_OK;
+}
+template <auto K, typename... ARGS>
+int start(int64_t blocks, int threads, hipStream_t st, const char* name, const ARGS&... args) {
+    if (blocks * threads > 0xFFFFFFFFll) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+    return start<K>(dim3((unsigned)blocks), threads, st, name, args...);
 }
 
 // Which tile for an M x N product cut into `slices` stretches of k: the largest that still fills the 256 CUs.
@@ -853,13 +900,15 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
 
 template <typename T, class C> int lse_start(const LseArgs& g, hipStream_t st) {
     const int64_t tiles = cdiv(g.w.rows, C::BM) * cdiv(g.N, C::BN), fit = 256 * (163840 / (C::LDS + C::WGM * C::BN * 8));     // resident workgroups
-    return start<k_xent_lse<T, C>>(g, tiles < fit ? tiles : fit, 1, C::THREADS, st, "k_xent_lse");
+    return start<k_xent_lse<T, C>>(tiles < fit ? tiles : fit, C::THREADS, st, "k_xent_lse", g);
 }
 template <typename T, class C> int dz_start(const DzArgs& g, hipStream_t st) {
-    return start<k_xent_dz<T, C>>(g, cdiv(g.w.rows, C::BM) * cdiv(BOTH_ORDERS<T> ? g.dzt_ld : g.N, C::BN), 1, C::THREADS, st, "k_xent_dz");
+    return start<k_xent_dz<T, C>>(cdiv(g.w.rows, C::BM) * cdiv(BOTH_ORDERS<T> ? g.dzt_ld : g.N, C::BN), C::THREADS, st, "k_xent_dz", g);
 }
 template <typename T, class C, bool SUMS, bool KA, bool KB> int product_start(const ProductArgs& g, int slices, hipStream_t st) {
-    return start<k_xent_product<T, C, SUMS, KA, KB>>(g, cdiv(g.M, C::BM) * cdiv(g.N, C::BN), slices, C::THREADS, st, "k_xent_product");
+    const int64_t tiles = cdiv(g.M, C::BM) * cdiv(g.N, C::BN);
+    if (tiles * C::THREADS > 0xFFFFFFFFll) NK_FAIL(NK_ERR_UNSUPPORTED, "k_xent_product: too many tiles");
+    return start<k_xent_product<T, C, SUMS, KA, KB>>(dim3((unsigned)tiles, (unsigned)slices), C::THREADS, st, "k_xent_product", g);
 }
 template <typename T> int lse_launch(int kind, const LseArgs& g, hipStream_t st) {
     return kind == LARGE ? lse_start<T, Large>(g, st) : kind == MIDDLE ? lse_start<T, Middle>(g, st) : kind == FEW ? lse_start<T, Few>(g, st)
@@ -875,31 +924,36 @@ template <typename T, bool SUMS, bool KA, bool KB> int product_launch(const Prod
          : kind == FEW ? product_start<T, Few, SUMS, KA, KB>(g, slices, st) : product_start<T, Small, SUMS, KA, KB>(g, slices, st);
 }
 
-template <typename T> int pad(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* factor, void* dst, int64_t dst_ld, hipStream_t st) {
-    const dim3 grid = flat_grid(cdiv(rows * dst_ld, 256 * (16 / (int64_t)sizeof(T))));
-    if (((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0)
-        hipLaunchKernelGGL((k_xent_pad<T, true>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
-    else
-        hipLaunchKernelGGL((k_xent_pad<T, false>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
+template <typename T, bool SUMS> int pair_start(const PairArgs& g, hipStream_t st) {
+    auto tiles = [](const ProductArgs& p) { return cdiv(p.M, Small::BM) * cdiv(p.N, Small::BN); };        // some hundreds: SMALL
+    const int64_t x = tiles(g.p[0]) > tiles(g.p[1]) ? tiles(g.p[0]) : tiles(g.p[1]);
+    const int y = g.p[0].slices > g.p[1].slices ? g.p[0].slices : g.p[1].slices;
+    return start<k_xent_pair<T, Small, SUMS>>(dim3((unsigned)x, (unsigned)y, 2), Small::THREADS, st, "k_xent_pair", g);
+}
+
+template <typename T> CopyArgs pad_of(const void* src, int64_t ld, int64_t rows, int64_t cols, const int64_t* target, int64_t ignore, void* dst, int64_t dst_ld) {
+    return CopyArgs{src, ld, rows, cols, target, ignore, dst, dst_ld, cdiv(rows * dst_ld, 256 * (16 / (int64_t)sizeof(T))), ((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0, 0};
+}
+template <typename T> CopyArgs transpose_of(const void* src, int64_t ld, int64_t rows, int64_t cols, const int64_t* target, int64_t ignore, void* dst, int64_t dst_ld) {
+    const int64_t across = cdiv(dst_ld, 64);
+    return CopyArgs{src, ld, rows, cols, target, ignore, dst, dst_ld, across * cdiv(cols, 64), ((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0, (int)across};
+}
+template <typename T> int pad(const CopyArgs& g, hipStream_t st) {
+    hipLaunchKernelGGL(k_xent_pad<T>, flat_grid(g.blocks), dim3(256), 0, st, g);
     NK_CHECK_LAUNCH("k_xent_pad");
     return NK_OK;
 }
-template <typename T> int transpose(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* factor, void* dst, int64_t dst_ld, hipStream_t st) {
-    const dim3 grid((unsigned)cdiv(dst_ld, 64), (unsigned)cdiv(cols, 64));
-    if (((uintptr_t)src & 15) == 0 && ld * sizeof(T) % 16 == 0)
-        hipLaunchKernelGGL((k_xent_transpose<T, true>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
-    else
-        hipLaunchKernelGGL((k_xent_transpose<T, false>), grid, dim3(256), 0, st, (const T*)src, ld, rows, cols, factor, (T*)dst, dst_ld);
+template <typename T> int transpose(const CopyArgs& g, hipStream_t st) {
+    hipLaunchKernelGGL(k_xent_transpose<T>, flat_grid(g.blocks), dim3(256), 0, st, g);
     NK_CHECK_LAUNCH("k_xent_transpose");
     return NK_OK;
 }
-
-template <typename T>
-int finish(const float* sums, int slices, int64_t rows, int64_t D, const float* c, const float* rest, float scale, void* out, hipStream_t st) {
-    if (D % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0)
-        hipLaunchKernelGGL((k_xent_finish<T, 4>), flat_grid(cdiv(rows * D, 1024)), dim3(256), 0, st, sums, slices, rows, D, c, rest, scale, (T*)out);
-    else
-        hipLaunchKernelGGL((k_xent_finish<T, 1>), flat_grid(cdiv(rows * D, 256)), dim3(256), 0, st, sums, slices, rows, D, c, rest, scale, (T*)out);
+template <typename T> FinishArgs finish_of(const float* sums, int slices, int64_t rows, int64_t D, const float* c, const float* rest, void* out) {
+    const int vec = D % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
+    return FinishArgs{sums, slices, vec, rows, D, c, rest, 1.0f / Op<T>::SCALE, out, cdiv(rows * D, vec ? 1024 : 256)};
+}
+template <typename T> int finish(const FinishArgs& a, const FinishArgs& b, hipStream_t st) {
+    hipLaunchKernelGGL(k_xent_finish<T>, flat_grid(a.blocks + b.blocks), dim3(256), 0, st, a, b);
     NK_CHECK_LAUNCH("k_xent_finish");
     return NK_OK;
 }
@@ -911,7 +965,7 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
     int rc;
     Mat h = {(const char*)hidden, o->N, o->hidden_stride * es, o->D * es};
     if (p.copy_h) {
-        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, nullptr, ws + p.h, p.Dp, st)) < 0) return rc;
+        if ((rc = pad<T>(pad_of<T>(hidden, o->hidden_stride, o->N, o->D, nullptr, 0, ws + p.h, p.Dp), st)) < 0) return rc;
         h = Mat{ws + p.h, o->N, p.Dp * es, p.Dp * es};
     }
     int64_t tiles = 0;
@@ -920,7 +974,7 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
         const char* src = (const char*)weight + v0 * o->weight_stride * es;
         Mat w = {src, rows, o->weight_stride * es, o->D * es};
         if (p.pad_w) {
-            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.w, p.Dp, st)) < 0) return rc;
+            if ((rc = pad<T>(pad_of<T>(src, o->weight_stride, rows, o->D, nullptr, 0, ws + p.w, p.Dp), st)) < 0) return rc;
             w = Mat{ws + p.w, rows, p.Dp * es, p.Dp * es};
         }
         const LseArgs g = {w, h, o->D * es, v0, o->V, o->N, target, (float2*)(ws + p.parts), tiles, (float*)(ws + p.zt)};
@@ -957,71 +1011,87 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
     float* c = (float*)(ws + p.c);
     float* rest = (float*)(ws + p.rest);
     int rc;
-    const int groups = (int)cdiv(o->N, TALLY_TOKENS);
-    Tally* parts = groups > 2 ? (Tally*)(ws + p.tally) : nullptr;       // up to two: less than another launch
-    if (parts) {
-        hipLaunchKernelGGL(k_xent_tally, dim3(groups), dim3(1024), 0, st, target, o->N, o->ignore_index, o->reduction, d_loss, parts);
-        NK_CHECK_LAUNCH("k_xent_tally");
-    }
-    hipLaunchKernelGGL(k_xent_factors, dim3(parts ? groups : 1), dim3(1024), 0, st, target, o->N, o->V, o->ignore_index, o->reduction, d_loss, parts,
-                       groups, c, rest);
-    NK_CHECK_LAUNCH("k_xent_factors");
-    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es, o->D * es};
     constexpr bool BOTH = BOTH_ORDERS<T>;
-    if (p.copy_h && (p.pad_h || d_weight)) {
-        if ((rc = pad<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.h, p.Dp, st)) < 0) return rc;
+    Mat h = {(const char*)hidden, o->N, o->hidden_stride * es, o->D * es};
+    const bool one = p.piece >= o->V, copy_h = p.copy_h && (p.pad_h || d_weight);
+    FactorArgs f = {target, o->N, o->V, o->ignore_index, o->reduction, (int)cdiv(o->N, TALLY_TOKENS), d_loss, nullptr, c, rest};
+    const CopyArgs clean = pad_of<T>(hidden, o->hidden_stride, o->N, o->D, target, o->ignore_index, ws + p.h, p.Dp);
+    const CopyArgs ht = transpose_of<T>(hidden, o->hidden_stride, o->N, o->D, target, o->ignore_index, ws + p.ht, p.Np);
+    const bool few = o->N <= 2048 && (BOTH ? one && d_weight && d_hidden : copy_h);        // factors and copies in one launch
+    if (few) {
+        CopyArgs wt = {};
+        if (BOTH) wt = transpose_of<T>(weight, o->weight_stride, o->V, o->D, nullptr, 0, ws + p.wt, up(o->V, 128 / es));
+        const CopyArgs& a = BOTH ? ht : clean;
+        if ((rc = start<k_xent_prepare<T>>(1 + a.blocks + wt.blocks, 256, st, "k_xent_prepare", f, a, wt)) < 0) return rc;
+    } else {
+        if (f.n_parts > 2) {                // up to two: less than another launch
+            f.parts = (const Tally*)(ws + p.tally);
+            hipLaunchKernelGGL(k_xent_tally, dim3(f.n_parts), dim3(1024), 0, st, target, o->N, o->ignore_index, o->reduction, d_loss, (Tally*)(ws + p.tally));
+            NK_CHECK_LAUNCH("k_xent_tally");
+        }
+        hipLaunchKernelGGL(k_xent_factors, dim3(f.parts ? f.n_parts : 1), dim3(1024), 0, st, f);
+        NK_CHECK_LAUNCH("k_xent_factors");
+    }
+    if (copy_h) {
+        if ((!few || BOTH) && (rc = pad<T>(clean, st)) < 0) return rc;
         h = Mat{ws + p.h, o->N, p.Dp * es, p.Dp * es};
     }
-    if (BOTH && d_weight && (rc = transpose<T>(hidden, o->hidden_stride, o->N, o->D, c, ws + p.ht, p.Np, st)) < 0) return rc;
+    if (BOTH && d_weight && !few && (rc = transpose<T>(ht, st)) < 0) return rc;
     const int64_t slice = up(cdiv(p.piece, p.slices), 128 / es) * es;
-    const bool direct = p.slices == 1 && p.piece >= o->V;      // d_hidden in one product: no sums to keep
+    const bool direct = p.slices == 1 && one;      // d_hidden in one product: no sums to keep
     for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
         const int64_t rows = o->V - v0 < p.piece ? o->V - v0 : p.piece;
         const char* src = (const char*)weight + v0 * o->weight_stride * es;
         Mat w = {src, rows, o->weight_stride * es, o->D * es};
         if (p.pad_w) {
-            if ((rc = pad<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.w, p.Dp, st)) < 0) return rc;
+            if ((rc = pad<T>(pad_of<T>(src, o->weight_stride, rows, o->D, nullptr, 0, ws + p.w, p.Dp), st)) < 0) return rc;
             w = Mat{ws + p.w, rows, p.Dp * es, p.Dp * es};
         }
         const int64_t kv = up(rows, 128 / es);          // columns of dz that the product takes: zeros behind `rows`
         const DzArgs g = {w, h, o->D * es, v0, o->N, target, lse, c, ws + p.dz, kv, ws + p.dzt, p.Np};
         if ((rc = dz_launch<T>(tile_kind(rows, o->N), g, st)) < 0) return rc;
+        ProductArgs qw = {}, qh = {};
+        char* out_w = (char*)d_weight + v0 * o->D * es;
+        const int cut = d_weight ? (int)cut_of(o->D, rows, p.Np, 128 / es) : 1;
         if (d_weight) {
-            ProductArgs q = {};
-            if (BOTH) { q.a = Mat{ws + p.ht, o->D, p.Np * es, 0}; q.b = Mat{ws + p.dzt, rows, p.Np * es, 0}; }
-            else { q.a = h; q.b = Mat{ws + p.dz, o->N, kv * es, kv * es}; }
-            q.kbytes = q.kslice = p.Np * es; q.M = o->D; q.N = rows;
-            char* out = (char*)d_weight + v0 * o->D * es;
-            const int cut = (int)cut_of(o->D, rows, p.Np, 128 / es);
-            if (cut == 1) {
-                q.out = out; q.ld = o->D; q.rest = rest; q.scale = unscale;
-                if ((rc = product_launch<T, false, !BOTH, !BOTH>(q, 1, st)) < 0) return rc;
+            if (BOTH) { qw.a = Mat{ws + p.ht, o->D, p.Np * es, 0}; qw.b = Mat{ws + p.dzt, rows, p.Np * es, 0}; }
+            else { qw.a = h; qw.b = Mat{ws + p.dz, o->N, kv * es, kv * es}; }
+            qw.kbytes = qw.kslice = p.Np * es; qw.M = o->D; qw.N = rows; qw.slices = cut;
+            if (cut == 1) { qw.out = out_w; qw.ld = o->D; qw.rest = rest; qw.scale = unscale; }
+            else { qw.kslice = up(cdiv(p.Np, cut), 128 / es) * es; qw.sums = (float*)(ws + p.wsums); }
+        }
+        if (d_hidden) {
+            if (BOTH) {
+                if (!few && (rc = transpose<T>(transpose_of<T>(src, o->weight_stride, rows, o->D, nullptr, 0, ws + p.wt, kv), st)) < 0) return rc;
+                qh.a = Mat{ws + p.wt, o->D, kv * es, 0};
             } else {
-                q.kslice = up(cdiv(p.Np, cut), 128 / es) * es; q.sums = (float*)(ws + p.wsums);
-                if ((rc = product_launch<T, true, !BOTH, !BOTH>(q, cut, st)) < 0) return rc;
-                if ((rc = finish<T>(q.sums, cut, rows, o->D, nullptr, rest, unscale, out, st)) < 0) return rc;
+                qh.a = w;
+            }
+            qh.b = Mat{ws + p.dz, o->N, kv * es, kv * es};
+            qh.kbytes = kv * es; qh.kslice = slice; qh.M = o->D; qh.N = o->N; qh.slices = p.slices;
+            if (direct) { qh.out = d_hidden; qh.ld = o->D; qh.rest = rest; qh.scale = unscale; qh.row_on = c; }
+            else { qh.sums = (float*)(ws + p.sums); qh.add = v0 > 0; }
+        }
+        if (d_weight && d_hidden && one && direct == (cut == 1) && tile_kind(o->D, rows, cut) == SMALL && tile_kind(o->D, o->N, p.slices) == SMALL) {
+            const PairArgs pair = {{qw, qh}};
+            if (direct) return pair_start<T, false>(pair, st);
+            if ((rc = pair_start<T, true>(pair, st)) < 0) return rc;
+            return finish<T>(finish_of<T>(qw.sums, cut, rows, o->D, nullptr, rest, out_w), finish_of<T>(qh.sums, p.slices, o->N, o->D, c, rest, d_hidden), st);
+        }
+        if (d_weight) {
+            if (cut == 1) {
+                if ((rc = product_launch<T, false, !BOTH, !BOTH>(qw, 1, st)) < 0) return rc;
+            } else {
+                if ((rc = product_launch<T, true, !BOTH, !BOTH>(qw, cut, st)) < 0) return rc;
+                if ((rc = finish<T>(finish_of<T>(qw.sums, cut, rows, o->D, nullptr, rest, out_w), FinishArgs{}, st)) < 0) return rc;
             }
         }
         if (d_hidden) {
-            ProductArgs q = {};
-            if (BOTH) {
-                if ((rc = transpose<T>(src, o->weight_stride, rows, o->D, nullptr, ws + p.wt, kv, st)) < 0) return rc;
-                q.a = Mat{ws + p.wt, o->D, kv * es, 0};
-            } else {
-                q.a = w;
-            }
-            q.b = Mat{ws + p.dz, o->N, kv * es, kv * es};
-            q.kbytes = kv * es; q.kslice = slice; q.M = o->D; q.N = o->N;
-            if (direct) {
-                q.out = d_hidden; q.ld = o->D; q.rest = rest; q.scale = unscale; q.row_on = c;
-                if ((rc = product_launch<T, false, !BOTH, false>(q, 1, st)) < 0) return rc;
-            } else {
-                q.sums = (float*)(ws + p.sums); q.add = v0 > 0;
-                if ((rc = product_launch<T, true, !BOTH, false>(q, p.slices, st)) < 0) return rc;
-            }
+            if (direct) { if ((rc = product_launch<T, false, !BOTH, false>(qh, 1, st)) < 0) return rc; }
+            else if ((rc = product_launch<T, true, !BOTH, false>(qh, p.slices, st)) < 0) return rc;
         }
     }
-    if (d_hidden && !direct && (rc = finish<T>((const float*)(ws + p.sums), p.slices, o->N, o->D, c, rest, unscale, d_hidden, st)) < 0) return rc;
+    if (d_hidden && !direct) return finish<T>(finish_of<T>((const float*)(ws + p.sums), p.slices, o->N, o->D, c, rest, d_hidden), FinishArgs{}, st);
     return NK_OK;
 }
 

@@ -26,6 +26,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of `t`'s shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _opts(a, x, g, lengths, reverse) -> "_lib.NkScanOpts":
     B, T, C = x.shape
     ab, at, _ = a.stride()
@@ -48,7 +53,7 @@ def _forward(a, x, h0, lengths, reverse, training):
     dev = x.device
     if B == 0 or T == 0:        # no step: the state passes through
         return x.new_empty(B, T, C), (h0.clone() if h0 is not None else torch.zeros(B, C, dtype=torch.float32, device=dev)), None
-    h = torch.empty_like(x) if x.is_contiguous() else torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    h = _like(x)
     last = torch.empty_like(h0) if h0 is not None else torch.empty((B, C), dtype=torch.float32, device=dev)
     o = _opts(a, x, None, lengths, reverse)
     states = torch.empty(B * (-(-T // _KEEP)) * C, dtype=torch.float32, device=dev) if training else None
@@ -87,9 +92,9 @@ class _GatedScan(torch.autograd.Function):
         L = _lib.load()
         g = _rows(d_h) if d_h is not None else None
         o = _opts(a, x, g, lengths, ctx.reverse)
-        d_a = torch.empty(a.shape, dtype=a.dtype, device=dev) if want_a else None
-        d_x = torch.empty((B, T, C), dtype=x.dtype, device=dev) if want_x else None
-        d_0 = torch.empty((B, C), dtype=torch.float32, device=dev) if want_0 else None
+        d_a = _like(a) if want_a else None
+        d_x = _like(x) if want_x else None
+        d_0 = torch.empty_like(h0) if want_0 else None
         ws, n = _workspace(L, o, 1, dev)
         _lib.launch(dev, L.nk_gated_scan_bwd, o, a.data_ptr(), x.data_ptr(), _ptr(states), _ptr(h0), _ptr(g), _ptr(d_last),
                     _ptr(d_a), _ptr(d_x), _ptr(d_0), _ptr(ws), n)

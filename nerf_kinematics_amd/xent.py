@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _ptr
+from .scan import _like, _ptr
 
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
@@ -32,12 +32,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _forward(hidden, weight, target, o, reduction):
     L = _lib.load()
     N, dev = hidden.shape[0], hidden.device
-    loss, lse = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
-    total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     ws, n = _workspace(L, o, hidden, weight, 0)
-    _lib.launch(dev, L.nk_linear_xent_fwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), loss.data_ptr(),
-                lse.data_ptr(), _ptr(total), ws.data_ptr(), n)
-    return (loss if total is None else total), lse
+    if reduction:       # the losses of the tokens, which nobody asked for, lie behind lse
+        lse, out = torch.empty(2 * N, dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+        loss, reduced = lse.data_ptr() + 4 * N, out.data_ptr()
+    else:
+        lse, out = torch.empty(N, dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
+        loss, reduced = out.data_ptr(), None
+    _lib.launch(dev, L.nk_linear_xent_fwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), loss, lse.data_ptr(), reduced,
+                ws.data_ptr(), n)
+    return out, lse
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -55,10 +59,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         hidden, weight, target, lse = ctx.saved_tensors
         dev = hidden.device
         want_h, want_w = ctx.needs_input_grad[:2]
-        d_hidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
+        d_hidden = _like(hidden) if want_h else None
         if hidden.shape[0] == 0:
             return d_hidden, torch.zeros_like(weight) if want_w else None, None, None, None, None
-        d_weight = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
+        d_weight = _like(weight) if want_w else None
         d_loss = d_loss.contiguous()
         L = _lib.load()
         ws, n = _workspace(L, ctx.opts, hidden, weight, 1)
@@ -87,7 +91,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     N, D = hidden.shape
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != D or weight.shape[0] < 1 or weight.dtype != hidden.dtype:
         raise ValueError(f"weight: expected a [V, {D}] tensor of {hidden.dtype}")
-    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64 or tuple(target.shape) != (N,):
+    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64 or target.shape != (N,):
         raise ValueError(f"target: expected an int64 tensor of shape {(N,)}")
     if piece < 0:
         raise ValueError(f"piece={piece} (>= 0)")

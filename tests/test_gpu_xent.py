@@ -213,6 +213,18 @@ def test_single_rows_of_any_stride():
 
 
 @gpu
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_the_loss_may_be_changed_in_place(reduction):
+    import nerf_kinematics_amd as nk
+    h, w, t, _ = make(40, 24, 50, F32, 16)
+    a, b = h.clone().requires_grad_(True), h.clone().requires_grad_(True)
+    x, y = nk.linear_cross_entropy(a, w, t, reduction=reduction), nk.linear_cross_entropy(b, w, t, reduction=reduction)
+    x *= 2.0
+    (got,), (want,) = torch.autograd.grad(x.sum(), a), torch.autograd.grad((y * 2.0).sum(), b)
+    assert torch.equal(got, want) and bool(got.any())
+
+
+@gpu
 def test_only_one_gradient():
     import nerf_kinematics_amd as nk
     h, w, t, g = make(100, 64, 500, BF16, 9)
