@@ -15,8 +15,8 @@
 // is written in both orders by the tile that computes it.
 //
 // What bounds it (MI355X; a library product of 8192^3 reaches 1 383 TFLOP/s in bf16): the matrix units at the clock that
-// power leaves them, 2.1 GHz.  8192 x 2048 x 65536 in bf16, forward and backward: 7.0 ms, 1 257 TFLOP/s over the four
-// products (the logits twice); forward alone 1.72 ms.  4096 x 1024 x 32003: 0.99 ms, the epilogue of dz costs more
+// power leaves them, 2.1 GHz.  8192 x 2048 x 65536 in bf16, forward and backward: 7.0 to 7.3 ms from card to card, 1 204 to
+// 1 257 TFLOP/s over the four products (the logits twice); forward alone 1.75 ms.  4096 x 1024 x 32003: 1.0 ms, the epilogue of dz costs more
 // where k is short.  16 x 1024 x 50000 forward: 24 us, 4.3 TB/s of weight.  Small calls: launches.
 #include "nk_common.h"
 
@@ -58,7 +58,8 @@ template <> struct Op<float> {
 };
 
 // ---- the tile product -------------------------------------------------------------------------
-// A workgroup computes BM x BN of C with WGM x WGN wavefronts, each TM x TN tiles of 16 x 16.  k advances
+// A workgroup computes BM x BN of C with WGM x WGN wavefronts, each TM x TN tiles of 16 x 16 (with 32 x 32 x 16
+// instructions the largest products take 6 % longer: half as many independent sums).  k advances
 // by 128 bytes of every row; the rows of a step are loaded straight into LDS (16 bytes a lane, 8 rows a
 // wavefront and instruction) STAGES - 1 steps ahead.  Row r keeps its eight 16-byte chunks in the order
 // chunk ^ (r & 7), so that the 16 rows a fragment read touches fall on different banks; the order is made by the
