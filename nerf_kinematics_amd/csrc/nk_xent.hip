@@ -15,8 +15,9 @@
 // is written in both orders by the tile that computes it.
 //
 // What bounds it (MI355X; a library product of 8192^3 reaches 1 383 TFLOP/s in bf16): power and the way to memory.  The
-// matrix units are 55 % busy at 2.1 GHz, LDS 21 %; over data that stays in the caches the loop is a quarter faster.  8192 x 2048 x 65536 in bf16, forward and backward: 7.0 to 7.3 ms from card to card, 1 204 to
-// 1 257 TFLOP/s over the four products (the logits twice); forward alone 1.75 ms.  4096 x 1024 x 32003: 1.0 ms, the epilogue of dz costs more
+// matrix units are 55 % busy at 2.1 GHz, LDS 21 %; over data that stays in the caches the loop is a quarter faster.
+// 8192 x 2048 x 65536 in bf16, forward and backward: 7.0 to 7.3 ms from card to card, 1 204 to 1 257 TFLOP/s over the
+// four products (the logits twice); forward alone 1.75 ms.  4096 x 1024 x 32003: 1.0 ms, the epilogue of dz costs more
 // where k is short.  16 x 1024 x 50000 forward: 24 us, 4.3 TB/s of weight.  Small calls: launches.
 #include "nk_common.h"
 
