@@ -133,6 +133,15 @@ def test_types(shape, dt, gdt):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(2, 300, 129, 1), (2, 70, 255, 3), (3, 40, 127, 127), (2, 1100, 2, 1), (1, 2100, 3, 3)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dt,gdt", [(F32, F32), (BF16, F32), (F16, F16)])
+def test_odd_widths(shape, dt, gdt):
+    """Columns of two channels over an odd number of them, gates wider than a wavefront among them."""
+    a, x, h0, lengths, d_h, d_last = inputs(*shape, dt, gdt, 31, True)
+    check(a, x, h0, lengths, True, d_h, d_last)
+
+
+@gpu
 @pytest.mark.parametrize("which", ["sliced", "odd address", "gates shared by sequences", "one gate expanded", "sum", "last only", "h only"])
 def test_layouts(which):
     a, x, h0, _, d_h, d_last = inputs(3, 150, 24, 24, BF16, F32, 3, False)
