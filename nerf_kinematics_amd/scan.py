@@ -31,6 +31,19 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _kinds(tensors) -> list:
+    return [None if t is None else (t.dtype, t.shape, t.device) for t in tensors]
+
+
+def _unpacked(ctx):
+    """The saved tensors.  Saved-tensor hooks may hand them back in another layout (copies of strided ones come back dense), so
+    strides are read from these and not kept from the forward pass; a hook that changes more than that is refused."""
+    tensors = ctx.saved_tensors
+    if _kinds(tensors) != ctx.kinds:
+        raise RuntimeError("a saved-tensor hook returned a tensor of another dtype, shape or device than it was given")
+    return tensors
+
+
 def _opts(a, x, g, lengths, reverse) -> "_lib.NkScanOpts":
     B, T, C = x.shape
     ab, at, _ = a.stride()

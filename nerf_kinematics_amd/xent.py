@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _like, _ptr
+from .scan import _kinds, _like, _ptr, _unpacked
 
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
@@ -47,16 +47,18 @@ def _forward(hidden, weight, target, o, reduction):
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction, piece):
-        o = _opts(hidden, weight, ignore_index, reduction, piece)
-        loss, lse = _forward(hidden, weight, target, o, reduction)
+        ctx.options = ignore_index, reduction, piece
+        loss, lse = _forward(hidden, weight, target, _opts(hidden, weight, *ctx.options), reduction)
         ctx.save_for_backward(hidden, weight, target, lse)
-        ctx.opts = o
+        ctx.kinds = _kinds((hidden, weight, target, lse))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
-        hidden, weight, target, lse = ctx.saved_tensors
+        hidden, weight, target, lse = _unpacked(ctx)
+        hidden, weight, target, lse = _rows(hidden), _rows(weight), target.contiguous(), lse.contiguous()
+        o = _opts(hidden, weight, *ctx.options)
         dev = hidden.device
         want_h, want_w = ctx.needs_input_grad[:2]
         d_hidden = _like(hidden) if want_h else None
@@ -65,8 +67,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         d_weight = _like(weight) if want_w else None
         d_loss = d_loss.contiguous()
         L = _lib.load()
-        ws, n = _workspace(L, ctx.opts, hidden, weight, 1)
-        _lib.launch(dev, L.nk_linear_xent_bwd, ctx.opts, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
+        ws, n = _workspace(L, o, hidden, weight, 1)
+        _lib.launch(dev, L.nk_linear_xent_bwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
                     d_loss.data_ptr(), _ptr(d_hidden), _ptr(d_weight), ws.data_ptr(), n)
         return d_hidden, d_weight, None, None, None, None
 
