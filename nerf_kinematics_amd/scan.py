@@ -22,6 +22,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if (sc == 1 or t.shape[2] == 1) and sb >= 0 and st >= 0 else t.contiguous()
 
 
+def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -81,6 +85,7 @@ class _GatedScan(torch.autograd.Function):
         # the kept states serve the gates' gradient alone
         h, last, states = _forward(a, x, h0, lengths, reverse, ctx.needs_input_grad[0])
         ctx.save_for_backward(a, x, h0, lengths, states)
+        ctx.kinds = _kinds((a, x, h0, lengths, states))
         ctx.reverse = reverse
         ctx.set_materialize_grads(False)
         return h, last
@@ -88,7 +93,8 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_h, d_last):
-        a, x, h0, lengths, states = ctx.saved_tensors
+        a, x, h0, lengths, states = _unpacked(ctx)
+        a, x, h0, lengths, states = _rows(a), _rows(x), _whole(h0), _whole(lengths), _whole(states)
         want_a, want_x, want_0 = ctx.needs_input_grad[:3]
         B, T, C = x.shape
         dev = x.device

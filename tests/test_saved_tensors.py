@@ -3,7 +3,7 @@
 On the CPU the launch is replaced by a recorder: the addresses and strides that a call would have been made with have to
 describe the values that were saved, inside the memory that the hook gave.  On the GPU the gradients have to be the same bits as
 without hooks: the same values in the same order, whatever the rows' distance."""
-import ctypes as C
+import ctypes
 
 import pytest
 import torch
@@ -42,7 +42,7 @@ def reading(address, shape, strides):
         for n, s in zip(reversed(shape[:-1]), reversed(strides)):
             at += 4 * (k % n) * s
             k //= n
-        rows[i] = torch.tensor((C.c_float * shape[-1]).from_address(at)[:])
+        rows[i] = torch.tensor((ctypes.c_float * shape[-1]).from_address(at)[:])
     return out
 
 
@@ -73,7 +73,7 @@ def test_cross_entropy_values_behind_the_addresses(monkeypatch):
     target, seen = torch.arange(18)[::2] % 7, []
 
     def launch(dev, fn, o, h, w, t, *rest):
-        seen.append((reading(h, (o.N, o.D), (o.hidden_stride,)), reading(w, (o.V, o.D), (o.weight_stride,)), (C.c_int64 * o.N).from_address(t)[:]))
+        seen.append((reading(h, (o.N, o.D), (o.hidden_stride,)), reading(w, (o.V, o.D), (o.weight_stride,)), (ctypes.c_int64 * o.N).from_address(t)[:]))
     monkeypatch.setattr(lib, "launch", launch)
     for hook in sorted(HOOKS):
         del seen[:]
@@ -97,6 +97,46 @@ def test_cross_entropy_refuses_other_tensors(calls):
     assert all(c[0] == "nk_linear_xent_fwd" for c in calls)
 
 
+def test_scan_values_behind_the_addresses(monkeypatch):
+    from nerf_kinematics_amd import lib
+    from nerf_kinematics_amd.scan import _GatedScan
+    B, T, C, J = 3, 5, 8, 4
+    a, x, h0 = torch.rand(B, T, J, requires_grad=True), torch.randn(B, 2 * T, C)[:, ::2].requires_grad_(True), torch.randn(B, C, requires_grad=True)
+    lengths, seen = torch.tensor([5, 0, 3], dtype=torch.int32), []
+    kept = torch.arange(float(B * C))           # states [B][1][C]
+
+    def launch(dev, fn, o, *args):
+        pa, px = args[:2]
+        p0 = args[2] if fn.__name__ == "nk_gated_scan_fwd" else args[3]
+        seen.append((reading(pa, (B, T, J), (o.a_stride_b, o.a_stride_t)), reading(px, (B, T, C), (o.x_stride_b, o.x_stride_t)),
+                     reading(p0, (B, C), (C,)), (ctypes.c_int32 * B).from_address(o.lengths)[:]))
+        if fn.__name__ == "nk_gated_scan_fwd":
+            ctypes.memmove(args[5], kept.data_ptr(), 4 * B * C)
+        else:
+            seen.append(reading(args[2], (B * C,), ()))
+    monkeypatch.setattr(lib, "launch", launch)
+    for hook in sorted(HOOKS):
+        del seen[:]
+        with HOOKS[hook]():
+            h, last = _GatedScan.apply(a, x, h0, lengths, 0)
+        torch.autograd.grad((h, last), (a, x, h0), (torch.ones_like(h), torch.ones_like(last)))
+        assert len(seen) == 3
+        for pa, px, p0, n in seen[:2]:
+            assert torch.equal(pa, a.detach()) and torch.equal(px, x.detach()) and torch.equal(p0, h0.detach()) and n == lengths.tolist(), hook
+        assert torch.equal(seen[2], kept)
+
+
+def test_scan_refuses_other_tensors(calls):
+    from nerf_kinematics_amd.scan import _GatedScan
+    a, x, h0 = torch.rand(3, 5, 4, requires_grad=True), torch.randn(3, 5, 8, requires_grad=True), torch.randn(3, 8, requires_grad=True)
+    for change in (lambda t: t[:2], lambda t: t.half(), lambda t: t.bfloat16() if t.shape == x.shape else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            h, last = _GatedScan.apply(a, x, h0, None, 0)
+        with pytest.raises(RuntimeError, match="saved"):
+            torch.autograd.grad(h, (a, x, h0), torch.ones_like(h))
+    assert all(c[0] == "nk_gated_scan_fwd" for c in calls)
+
+
 @gpu
 @pytest.mark.parametrize("hook", sorted(GPU_HOOKS))
 @pytest.mark.parametrize("dt", [F32, BF16])
@@ -118,3 +158,25 @@ def test_cross_entropy_gradients_under_hooks(dt, hook):
         a, b, loss = run()
     got = torch.autograd.grad(loss, (a, b), d)
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and bool(want[0].any())
+
+
+@gpu
+@pytest.mark.parametrize("hook", sorted(GPU_HOOKS))
+@pytest.mark.parametrize("J", [1, 4, 24])
+def test_scan_gradients_under_hooks(J, hook):
+    import nerf_kinematics_amd as nk
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)
+    a0, x0, h0, d, dl = torch.sigmoid(r(3, 200, J)), r(3, 200, 48), r(3, 24), r(3, 200, 24), r(3, 24)
+    lengths = torch.tensor([200, 0, 77], dtype=torch.int32, device=dev)
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (a0, x0, h0)]
+        return leaves, nk.gated_scan(leaves[0], leaves[1][:, :, 24:], leaves[2], lengths=lengths, reverse=True)
+    leaves, out = run()
+    want = torch.autograd.grad(out, leaves, (d, dl))
+    with GPU_HOOKS[hook]():
+        leaves, out = run()
+    got = torch.autograd.grad(out, leaves, (d, dl))
+    assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(bool(p.any()) for p in want)
