@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import lib as _lib
 
@@ -33,6 +34,12 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 def _like(t: torch.Tensor) -> torch.Tensor:
     """An empty contiguous tensor of `t`'s shape, type and device."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses forward-mode tangents: a call that autograd does not see would drop them, and their absence reads as zero."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives are not available here (first-order gradients by backward() are)")
 
 
 def _kinds(tensors) -> list:
@@ -130,7 +137,7 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     from the last step to the first.  ``lengths`` [B] int32 cuts sequence b short: rows behind it are not read and
     ``h`` and all gradients are zero there; values outside 0..T are clamped.
 
-    Differentiable in ``a``, ``x`` and ``h0`` (first order), through both results.  For one step at a time pass T = 1
+    Differentiable in ``a``, ``x`` and ``h0`` (first order, reverse mode), through both results.  For one step at a time pass T = 1
     and the last state as ``h0``.  A training call also keeps the float32 state in front of every 32nd step.
     """
     if not isinstance(x, torch.Tensor) or x.dtype not in _lib.DTYPES or x.dim() != 3:
@@ -141,6 +148,7 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     J = a.shape[2]
     if C < 1 or J < 1 or C % J:
         raise ValueError(f"a: {J} gates for {C} channels (a divisor of them)")
+    _no_tangents(a, x, h0)
     reverse = bool(reverse)
     dev = x.device
     if dev.type != "cuda":

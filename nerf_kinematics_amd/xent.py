@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _kinds, _like, _ptr, _unpacked
+from .scan import _kinds, _like, _no_tangents, _ptr, _unpacked
 
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
@@ -82,7 +82,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     holds; any other target outside 0..V-1 makes its loss and the gradients NaN.  ``reduction`` is "mean" (over the
     tokens that are not ignored; 0 without any), "sum" or "none" ([N] losses).
 
-    Differentiable in ``hidden`` and ``weight`` (first order).  The backward pass walks the vocabulary in pieces
+    Differentiable in ``hidden`` and ``weight`` (first order, reverse mode).  The backward pass walks the vocabulary in pieces
     of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB, 2048 at least) and rounds the logit
     gradients once to the operands' dtype between its products; sums are float32.
     """
@@ -97,6 +97,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         raise ValueError(f"target: expected an int64 tensor of shape {(N,)}")
     if piece < 0:
         raise ValueError(f"piece={piece} (>= 0)")
+    _no_tangents(hidden, weight)
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("hidden: expected a GPU tensor (there is no CPU implementation)")
