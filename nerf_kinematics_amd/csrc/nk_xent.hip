@@ -447,8 +447,8 @@ __global__ __launch_bounds__(1024) void k_xent_reduce(const double2* __restrict_
 // ---- backward ---------------------------------------------------------------------------------
 // Row factors of dz and the factor that is left for the end: the products see dz with |c| <= 1.
 //   mean / sum: c = 1 for tokens that count, rest = d_loss / count or d_loss
-//   none:       c = d_loss_n / rest with rest the power of two above the largest |d_loss|
-struct Tally { int count; uint32_t peak; };     // tokens that count, bits of the largest |d_loss| among them
+//   none:       c = d_loss_n / rest with rest the power of two above the largest finite |d_loss|
+struct Tally { int count; uint32_t peak; };     // tokens that count, bits of the largest finite |d_loss| among them
 enum { TALLY_TOKENS = 4096 };
 
 template <int THREADS> NK_D Tally tally(const int64_t* target, int64_t n0, int64_t n1, int64_t ignore, int reduction, const float* d_loss) {
@@ -457,7 +457,10 @@ template <int THREADS> NK_D Tally tally(const int64_t* target, int64_t n0, int64
     for (int64_t n = n0 + threadIdx.x; n < n1; n += THREADS)
         if (target[n] != ignore) {
             ++r.count;
-            if (reduction == NK_REDUCE_NONE) r.peak = max(r.peak, __float_as_uint(d_loss[n]) & 0x7FFFFFFFu);
+            if (reduction == NK_REDUCE_NONE) {
+                const uint32_t b = __float_as_uint(d_loss[n]) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u) r.peak = max(r.peak, b);       // an infinite one would shrink all others to nothing
+            }
         }
     return r;
 }
