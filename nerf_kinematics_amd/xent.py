@@ -24,9 +24,12 @@ def _workspace(L, o, hidden, weight, backward):
     return torch.empty(n, dtype=torch.uint8, device=hidden.device), n         # torch's blocks are 512-byte aligned
 
 
+_FAR = 1 << 22          # bytes between rows that the library takes
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` with unit stride along its rows, which do not overlap (a copy where they do)."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    """`t` with unit stride along its rows, which neither overlap nor lie further apart than the library takes (a copy where they do)."""
+    return t if t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= _FAR // t.element_size() else t.contiguous()
 
 
 def _forward(hidden, weight, target, o, reduction):

@@ -1,0 +1,42 @@
+"""Limits of the cross entropy's call surface: what the Python call takes and refuses, on the host."""
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_rows_far_apart_are_copied(dt):
+    """Rows up to 2^22 bytes apart are taken as they lie, others are copied: the library addresses 256 of them with 31 bits."""
+    import nerf_kinematics_amd as nk
+    from nerf_kinematics_amd.xent import _opts, _rows
+    L, most = nk.load(), (1 << 22) // dt.itemsize
+    near = torch.empty(2 * most + 16, dtype=dt)
+    for step, copied in ((most, False), (most + 8, True), (2 * most, True)):
+        t = near.as_strided((2, 16), (step, 1))
+        got = _rows(t)
+        assert (got is not t) == copied and got.stride() == ((16, 1) if copied else (step, 1))
+        o = _opts(got, got, -100, 1, 0)
+        for backward in (0, 1):
+            assert L.nk_linear_xent_workspace_bytes(o, got.data_ptr(), got.data_ptr(), backward) > 0
+    wide = torch.empty(1, 1 << 20, dtype=dt).expand(3, -1)          # as wide as rows may be
+    assert L.nk_linear_xent_workspace_bytes(_opts(_rows(wide), _rows(wide), -100, 1, 0), 1024, 1024, 0) > 0
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_last_positions_of_long_sequences(dt):
+    """hidden = states[:, -1]: rows further apart than 2^22 bytes give the same bits as dense ones."""
+    import nerf_kinematics_amd as nk
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(1)
+    states = torch.randn(3, (1 << 22) // (64 * dt.itemsize) + 1, 64, generator=g, device=dev).to(dt)
+    w, t = (torch.randn(500, 64, generator=g, device=dev) / 8).to(dt), torch.tensor([4, -100, 499], device=dev)
+    s, b = states.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = nk.linear_cross_entropy(s[:, -1], b, t)
+    ds, db = torch.autograd.grad(got, (s, b))
+    h, c = states[:, -1].clone().requires_grad_(True), w.clone().requires_grad_(True)
+    want = nk.linear_cross_entropy(h, c, t)
+    dh, dc = torch.autograd.grad(want, (h, c))
+    assert torch.equal(got, want) and torch.equal(ds[:, -1], dh) and torch.equal(db, dc) and not ds[:, :-1].any() and bool(dh[0].any())
