@@ -25,6 +25,7 @@ def _workspace(L, o, hidden, weight, backward):
 
 
 _FAR = 1 << 22          # bytes between rows that the library takes
+_TOKENS32 = 1 << 20     # and tokens of a backward pass in float32
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -88,6 +89,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     Differentiable in ``hidden`` and ``weight`` (first order, reverse mode).  The backward pass walks the vocabulary in pieces
     of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB, 2048 at least) and rounds the logit
     gradients once to the operands' dtype between its products; sums are float32.
+
+    A call takes D up to 2^20, V up to 2^26 and N up to 2^24 (float32 with gradients: 2^20).  Rows of any layout are taken; those that
+    overlap, are strided inside or lie more than 2^22 bytes apart are copied.
     """
     if reduction not in _lib.REDUCTIONS:
         raise ValueError(f"reduction={reduction!r}: expected one of {sorted(_lib.REDUCTIONS)}")
@@ -101,6 +105,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if piece < 0:
         raise ValueError(f"piece={piece} (>= 0)")
     _no_tangents(hidden, weight)
+    training = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+    if training and N > _TOKENS32 and hidden.dtype == torch.float32:
+        raise ValueError(f"hidden: float32 gradients of up to {_TOKENS32} tokens a call, got {N}")
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("hidden: expected a GPU tensor (there is no CPU implementation)")
@@ -108,6 +115,6 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         raise ValueError(f"weight, target: expected tensors on {dev}")
     hidden, weight, target = _rows(hidden), _rows(weight), target.contiguous()
     r = _lib.REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if training:
         return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), r, int(piece))
     return _forward(hidden, weight, target, _opts(hidden, weight, int(ignore_index), r, int(piece)), r)[0]

@@ -40,3 +40,29 @@ def test_last_positions_of_long_sequences(dt):
     want = nk.linear_cross_entropy(h, c, t)
     dh, dc = torch.autograd.grad(want, (h, c))
     assert torch.equal(got, want) and torch.equal(ds[:, -1], dh) and torch.equal(db, dc) and not ds[:, :-1].any() and bool(dh[0].any())
+
+
+def test_too_many_float32_tokens_are_refused_before_the_forward_pass():
+    """float32 gradients: 2^20 tokens a call.  A training call of more is refused where it is made, not in backward(); one
+    without gradients, and 16-bit types, get as far as the question of the device (there is none here)."""
+    import nerf_kinematics_amd as nk
+    N = (1 << 20) + 1
+    h, w, t = torch.zeros(1, 8).expand(N, 8), torch.zeros(5, 8), torch.zeros(1, dtype=torch.int64).expand(N)
+    leaf = lambda x: x.detach().requires_grad_(True)
+    for a, b in ((leaf(h), w), (h, leaf(w)), (leaf(h), leaf(w))):
+        with pytest.raises(ValueError, match="float32 gradients"):
+            nk.linear_cross_entropy(a, b, t)
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            nk.linear_cross_entropy(a, b, t)
+        with pytest.raises(ValueError, match="GPU"):
+            nk.linear_cross_entropy(leaf(a.detach()[1:]), b, t[1:])
+    with pytest.raises(ValueError, match="GPU"):
+        nk.linear_cross_entropy(h, w, t)
+    with pytest.raises(ValueError, match="GPU"):
+        nk.linear_cross_entropy(leaf(h.to(BF16)), w.to(BF16), t)
+    # the limit is the library's
+    from nerf_kinematics_amd.xent import _opts
+    L = nk.load()
+    for n, rc in ((N, -2), (N - 1, 0)):
+        got = L.nk_linear_xent_workspace_bytes(_opts(h[:1].expand(n, 8).contiguous(), w, -100, 1, 0), 1024, 1024, 1)
+        assert (got == rc) if rc else got > 0
