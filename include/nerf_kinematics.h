@@ -265,8 +265,9 @@ typedef struct nk_xent_opts {
     int32_t dtype;                /* NK_F32 | NK_BF16 | NK_F16                                */
     int32_t reduction;            /* NK_REDUCE_*                                              */
     int64_t piece;                /* rows of the vocabulary per piece of the backward call, rounded up to 256;
-                                     0: as many as keep a piece's gradients (N piece elements; fp32 keeps
-                                     them twice) near 256 MB, 2048 at least; 2^22 bytes of them at most */
+                                     0: as many as keep a piece's scratch (its gradients, which fp32 keeps
+                                     twice, and the copies of its rows of weight) near 256 MB, 2048 at
+                                     least; 2^22 bytes of a gradient's row at most                     */
 } nk_xent_opts;
 /* Scratch of a call on these operands (256-byte aligned; it holds nothing between calls). */
 int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int backward);

@@ -25,7 +25,7 @@ namespace {
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-// A piece's dz, unless the caller names a piece.  Kernel time of a training pass of 8192 x 2048 x 65536 /
+// Scratch of a piece (its dz, and the copies of its rows), unless the caller names one.  Kernel time of a training pass of 8192 x 2048 x 65536 /
 // 4096 x 1024 x 32003: 64 MB 8.4 / 1.41 ms, 128 MB 7.75 / 1.25, 256 MB 7.64 / 1.20, 512 MB 7.61 / 1.25.
 enum { XENT_PIECE_MB = 256 };
 
@@ -858,16 +858,17 @@ int plan_of(const nk_xent_opts* o, const void* hidden, const void* weight, int b
     p->pad_h = !aligned(hidden, o->hidden_stride); p->pad_w = !aligned(weight, o->weight_stride);
     p->Np = up(o->N, step);
     const int64_t asked = o->piece < o->V ? up(o->piece, 256) : up(o->V, 256);       // 0: not asked for
-    int64_t piece;
-    if (backward) {
-        piece = asked ? asked : up(((int64_t)XENT_PIECE_MB << 20) / (p->Np > 0 ? p->Np : 1) / es, 256);
-        if (piece < 2048 && !asked) piece = 2048;
-    } else {
-        piece = p->pad_w ? (asked ? asked : 16384) : up(o->V, 256);
-    }
+    const bool both = o->dtype == NK_F32;               // dz in both orders, transposed copies of weight and hidden
+    // bytes of scratch that a row of the piece takes: its dz, and its copies
+    const int64_t row = ((backward ? p->Np * (both ? 2 : 1) + (both ? o->D : 0) : 0) + (p->pad_w ? p->Dp : 0)) * es;
+    int64_t piece = up(((int64_t)XENT_PIECE_MB << 20) / (row > 0 ? row : 1), 256);
+    if (piece < 2048) piece = 2048;
+    // pieces of one length, up to an eighth longer rather than one more: 16384 x 1023 x 32003 in bf16, 4.73 ms with a fifth piece of 259 rows
+    piece = up(cdiv(o->V, cdiv(o->V, piece + piece / 8)), 256);
+    if (!backward) piece = !p->pad_w ? up(o->V, 256) : piece < 16384 ? piece : 16384;
+    if (asked && (backward || p->pad_w)) piece = asked;
     if (piece > (1 << 22) / es) piece = (1 << 22) / es;         // a row of dz: up to 2^22 bytes, as of the other operands
     if (piece > o->V) piece = up(o->V, step);           // the only one
-    const bool both = o->dtype == NK_F32;               // dz in both orders, transposed copies of weight and hidden
     if (backward && both && o->N > (1 << 20)) NK_FAIL(NK_ERR_UNSUPPORTED, "%s: fp32 gradients of up to 2^20 tokens a call", who);
     p->piece = piece;
     int64_t off = 0;

@@ -87,8 +87,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     tokens that are not ignored; 0 without any), "sum" or "none" ([N] losses).
 
     Differentiable in ``hidden`` and ``weight`` (first order, reverse mode).  The backward pass walks the vocabulary in pieces
-    of ``piece`` rows (default: as many as keep a piece's logit gradients near 256 MB, 2048 at least) and rounds the logit
-    gradients once to the operands' dtype between its products; sums are float32.
+    of ``piece`` rows (default: as many as keep a piece's scratch near 256 MB, 2048 at least) and rounds the logit gradients once to
+    the operands' dtype between its products; sums are float32.
 
     A call takes D up to 2^20, V up to 2^26 and N up to 2^24 (float32 with gradients: 2^20).  Rows of any layout are taken; those that
     overlap, are strided inside or lie more than 2^22 bytes apart are copied.

@@ -66,3 +66,25 @@ def test_too_many_float32_tokens_are_refused_before_the_forward_pass():
     for n, rc in ((N, -2), (N - 1, 0)):
         got = L.nk_linear_xent_workspace_bytes(_opts(h[:1].expand(n, 8).contiguous(), w, -100, 1, 0), 1024, 1024, 1)
         assert (got == rc) if rc else got > 0
+
+
+@pytest.mark.parametrize("dt,N,D,V", [(F32, 16, 4096, 131072), (F32, 16, 2048, 65536), (BF16, 16, 4095, 131072), (F16, 3, 8190, 200000), (F32, 1, 1, 1 << 26),
+                                      (F32, 2000, 500, 100000), (F32, 8192, 2048, 65536), (BF16, 8192, 2048, 65536), (BF16, 300, 4099, 1 << 20), (F32, 5, 300, 7)])
+def test_scratch_of_a_call_that_names_no_piece(dt, N, D, V):
+    """Everything that grows with the piece stays within 256 MB (2048 rows at least), the eighth that saves one more piece, and the 256
+    rows that a piece is rounded up by, twice: logit gradients (float32: in both orders, of whole steps of tokens), the transposed copy of the weight's rows (float32) and the
+    copy of unaligned ones.  What does not grow with it: copies of hidden, and float32 sums of d_hidden (one, or partial ones:
+    512 tiles of 64 x 64, of more than 32 tokens 512 of 256 x 256) and likewise of a d_weight that is cut."""
+    import nerf_kinematics_amd as nk
+    from nerf_kinematics_amd import lib as nklib
+    L, es = nk.load(), dt.itemsize
+    up = lambda a, b: -(-a // b) * b
+    Dp, Np = up(D, 128 // es), up(N, 128 // es)
+    o = nklib.NkXentOpts(N, D, V, D, D, -100, nklib.DTYPES[dt], 1, 0)
+    unaligned = D * es % 16 != 0
+    row = Np * es * (2 if dt == F32 else 1) + (D * es if dt == F32 else 0) + (Dp * es if unaligned else 0)
+    fixed = N * Dp * es + D * Np * es + N * D * 4 + 2 * 512 * (256 * 256 if N > 32 else 64 * 64) * 4 + 16 * N + (1 << 16)
+    got = L.nk_linear_xent_workspace_bytes(o, 1024, 1024, 1)
+    assert 0 < got <= max(256 << 20, 2048 * row) * 9 / 8 + 2 * 256 * row + fixed, (got / 2**20, row, fixed / 2**20)
+    got = L.nk_linear_xent_workspace_bytes(o, 1024, 1024, 0)
+    assert 0 < got <= N * Dp * es + (V + 255) // 64 * N * 8 + 32 * N + (1 << 16) + (((288 << 20) + 512 * Dp * es) if unaligned else 0)
