@@ -100,7 +100,8 @@ class AdamW:
     copies that the step updates instead, the parameters then receive them rounded; low-precision
     parameters without masters lose updates below half their last place.  ``state_bits``: 32 or 8.
     ``state``: moments to continue from, as ``adamw_state`` lays them out (their dtype decides the format); they
-    stay the optimiser's, load into them with ``copy_``.  Parameters and masters may move (``p.data = ...``)."""
+    stay the optimiser's, load into them with ``copy_``.  Parameters and masters may move (``p.data = ...``), and ``lr``, ``betas``,
+    ``eps`` and ``weight_decay`` may be assigned: a step takes them as they are then."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, masters: Optional[Sequence[torch.Tensor]] = None,
@@ -137,7 +138,6 @@ class AdamW:
         self._bind()
         self._opts = _lib.NkAdamwOpts()
         self._opts.param_dtype, self._opts.state_bits = _lib.DTYPES[dt], state_bits
-        self._opts.beta1, self._opts.beta2, self._opts.eps = self.betas[0], self.betas[1], self.eps
 
     def _bind(self) -> None:
         """Checks every tensor and lays down the launch table."""
@@ -199,7 +199,7 @@ class AdamW:
             raise ValueError(f"step={step}: from 1")
         o = self._opts
         o.grad_dtype, o.step, o.lr, o.weight_decay = _lib.DTYPES[gd], step, self.lr if lr is None else float(lr), self.weight_decay
-        o.grad_scale = float(grad_scale)
+        (o.beta1, o.beta2), o.eps, o.grad_scale = self.betas, self.eps, float(grad_scale)
         o.seed = (self.seed + 0x9E3779B1 * step if seed is None else int(seed)) & 0xFFFFFFFF
         o.state = step_state
         _lib.launch(self.device, self._L.nk_adamw_step, self._table, n, o)
