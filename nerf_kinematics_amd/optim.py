@@ -204,7 +204,7 @@ class AdamW:
         o.state = step_state
         _lib.launch(self.device, self._L.nk_adamw_step, self._table, n, o)
         self.steps = step
-        _increment_version(self.params)         # autograd refuses to use what it saved of them before
+        _increment_version(self._owned)         # autograd refuses to use what it saved of them before
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],

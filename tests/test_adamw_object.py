@@ -35,3 +35,17 @@ def test_settings_changed_between_steps(bits):
             opt.step(g2)
         setattr(opt, name, keep)
         assert all(torch.equal(a, b) for a, b in zip(p, was)) and opt.steps == 2
+
+
+@gpu
+def test_autograd_notices_that_masters_changed():
+    """A master is updated in place as a parameter is: what autograd saved of either must not be used afterwards."""
+    import nerf_kinematics_amd as nk
+    dev = torch.device("cuda:0")
+    w = torch.randn(40, device=dev, requires_grad=True)
+    p = w.detach().bfloat16()
+    opt = nk.AdamW([p], 1e-2, masters=[w])
+    loss = (w * w).sum()
+    opt.step([torch.ones(40, device=dev)])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
