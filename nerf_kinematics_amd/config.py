@@ -9,6 +9,7 @@ reference loads here unchanged; missing keys take the values of the lego file.
 from __future__ import annotations
 
 import copy
+import math
 from typing import Any, Dict, Optional
 
 import yaml
@@ -56,6 +57,14 @@ def _merge(base: dict, over: dict, path: str = "") -> dict:
     return out
 
 
+def _number(value: Any) -> float:
+    """A number, also one that YAML took for text (1e-2); NaN for anything else."""
+    try:
+        return float(value)
+    except (TypeError, ValueError):
+        return math.nan
+
+
 def validate(cfg: dict) -> dict:
     """Reject what the HIP render path cannot run, naming the key (plain ValueError subclass,
     raised before anything touches the GPU)."""
@@ -96,9 +105,9 @@ def validate(cfg: dict) -> dict:
     if opt.get("type", "Adam") not in ("Adam", "AdamW"):
         raise ConfigError(f"optimizer.type: Adam or AdamW, got {opt['type']!r}")
     if opt.get("type", "Adam") == "AdamW":
-        if int(opt.get("state_bits", 32)) not in (32, 8):
+        if _number(opt.get("state_bits", 32)) not in (32, 8):
             raise ConfigError(f"optimizer.state_bits: 32 or 8, got {opt['state_bits']!r}")
-        if not float(opt.get("weight_decay", 0.01)) >= 0.0:
+        if not 0.0 <= _number(opt.get("weight_decay", 0.01)) < math.inf:
             raise ConfigError(f"optimizer.weight_decay: >= 0, got {opt['weight_decay']!r}")
     if cfg["dataset"]["type"] not in ("blender", "robot", "transforms", "teacher", "forward_grid"):
         raise ConfigError(f"dataset.type: unknown dataset type {cfg['dataset']['type']!r}")

@@ -52,6 +52,9 @@ class TrainOpts:
     def from_config(cfg: dict) -> "TrainOpts":
         t = cfg.get("nerf", {}).get("train", {})
         o, s = cfg.get("optimizer", {}), cfg.get("scheduler", {})
+        more = {}
+        if o.get("type", "Adam") == "AdamW":        # Adam does not read these: its files may hold anything there
+            more = dict(weight_decay=float(o.get("weight_decay", 0.01)), state_bits=int(float(o.get("state_bits", 32))))
         return TrainOpts(num_coarse=int(t.get("num_coarse", 64)), num_fine=int(t.get("num_fine", 128)),
                          num_random_rays=int(t.get("num_random_rays", 1024)), perturb=bool(t.get("perturb", True)),
                          lindisp=bool(t.get("lindisp", False)),
@@ -59,8 +62,7 @@ class TrainOpts:
                          white_background=bool(t.get("white_background", False)), lr=float(o.get("lr", 5e-4)),
                          lr_decay=int(s.get("lr_decay", 250)), lr_decay_factor=float(s.get("lr_decay_factor", 0.1)),
                          seed=int(cfg.get("experiment", {}).get("randomseed", 42)),
-                         act_format=str(t.get("act_format", "bf16")), optimizer=str(o.get("type", "Adam")),
-                         weight_decay=float(o.get("weight_decay", 0.01)), state_bits=int(o.get("state_bits", 32)))
+                         act_format=str(t.get("act_format", "bf16")), optimizer=str(o.get("type", "Adam")), **more)
 
 
 def lr_at(iteration: int, o: TrainOpts) -> float:
