@@ -279,6 +279,13 @@ int nk_linear_xent_fwd(const nk_xent_opts* opts /*host*/, const void* hidden, co
 int nk_linear_xent_bwd(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, const int64_t* target,
                        const float* lse, const float* d_loss, void* d_hidden, void* d_weight, void* workspace,
                        int64_t workspace_bytes, void* stream);
+/* Diagnostic: how the products of calls on these operands are cut, with both gradients wanted.  cuts[0] the logits of
+ * the forward call, cuts[1] the logit gradients, cuts[2] d_weight and cuts[3] d_hidden of piece `piece` of the backward call: an
+ * NK_TILE_*, plus 16 times the stretches of k that are summed in fp32 afterwards (0: the product leaves its
+ * result by itself; a d_hidden over several pieces has one stretch at least).  Returns the number of pieces.  */
+enum { NK_TILE_256x256 = 0, NK_TILE_128x128 = 1, NK_TILE_128x32 = 2, NK_TILE_64x64 = 3 };
+int64_t nk_linear_xent_cuts(const nk_xent_opts* opts /*host*/, const void* hidden, const void* weight, int64_t piece,
+                            int32_t cuts[4] /*host*/);
 
 /* AdamW (torch.optim.AdamW's update, decoupled weight decay) over many tensors in one launch per 56 of
  * them.  No counterpart in the reference, whose optimiser is Adam on fp32 parameters.

@@ -811,7 +811,7 @@ int start(int64_t blocks, int threads, hipStream_t st, const char* name, const A
 }
 
 // Which tile for an M x N product cut into `slices` stretches of k: the largest that still fills the 256 CUs.
-enum { LARGE = 0, MIDDLE = 1, FEW = 2, SMALL = 3 };
+enum { LARGE = NK_TILE_256x256, MIDDLE = NK_TILE_128x128, FEW = NK_TILE_128x32, SMALL = NK_TILE_64x64 };
 int tile_kind(int64_t M, int64_t N, int64_t slices = 1) {
     if (N <= 32) return FEW;
     if (cdiv(M, 256) * cdiv(N, 256) * slices >= 224) return LARGE;
@@ -1113,6 +1113,21 @@ extern "C" int64_t nk_linear_xent_workspace_bytes(const nk_xent_opts* o, const v
     Plan p;
     const int rc = plan_of(o, hidden, weight, backward, &p, "nk_linear_xent_workspace_bytes");
     return rc < 0 ? rc : p.total;
+}
+
+extern "C" int64_t nk_linear_xent_cuts(const nk_xent_opts* o, const void* hidden, const void* weight, int64_t piece, int32_t* cuts) {
+    Plan f, b;
+    int rc = plan_of(o, hidden, weight, 0, &f, "nk_linear_xent_cuts");
+    if (rc < 0 || (rc = plan_of(o, hidden, weight, 1, &b, "nk_linear_xent_cuts")) < 0) return rc;
+    const int64_t pieces = cdiv(o->V, b.piece);
+    if (!cuts || o->N < 1 || piece < 0 || piece >= pieces) NK_FAIL(NK_ERR_ARG, "nk_linear_xent_cuts: no tokens, or no piece %lld of %lld", (long long)piece, (long long)pieces);
+    const int64_t v0 = piece * b.piece, rows = o->V - v0 < b.piece ? o->V - v0 : b.piece;
+    const int cut = (int)cut_of(o->D, rows, b.Np, 128 / elem(o->dtype));
+    cuts[0] = f.kind;
+    cuts[1] = tile_kind(rows, o->N);
+    cuts[2] = tile_kind(o->D, rows, cut) + 16 * (cut > 1 ? cut : 0);
+    cuts[3] = tile_kind(o->D, o->N, b.slices) + 16 * (b.slices > 1 || pieces > 1 ? b.slices : 0);
+    return pieces;
 }
 
 extern "C" int nk_linear_xent_fwd(const nk_xent_opts* o, const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,

@@ -103,6 +103,7 @@ SIGNATURES = {
     "nk_set_step_state": (C.c_int, [C.POINTER(NkStepState), _P, _P]),
     "nk_adam_step_dev": (C.c_int, [_P, _P, _P, _P, _I64, _P, C.c_double, C.c_double, C.c_double, _F, _P]),
     "nk_linear_xent_workspace_bytes": (_I64, [C.POINTER(NkXentOpts), _P, _P, C.c_int]),
+    "nk_linear_xent_cuts": (_I64, [C.POINTER(NkXentOpts), _P, _P, _I64, C.POINTER(C.c_int32)]),
     "nk_linear_xent_fwd": (C.c_int, [C.POINTER(NkXentOpts), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "nk_linear_xent_bwd": (C.c_int, [C.POINTER(NkXentOpts), _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "nk_gated_scan_workspace_bytes": (_I64, [C.POINTER(NkScanOpts), C.c_int]),
