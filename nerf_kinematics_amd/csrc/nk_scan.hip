@@ -613,7 +613,6 @@ struct Shape {
 
 inline int ceil_log2(int64_t x) { int k = 0; while (((int64_t)1 << k) < x) ++k; return k; }
 inline int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
-inline int elem(int dt) { return dt == NK_F32 ? 4 : 2; }
 
 // The variant for a shape.
 void shape_of(const nk_scan_opts* o, int bwd, Shape* s) {

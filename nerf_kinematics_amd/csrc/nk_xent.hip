@@ -289,7 +289,7 @@ NK_D void tile_of(int64_t id, int64_t mt, int64_t nt, int64_t* m, int64_t* n) {
 // ---- forward ----------------------------------------------------------------------------------
 struct LseArgs {
     Mat w, h;
-    int64_t kbytes, v0, V, N;              // rows v0 .. of the vocabulary are w's rows 0 ..
+    int64_t kbytes, v0, N;                 // rows v0 .. of the vocabulary are w's rows 0 ..
     const int64_t* target;
     float2* part; int64_t part0;            // [tile of vocabulary][token]: maximum, sum of exponentials
     float* zt;                              // logit of the target
@@ -784,8 +784,8 @@ template <typename T> __global__ __launch_bounds__(256) void k_xent_transpose(co
 template <typename T> __global__ __launch_bounds__(256) void k_xent_prepare(const FactorArgs f, const CopyArgs a, const CopyArgs b) {
     const int64_t block = (int64_t)blockIdx.x - 1;
     if (block < 0) factors<256>(f, 0, 1);
-    else if (block < a.blocks) { if (BOTH_ORDERS<T>) transpose_block<T>(a, block); else pad_block<T>(a, block); }
-    else if (BOTH_ORDERS<T>) transpose_block<T>(b, block - a.blocks);
+    else if constexpr (BOTH_ORDERS<T>) { if (block < a.blocks) transpose_block<T>(a, block); else transpose_block<T>(b, block - a.blocks); }
+    else if (block < a.blocks) pad_block<T>(a, block);
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -983,7 +983,7 @@ int forward(const nk_xent_opts* o, const Plan& p, const void* hidden, const void
             if ((rc = pad<T>(pad_of<T>(src, o->weight_stride, rows, o->D, nullptr, 0, ws + p.w, p.Dp), st)) < 0) return rc;
             w = Mat{ws + p.w, rows, p.Dp * es, p.Dp * es};
         }
-        const LseArgs g = {w, h, o->D * es, v0, o->V, o->N, target, (float2*)(ws + p.parts), tiles, (float*)(ws + p.zt)};
+        const LseArgs g = {w, h, o->D * es, v0, o->N, target, (float2*)(ws + p.parts), tiles, (float*)(ws + p.zt)};
         if ((rc = lse_launch<T>(p.kind, g, st)) < 0) return rc;
         tiles += cdiv(rows, kind_bm(p.kind));
     }
@@ -1042,7 +1042,7 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
         if ((!few || BOTH) && (rc = pad<T>(clean, st)) < 0) return rc;
         h = Mat{ws + p.h, o->N, p.Dp * es, p.Dp * es};
     }
-    if (BOTH && d_weight && !few && (rc = transpose<T>(ht, st)) < 0) return rc;
+    if constexpr (BOTH) { if (d_weight && !few && (rc = transpose<T>(ht, st)) < 0) return rc; }
     const int64_t slice = up(cdiv(p.piece, p.slices), 128 / es) * es;
     const bool direct = p.slices == 1 && one;      // d_hidden in one product: no sums to keep
     for (int64_t v0 = 0; v0 < o->V; v0 += p.piece) {
@@ -1067,7 +1067,7 @@ int backward(const nk_xent_opts* o, const Plan& p, const void* hidden, const voi
             else { qw.kslice = up(cdiv(p.Np, cut), 128 / es) * es; qw.sums = (float*)(ws + p.wsums); }
         }
         if (d_hidden) {
-            if (BOTH) {
+            if constexpr (BOTH) {
                 if (!few && (rc = transpose<T>(transpose_of<T>(src, o->weight_stride, rows, o->D, nullptr, 0, ws + p.wt, kv), st)) < 0) return rc;
                 qh.a = Mat{ws + p.wt, o->D, kv * es, 0};
             } else {
