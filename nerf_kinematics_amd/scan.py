@@ -20,11 +20,12 @@ _KEEP = 32              # the forward pass of a training step keeps the state in
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, T, n] with unit stride along n and no negative strides (a copy where it has neither)."""
     sb, st, sc = t.stride()
-    return t if (sc == 1 or t.shape[2] == 1) and sb >= 0 and st >= 0 else t.contiguous()
+    return t if (sc == 1 or t.shape[2] == 1) and sb >= 0 and st >= 0 and not t.is_neg() else t.contiguous().resolve_neg()
 
 
 def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()
+    """`t` contiguous, with its values in memory as they are (torch negates the imaginary part of a conjugate lazily)."""
+    return None if t is None else t.contiguous().resolve_neg()
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -107,8 +108,7 @@ class _GatedScan(torch.autograd.Function):
         dev = x.device
         if d_h is None and d_last is None:
             return None, None, None, None, None
-        if d_last is not None:
-            d_last = d_last.contiguous()
+        d_last = _whole(d_last)
         if B == 0 or T == 0:
             z = lambda t, want: torch.zeros_like(t) if want else None
             d_0 = None
@@ -125,6 +125,14 @@ class _GatedScan(torch.autograd.Function):
         _lib.launch(dev, L.nk_gated_scan_bwd, o, a.data_ptr(), x.data_ptr(), _ptr(states), _ptr(h0), _ptr(g), _ptr(d_last),
                     _ptr(d_a), _ptr(d_x), _ptr(d_0), _ptr(ws), n)
         return d_a, d_x, d_0, None, None
+
+
+def _call(a, x, h0, lengths, reverse):
+    """The operator on checked arguments."""
+    a, x, h0, lengths = _rows(a), _rows(x), _whole(h0), _whole(lengths)
+    if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _GatedScan.apply(a, x, h0, lengths, reverse)
+    return _forward(a, x, h0, lengths, reverse, False)[:2]
 
 
 def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *, lengths: Optional[torch.Tensor] = None,
@@ -158,12 +166,7 @@ def gated_scan(a: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = No
     if h0 is not None:
         if h0.dtype != torch.float32 or h0.shape != (B, C) or h0.device != dev:
             raise ValueError(f"h0: expected a float32 tensor of shape {(B, C)} on {dev}")
-        h0 = h0.contiguous()
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.shape != (B,) or lengths.device != dev:
             raise ValueError(f"lengths: expected an int32 tensor of shape {(B,)} on {dev}")
-        lengths = lengths.contiguous()
-    a, x = _rows(a), _rows(x)
-    if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(a, x, h0, lengths, int(reverse))
-    return _forward(a, x, h0, lengths, int(reverse), False)[:2]
+    return _call(a, x, h0, lengths, int(reverse))

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _kinds, _like, _no_tangents, _ptr, _unpacked
+from .scan import _kinds, _like, _no_tangents, _ptr, _unpacked, _whole
 
 
 def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
@@ -30,7 +30,7 @@ _TOKENS32 = 1 << 20     # and tokens of a backward pass in float32
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with unit stride along its rows, which neither overlap nor lie further apart than the library takes (a copy where they do)."""
-    return t if t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= _FAR // t.element_size() else t.contiguous()
+    return t if t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= _FAR // t.element_size() and not t.is_neg() else _whole(t)
 
 
 def _forward(hidden, weight, target, o, reduction):
@@ -69,12 +69,20 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if hidden.shape[0] == 0:
             return d_hidden, torch.zeros_like(weight) if want_w else None, None, None, None, None
         d_weight = _like(weight) if want_w else None
-        d_loss = d_loss.contiguous()
+        d_loss = _whole(d_loss)
         L = _lib.load()
         ws, n = _workspace(L, o, hidden, weight, 1)
         _lib.launch(dev, L.nk_linear_xent_bwd, o, hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), lse.data_ptr(),
                     d_loss.data_ptr(), _ptr(d_hidden), _ptr(d_weight), ws.data_ptr(), n)
         return d_hidden, d_weight, None, None, None, None
+
+
+def _call(hidden, weight, target, ignore_index, reduction, piece):
+    """The operator on checked arguments."""
+    hidden, weight, target = _rows(hidden), _rows(weight), target.contiguous()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(hidden, weight, target, ignore_index, reduction, piece)
+    return _forward(hidden, weight, target, _opts(hidden, weight, ignore_index, reduction, piece), reduction)[0]
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
@@ -105,16 +113,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if piece < 0:
         raise ValueError(f"piece={piece} (>= 0)")
     _no_tangents(hidden, weight)
-    training = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
-    if training and N > _TOKENS32 and hidden.dtype == torch.float32:
+    if N > _TOKENS32 and hidden.dtype == torch.float32 and torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         raise ValueError(f"hidden: float32 gradients of up to {_TOKENS32} tokens a call, got {N}")
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("hidden: expected a GPU tensor (there is no CPU implementation)")
     if weight.device != dev or target.device != dev:
         raise ValueError(f"weight, target: expected tensors on {dev}")
-    hidden, weight, target = _rows(hidden), _rows(weight), target.contiguous()
-    r = _lib.REDUCTIONS[reduction]
-    if training:
-        return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), r, int(piece))
-    return _forward(hidden, weight, target, _opts(hidden, weight, int(ignore_index), r, int(piece)), r)[0]
+    return _call(hidden, weight, target, int(ignore_index), _lib.REDUCTIONS[reduction], int(piece))
