@@ -38,6 +38,8 @@ def _check_list(name: str, tensors: Sequence[torch.Tensor], numels: Sequence[int
             raise ValueError(f"{name}[{i}]: {t.numel()} elements, expected {numels[i]}")
         if not t.is_contiguous():
             raise ValueError(f"{name}[{i}]: must be contiguous")
+        if t.is_neg():          # its memory holds the opposite sign
+            raise ValueError(f"{name}[{i}]: is negated lazily (an imaginary part of a conjugate): resolve_neg() it")
         at = t.data_ptr()
         out.append(at)
         if numels[i]:
@@ -133,6 +135,7 @@ class AdamW:
         self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
         self.device, self._dtype = dev, dt
         self._numels, self._indices = [p.numel() for p in params], [dev.index] * len(params)
+        self._single = [i for i, n in enumerate(self._numels) if n == 1]       # alone can be contiguous and an imaginary part of a conjugate
         self._owned = self.params + (self.masters or ())
         self._held = [t.detach() for t in (*m, *v, *(s for pair in scales or () for s in pair))]       # the table's moments, whatever becomes of `state`
         self._bind()
@@ -193,6 +196,9 @@ class AdamW:
             if any(g is None for g in grads):
                 raise ValueError("AdamW.step: a parameter has no .grad")
         self._words[1::_TENSOR_WORDS] = self._check_grads(grads)
+        if any(grads[i].is_neg() for i in self._single):        # the memory of such a view holds the opposite sign
+            grads = [g.resolve_neg() for g in grads]
+            self._words[1::_TENSOR_WORDS] = list(map(_address, grads))
         gd = grads[0].dtype
         step = self.steps + 1 if step is None else int(step)
         if step < 1:

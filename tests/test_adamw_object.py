@@ -49,3 +49,33 @@ def test_autograd_notices_that_masters_changed():
     opt.step([torch.ones(40, device=dev)])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def lazily(t):
+    """`t` as the imaginary part of a conjugate: the same values, negated lazily."""
+    out = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert out.is_neg()
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)])
+def test_gradients_that_torch_negates_lazily(shape):
+    """Only a tensor of one element can be both such a view and contiguous; autograd leaves such a .grad behind a complex loss."""
+    import nerf_kinematics_amd as nk
+    dev = torch.device("cuda:0")
+    start = lambda: [torch.ones(5, device=dev), torch.full(shape, 2.0, device=dev, requires_grad=True)]
+    p, q = start(), start()
+    torch.complex(torch.full(shape, 3.0, device=dev), p[1]).conj().abs().sum().backward()
+    assert p[1].grad.is_neg() and float(p[1].grad) > 0
+    p[0].grad = torch.ones(5, device=dev)
+    nk.AdamW(p, 1e-2).step()
+    nk.AdamW(q, 1e-2).step([torch.ones(5, device=dev), p[1].grad.clone().resolve_neg()])
+    assert all(torch.equal(a, b) for a, b in zip(p, q)) and float(p[1].detach()) < 2.0
+
+
+def test_parameters_that_torch_negates_lazily_are_refused():
+    from nerf_kinematics_amd.optim import _check_list
+    for t in (lazily(torch.ones(())), lazily(torch.ones(1))):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            _check_list("params", [torch.ones(3), t], [3, 1], torch.float32, t.device, [])
