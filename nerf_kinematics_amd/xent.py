@@ -8,15 +8,17 @@ from __future__ import annotations
 import torch
 
 from . import lib as _lib
-from .scan import _kinds, _like, _no_tangents, _ptr, _unpacked, _whole
+from .scan import _given, _layout, _like, _no_tangents, _once, _ptr, _unpacked, _whole
 
 
-def _opts(hidden, weight, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
-    N, D = hidden.shape
-    V = weight.shape[0]
+def _options(layout, ignore_index, reduction, piece) -> "_lib.NkXentOpts":
+    (N, D), (V, _), (sh, _), (sw, _), dt, _ = layout
     # a dimension of one row has any stride
-    return _lib.NkXentOpts(N, D, V, hidden.stride(0) if N > 1 else D, weight.stride(0) if V > 1 else D, ignore_index,
-                           _lib.DTYPES[hidden.dtype], reduction, piece)
+    return _lib.NkXentOpts(N, D, V, sh if N > 1 else D, sw if V > 1 else D, ignore_index, _lib.DTYPES[dt], reduction, piece)
+
+
+def _opts(hidden, weight, *more) -> "_lib.NkXentOpts":
+    return _options(_layout(hidden, weight), *more)
 
 
 def _workspace(L, o, hidden, weight, backward):
@@ -35,7 +37,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _forward(hidden, weight, target, o, reduction):
     L = _lib.load()
-    N, dev = hidden.shape[0], hidden.device
+    N, dev = o.N, hidden.device
     ws, n = _workspace(L, o, hidden, weight, 0)
     if reduction:       # the losses of the tokens, which nobody asked for, lie behind lse
         lse, out = torch.empty(2 * N, dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
@@ -51,18 +53,22 @@ def _forward(hidden, weight, target, o, reduction):
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction, piece):
-        ctx.options = ignore_index, reduction, piece
-        loss, lse = _forward(hidden, weight, target, _opts(hidden, weight, *ctx.options), reduction)
+        ctx.layout = _layout(hidden, weight)
+        ctx.opts = o = _options(ctx.layout, ignore_index, reduction, piece)
+        loss, lse = _forward(hidden, weight, target, o, reduction)
         ctx.save_for_backward(hidden, weight, target, lse)
-        ctx.kinds = _kinds((hidden, weight, target, lse))
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_loss):
-        hidden, weight, target, lse = _unpacked(ctx)
-        hidden, weight, target, lse = _rows(hidden), _rows(weight), target.contiguous(), lse.contiguous()
-        o = _opts(hidden, weight, *ctx.options)
+        saved = ctx.saved_tensors
+        hidden, weight, layout = _unpacked(ctx, _rows, saved, d_loss)
+        o = ctx.opts
+        if layout is not ctx.layout:
+            o = _options(layout, o.ignore_index, o.reduction, o.piece)
+        target = _given(saved[2], torch.int64, o.N, hidden)
+        lse = _given(saved[3], torch.float32, 2 * o.N if o.reduction else o.N, hidden)
         dev = hidden.device
         want_h, want_w = ctx.needs_input_grad[:2]
         d_hidden = _like(hidden) if want_h else None
@@ -106,7 +112,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if not isinstance(hidden, torch.Tensor) or hidden.dim() != 2 or hidden.dtype not in _lib.DTYPES or hidden.shape[1] < 1:
         raise ValueError("hidden: expected a [N, D] tensor of float32, bfloat16 or float16")
     N, D = hidden.shape
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != D or weight.shape[0] < 1 or weight.dtype != hidden.dtype:
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype != hidden.dtype or weight.numel() == 0 or weight.shape[1] != D:
         raise ValueError(f"weight: expected a [V, {D}] tensor of {hidden.dtype}")
     if not isinstance(target, torch.Tensor) or target.dtype != torch.int64 or target.shape != (N,):
         raise ValueError(f"target: expected an int64 tensor of shape {(N,)}")

@@ -46,3 +46,18 @@ def test_functional_jvp_is_refused():
         torch.func.jvp(lambda y: nk.gated_scan(a, y)[0], (x,), (x,))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda y: nk.linear_cross_entropy(y, w, t), (x[:, 0],), (x[:, 0],))
+
+
+def test_second_derivatives_are_refused(monkeypatch):
+    """create_graph=True gives first gradients that cannot be differentiated again."""
+    from nerf_kinematics_amd import lib
+    from nerf_kinematics_amd.scan import _GatedScan
+    from nerf_kinematics_amd.xent import _LinearCrossEntropy
+    monkeypatch.setattr(lib, "launch", lambda *args: None)
+    a, x = torch.rand(2, 3, 4, requires_grad=True), torch.randn(2, 3, 4, requires_grad=True)
+    h, w = torch.randn(4, 8, requires_grad=True), torch.randn(5, 8, requires_grad=True)
+    for out, inp in ((_GatedScan.apply(a, x, None, None, 0)[0], x), (_LinearCrossEntropy.apply(h, w, torch.zeros(4, dtype=torch.int64), -100, 0, 0), h)):
+        weight = torch.ones_like(out, requires_grad=True)
+        (g,) = torch.autograd.grad(out, inp, weight, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
