@@ -219,7 +219,8 @@ enum { NK_F32 = 0, NK_BF16 = 1, NK_F16 = 2 };
  * front-to-back compositing of raw2outputs is the case a = 1 - alpha, x = alpha * colour, reverse, one gate.
  * States and sums are fp32; h is rounded once to its type.  h0 [B, C] (NULL = zero) is the state before the
  * first step, h_last [B, C] (NULL = unwanted) the one after the last.  Gates are meant to decay (|a| <= 1);
- * growing ones work as long as the product of the gates over any stretch stays in the range of fp32.
+ * growing ones work as long as the product of the gates over any stretch stays in the range of fp32.  Behind
+ * an infinite state a product of gates that has fallen to zero may make NaN where step by step infinity would stay.
  *   lengths   NULL, or B device ints: sequence b has clamp(lengths[b], 0, T) steps.  Rows behind it are not read;
  *             the outputs there (h, d_a, d_x) are zero, and a reversed sequence starts at its own last step.
  * a, x and d_h may be strided over B and T, with unit channel stride; strides

@@ -10,7 +10,7 @@
 // again from its own start state, out of registers.  State, products and sums are fp32 throughout.
 //
 // A workgroup holds 2^LC columns x (256 >> LC) runs of SC_U steps ("a tile") and walks along the sequence
-// tile by tile, so every input is read once.  The forward pass of a training step keeps the fp32 state in
+// tile by tile, so a sequence that one workgroup walks whole has every input read once.  The forward pass of a training step keeps the fp32 state in
 // front of every 32nd step; the backward pass walks the tiles from the last to the first and rebuilds the
 // states inside a tile from these and x, which costs no more bytes than reading h and keeps dL/da free
 // of the rounding of h.

@@ -3,7 +3,8 @@
 Stands beside :func:`~nerf_kinematics_amd.render.adam_step` (Adam on flat fp32 buffers, the optimiser of
 the reference's checkpoints).  ``adamw_step`` updates lists of tensors once; :class:`AdamW` keeps the
 moments of a list of parameters and the launch table a program reuses.  Everything runs on the current
-torch stream of the tensors' GPU; bad shapes, types or overlaps raise ``ValueError`` before any launch.
+torch stream of the tensors' GPU; bad shapes, types or overlaps of parameters, masters and moments raise ``ValueError`` before any
+launch (that gradients share no memory with what a step writes is the caller's to see to).
 
 8-bit moments: blocks of 256 consecutive elements of a tensor share a power-of-two fp32 scale; an element
 is ``code * scale`` with an OCP e4m3 code (first moment) or e5m2 code (second moment).

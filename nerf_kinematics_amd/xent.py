@@ -102,7 +102,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
     Differentiable in ``hidden`` and ``weight`` (first order, reverse mode).  The backward pass walks the vocabulary in pieces
     of ``piece`` rows (default: as many as keep a piece's scratch near 256 MB, 2048 at least) and rounds the logit gradients once to
-    the operands' dtype between its products; sums are float32.
+    the operands' dtype between its products (float16: those below 2^-38 of the largest finite ``|d_loss|`` vanish); sums are
+    float32.
 
     A call takes D up to 2^20, V up to 2^26 and N up to 2^24 (float32 with gradients: 2^20).  Rows of any layout are taken; those that
     overlap, are strided inside or lie more than 2^22 bytes apart are copied.
