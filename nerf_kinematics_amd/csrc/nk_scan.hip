@@ -26,12 +26,12 @@
 //   8 steps a run against 4: 123 / 146 us and 312 / 375 us.
 //   Short sequences pay for what happens once a workgroup: the longest length by lane shifts and not by an LDS
 //   atomic, and rows walked by pointer (multiples of five strides no longer fill the scalar registers), took
-//   4096 x 192 x 64 from 123 to 98 us (31 forward, 67 backward; its bytes cost 75).
+//   4096 x 192 x 64 from 123 to 98 us (31 forward, 67 backward; its bytes cost 64 at 5.55 TB/s).
 //   Loading the next tile ahead in the backward pass costs registers and loses (280 against 164 us); in the
 //   forward pass it gains.
 // 2 x 32768 x 1024 in bf16 then takes 124 us forward (53 of them the first launch, 5.1 TB/s; the walk
-// moves 5.6 TB/s with the first launch's reads partly cached) and 184 us backward, against 169 us that the bytes of
-// one pass over every tensor cost; reading a and x (a and g) twice is what is left.
+// moves 5.6 TB/s with the first launch's reads partly cached) and 184 us backward, against 145 us that the bytes of
+// one pass over every tensor cost at 5.55 TB/s; reading a and x (a and g) twice is what is left.
 #include "nk_common.h"
 
 namespace {
