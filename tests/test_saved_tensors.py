@@ -180,3 +180,23 @@ def test_scan_gradients_under_hooks(J, hook):
         leaves, out = run()
     got = torch.autograd.grad(out, leaves, (d, dl))
     assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(bool(p.any()) for p in want)
+
+
+@gpu
+def test_gradients_under_recomputation():
+    """torch's checkpoint hands a backward pass the tensors of a second forward pass."""
+    import nerf_kinematics_amd as nk
+    from torch.utils.checkpoint import checkpoint
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)
+    alpha, feats, head, labels = torch.sigmoid(r(60, 70, 1)), r(60, 70, 96), r(300, 48) / 7, torch.randint(0, 300, (60,), generator=g, device=dev)
+
+    def loss(a, x, w):
+        return nk.linear_cross_entropy(nk.gated_scan(1 - a, a * x[:, :, 48:], reverse=True)[1], w, labels)
+
+    def run(f):
+        leaves = [t.clone().requires_grad_(True) for t in (alpha, feats, head)]
+        return torch.autograd.grad(f(*leaves), leaves)
+    want, got = run(loss), run(lambda *t: checkpoint(loss, *t, use_reentrant=False))
+    assert all(torch.equal(p, q) for p, q in zip(want, got)) and all(bool(p.any()) for p in want)
